@@ -11,7 +11,7 @@ import threading
 from . import build as _build
 
 # constants mirrored from include/chronicals_cce.h
-CCE_ABI_VERSION = 7
+CCE_ABI_VERSION = 8
 CCE_OK = 0
 CCE_ERR_INVALID_ARG = 1
 CCE_ERR_WORKSPACE = 2
@@ -27,6 +27,7 @@ CCE_SMOOTH_UNIFORM = 1
 CCE_LSE_ALL_ROWS = 0
 CCE_LSE_LABELLED_ROWS = 1
 CCE_NOALLOC_SCRATCH_BYTES = 64 << 20
+CCE_MAX_TEACHER_ENTRIES = 256
 
 CCE_KERNEL_FWD_LSE = 0
 CCE_KERNEL_BWD_GRAD = 1
@@ -50,6 +51,16 @@ _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
 _f32 = ctypes.c_float
 _sz = ctypes.c_size_t
+
+
+class Teacher(ctypes.Structure):
+    """cce_teacher"""
+    _fields_ = [("logits", _vp), ("indices", _vp), ("entries", _i64), ("logits_dtype", _i32), ("indices_int64", _i32),
+                ("temperature", _f32), ("distill_weight", _f32), ("ce_weight", _f32)]
+
+
+_teacher = ctypes.POINTER(Teacher)
+_size_out = ctypes.POINTER(_sz)
 
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -102,6 +113,44 @@ SIGNATURES = {
         _vp, _i32, _i64,                     # grad_logits, grad_dtype, ld_grad
         _vp, _sz, _vp,                       # workspace, workspace_bytes, stream
     ]),
+    "cce_distill_logits_workspace_bytes": (_i32, [_i64, _i64, _i32, _size_out]),
+    "cce_distill_logits_forward": (_i32, [
+        _vp, _i32, _i64, _teacher, _vp, _i32,  # logits, dtype, ld, teacher, labels, labels_int64
+        _i64, _i64, _i64, _i32,              # N, V, ignore_index, reduction
+        _vp, _vp, _vp,                       # loss_out, stats_out, n_valid_out
+        _vp, _sz, _vp,                       # workspace, workspace_bytes, stream
+    ]),
+    "cce_distill_logits_backward": (_i32, [
+        _vp, _vp, _i32, _i64, _teacher, _vp, _i32,  # grad_out, logits, dtype, ld, teacher, labels, labels_int64
+        _vp, _vp, _i64, _i64, _i64, _i32,    # stats, n_valid, N, V, ignore_index, reduction
+        _vp, _i64, _vp,                      # grad_logits, ld_grad, stream
+    ]),
+    "cce_distill_forward_workspace_bytes": (_i32, [_i64, _i64, _i64, _i32, _size_out]),
+    "cce_distill_forward": (_i32, [
+        _vp, _vp, _vp, _teacher, _vp, _i32,  # hidden, weight, bias, teacher, labels, labels_int64
+        _i64, _i64, _i64, _i64, _i32,        # N, d, V, ignore_index, reduction
+        _vp, _vp, _vp, _vp, _vp,             # loss_out, stats_out, entry_logits_out, rows_out, n_valid_out
+        _vp, _sz, _vp,                       # workspace, workspace_bytes, stream
+    ]),
+    "cce_distill_backward_workspace_bytes": (_i32, [_i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _size_out]),
+    "cce_distill_backward": (_i32, [
+        _vp, _vp, _vp, _vp, _teacher,        # grad_out, hidden, weight, bias, teacher
+        _vp, _vp, _vp, _vp,                  # stats, entry_logits, rows, n_valid
+        _i64, _i64, _i64, _i32, _i64,        # N, d, V, reduction, chunk_size
+        _vp, _i32, _vp, _i32, _vp,           # grad_hidden, dtype, grad_weight, dtype, grad_bias
+        _vp, _sz, _vp,                       # workspace, workspace_bytes, stream
+    ]),
+    "cce_top_logits": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "cce_layer_norm_forward": (_i32, [
+        _vp, _i32, _i64, _vp, _vp, _i32,     # x, dtype, ldx, weight, bias, param_dtype
+        _i64, _i64, _f32, _vp, _vp, _vp, _vp,  # N, D, eps, y_out, mean_out, rstd_out, stream
+    ]),
+    "cce_layer_norm_backward_workspace_bytes": (_i32, [_i64, _i64, _size_out]),
+    "cce_layer_norm_backward": (_i32, [
+        _vp, _vp, _i32, _i64, _vp, _i32,     # grad_y, x, dtype, ldx, weight, param_dtype
+        _vp, _vp, _i64, _i64,                # mean, rstd, N, D
+        _vp, _vp, _vp, _vp, _sz, _vp,        # grad_x, grad_weight, grad_bias, workspace, workspace_bytes, stream
+    ]),
     "cce_kernel_timing_enable": (_i32, [_i32]),
     "cce_kernel_timing_read": (_i32, [_i32, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(_i64),
                                       ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]),
@@ -127,7 +176,7 @@ def check_fresh(lib: ctypes.CDLL, path: str) -> None:
     its sources."""
     if os.path.abspath(path) != os.path.abspath(_build.LIB_PATH):
         return
-    if not (os.path.exists(_build.SRC) and os.path.exists(_build.HEADER)):
+    if not all(map(os.path.exists, (_build.SRC, _build.HEADER) + _build.PARTS)):
         return
     built = (lib.cce_source_hash() or b"").decode()
     want = _build.source_hash()

@@ -24,6 +24,9 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
 SRC = os.path.join(PKG_DIR, "csrc", "cce_kernels.hip")
 HEADER = os.path.join(REPO_DIR, "include", "chronicals_cce.h")
+# what SRC includes beside the header
+PARTS = tuple(os.path.join(PKG_DIR, "csrc", name)
+              for name in ("distill.h", "distill_linear.h", "layer_norm.h", "top_logits.h"))
 TORCH_SRC = os.path.join(PKG_DIR, "csrc", "torch_ops.cpp")
 LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_NAME = "libchronicals_cce.so"
@@ -41,11 +44,12 @@ def hipcc_path() -> str:
 
 
 def source_hash(paths=(SRC, HEADER)) -> str:
-    """SHA-256 (hex) over the files the library is compiled from, in order.
-    The build compiles it into the library (cce_source_hash()), so the loader
-    can tell a library built from other sources."""
+    """SHA-256 (hex) over the files the library is compiled from, in order, with
+    the parts that the kernel file includes.  The build compiles it into the
+    library (cce_source_hash()), so the loader can tell a library built from
+    other sources."""
     h = hashlib.sha256()
-    for p in paths:
+    for p in tuple(paths) + (PARTS if os.path.basename(SRC) in map(os.path.basename, paths) else ()):
         with open(p, "rb") as f:
             data = f.read()
         h.update(os.path.basename(p).encode() + b"\0" + str(len(data)).encode() + b"\0" + data)

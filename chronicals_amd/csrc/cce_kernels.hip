@@ -387,6 +387,8 @@ struct LseParams {
   float* pm;          // [splits][ldp] running max (log2 units)
   float* ps;          // [splits][ldp] sum of 2^(x - max)
   long ldp;           // row stride of pm / ps
+  float scale;        // log2(e) over a temperature (not with kOneSoftmax)
+  float* ps1;         // kTwoSoftmaxes: the same sums in units of log2(e)
   int splits;
   int tiles_n;
 };
@@ -406,14 +408,23 @@ __host__ __device__ inline float split_cost(int gl, int tn, int s, int ncu) {
 
 // Forward: per-row online (max, sum-exp) in base 2 over the workgroup's run of
 // vocabulary tiles; at the end one partial per (row, split) is written.
-template <int BN, bool HB>
+//
+// SM, the softmaxes that an epilogue computes: one of the logits, one at a
+// temperature (the launch's scale; as a parameter of the first kind too, it cost
+// the cross-entropy of 16384 x 896 x 151936 0.8%), or both.  With both the running maximum is kept in logits and starts at
+// kLogitFloor, whose products with either scale stay in range.
+constexpr int kOneSoftmax = 0, kAtTemperature = 1, kTwoSoftmaxes = 2;
+constexpr float kLogitFloor = -1e30f;
+
+template <int BN, bool HB, int SM = kOneSoftmax>
 struct EpiLseT {
+  static constexpr bool DU = SM == kTwoSoftmaxes;
   typedef LseParams Params;
   static constexpr bool kOneTile = false;
   static constexpr bool kDynSplits = true;
   static constexpr int FM = kFM;
   struct State {
-    float m[FM], s[FM];
+    float m[FM], s[FM], s1[DU ? FM : 1];
   };
   static __device__ inline void assign(const GemmShape& g, const Params& p, int bid, int nb, int& tm,
                                        int& t0, int& t1, int& split) {
@@ -432,8 +443,9 @@ struct EpiLseT {
   static __device__ inline void init(const Params&, State& st, const GemmShape&, int, int, int) {
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
-      st.m[i] = kNegBig;
+      st.m[i] = DU ? kLogitFloor : kNegBig;
       st.s[i] = 0.f;
+      if constexpr (DU) st.s1[i] = 0.f;
     }
   }
   static __device__ __forceinline__ void tile(const Params& p, State& st, WaveAcc<BN>& acc, const GemmShape& g, int tm,
@@ -441,20 +453,37 @@ struct EpiLseT {
     constexpr int FN = BN / 64;
     pin_epilogue(l, tm, tn);
     const int c0 = tn * BN;
-    // max over raw logits (log2e > 0 commutes with max), then one fused
-    // exp2(x*log2e - m) per element
+    const float scale = SM == kOneSoftmax ? kLog2e : p.scale;
+    // max over raw logits (the scale > 0 commutes with max), then one fused
+    // exp2(x*scale - m) per element and sum
     auto update = [&](int i, const f32x16 (&x)[FN]) {
       float mx = kNegBig;
 #pragma unroll
       for (int j = 0; j < FN; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, x[j][r]);
-      const float mn = fmaxf(st.m[i], mx * kLog2e);
+      if constexpr (DU) {
+        const float mn = fmaxf(st.m[i], mx), off = mn * scale, off1 = mn * kLog2e;
+        float sum = 0.f, sum1 = 0.f;
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            sum += fast_exp2(__builtin_fmaf(x[j][r], scale, -off));
+            sum1 += fast_exp2(__builtin_fmaf(x[j][r], kLog2e, -off1));
+          }
+        st.s[i] = st.s[i] * fast_exp2((st.m[i] - mn) * scale) + sum;
+        st.s1[i] = st.s1[i] * fast_exp2((st.m[i] - mn) * kLog2e) + sum1;
+        st.m[i] = mn;
+        __builtin_amdgcn_sched_barrier(0);
+        return;
+      }
+      const float mn = fmaxf(st.m[i], mx * scale);
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < FN; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sum += fast_exp2(__builtin_fmaf(x[j][r], kLog2e, -mn));
+        for (int r = 0; r < 16; ++r) sum += fast_exp2(__builtin_fmaf(x[j][r], scale, -mn));
       st.s[i] = st.s[i] * fast_exp2(st.m[i] - mn) + sum;
       st.m[i] = mn;
       __builtin_amdgcn_sched_barrier(0);
@@ -499,11 +528,23 @@ struct EpiLseT {
     s = s * fast_exp2(m - mn) + s2 * fast_exp2(m2 - mn);
     m = mn;
   }
+  // row block i with another partial of its rows
+  static __device__ inline void merge_row(const Params& p, State& st, int i, float m2, float s2, float s12) {
+    if constexpr (DU) {
+      const float mn = fmaxf(st.m[i], m2), a = st.m[i] - mn, b = m2 - mn;
+      st.s[i] = st.s[i] * fast_exp2(a * p.scale) + s2 * fast_exp2(b * p.scale);
+      st.s1[i] = st.s1[i] * fast_exp2(a * kLog2e) + s12 * fast_exp2(b * kLog2e);
+      st.m[i] = mn;
+    } else {
+      merge(st.m[i], st.s[i], m2, s2);
+    }
+  }
   static __device__ inline void finish(const Params& p, State& st, const GemmShape& g, int tm, int split,
                                        bf16_t* smem, int wm, int wn, int l) {
     // lanes l and l+32 hold the same rows
 #pragma unroll
-    for (int i = 0; i < FM; ++i) merge(st.m[i], st.s[i], __shfl_xor(st.m[i], 32), __shfl_xor(st.s[i], 32));
+    for (int i = 0; i < FM; ++i)
+      merge_row(p, st, i, __shfl_xor(st.m[i], 32), __shfl_xor(st.s[i], 32), DU ? __shfl_xor(st.s1[DU ? i : 0], 32) : 0.f);
     float* red = reinterpret_cast<float*>(smem);
     if (wn == 1 && l < 32) {
 #pragma unroll
@@ -511,6 +552,7 @@ struct EpiLseT {
         const int row = acc_row(wm, i, l);
         red[row] = st.m[i];
         red[kBM + row] = st.s[i];
+        if constexpr (DU) red[2 * kBM + row] = st.s1[i];
       }
     }
     __syncthreads();
@@ -518,12 +560,13 @@ struct EpiLseT {
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
         const int row = acc_row(wm, i, l);
-        merge(st.m[i], st.s[i], red[row], red[kBM + row]);
+        merge_row(p, st, i, red[row], red[kBM + row], DU ? red[2 * kBM + row] : 0.f);
         const int grow = tm * kBM + row;
         if (grow < g.M) {
           const long ldp = g.dyn == kDynM ? (long)(g.M + kBM - 1) / kBM * kBM : p.ldp;
           p.pm[(long)split * ldp + grow] = st.m[i];
           p.ps[(long)split * ldp + grow] = st.s[i];
+          if constexpr (DU) p.ps1[(long)split * ldp + grow] = st.s1[i];
         }
       }
     }
@@ -534,6 +577,14 @@ template <int BN>
 using EpiLse = EpiLseT<BN, false>;
 template <int BN>
 using EpiLseBias = EpiLseT<BN, true>;
+template <int BN>
+using EpiLseTemp = EpiLseT<BN, false, kAtTemperature>;
+template <int BN>
+using EpiLseBiasTemp = EpiLseT<BN, true, kAtTemperature>;
+template <int BN>
+using EpiLseTwo = EpiLseT<BN, false, kTwoSoftmaxes>;
+template <int BN>
+using EpiLseBiasTwo = EpiLseT<BN, true, kTwoSoftmaxes>;
 
 struct GradParams {
   const float* bias;     // [V] or null (full vocabulary, indexed by v0 + c)
@@ -543,10 +594,13 @@ struct GradParams {
   long ldg;
   int v0;                // first vocabulary row of the band
   int tiles_n;           // column tiles in the band
+  float scale;           // log2(e) over a temperature (not with kOneSoftmax)
 };
 
 // Backward recompute: G[n][c] = dLoss/dS for one vocabulary band, stored bf16.
-// rowp[n] = {lse*log2e, cP, cT, cU}: g = cP*2^(x*log2e - lse2) - cU - cT*[c == label].
+// rowp[n] = {lse2, cP, cT, cU}: g = cP*2^(x*scale - lse2) - cU - cT*[c == label].
+// kTwoSoftmaxes (no label then): rowp[n] = {lse2, cP, cA, lse2_1}:
+// g = cP*2^(x*scale - lse2) + cA*2^(x*log2e - lse2_1).
 //
 // Stores go through LDS: in the MFMA layout a lane holds one row, so a direct
 // store instruction would touch 32 rows with 16 bytes each.  Each wave writes
@@ -554,8 +608,9 @@ struct GradParams {
 // row so the 16 lanes of a write phase hit distinct banks), reads it back
 // row-major and stores whole 128-byte row segments, 8 rows per instruction.
 // A wave's LDS operations execute in order, so no barrier is needed.
-template <int BN, bool HB>
+template <int BN, bool HB, int SM = kOneSoftmax>
 struct EpiGradT {
+  static constexpr bool DU = SM == kTwoSoftmaxes;
   typedef GradParams Params;
   static constexpr bool kOneTile = true;  // splits == tiles_n: a workgroup takes one column tile
   static constexpr bool kDynSplits = false;
@@ -594,6 +649,7 @@ struct EpiGradT {
     constexpr int kArea = 32 * (BN / 2);  // 32 rows x the wave's columns, in 32 x 64 blocks
     bf16_t* const ws = scratch + (wm * 2 + wn) * 2 * kArea;
     const int col0 = tn * BN + wn * (BN / 2);
+    const float scale = SM == kOneSoftmax ? kLog2e : p.scale;
     auto stage = [&](int i, float4 rp, auto INTERIOR) __attribute__((always_inline)) {
       int lp = l;
       asm volatile("" : "+v"(lp));  // the columns' masks are not kept from row block to row block
@@ -613,7 +669,8 @@ struct EpiGradT {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float xe = HB ? x[j][4 * q + e] + bv[e] : x[j][4 * q + e];
-            const float gg = __builtin_fmaf(rp.y, fast_exp2(__builtin_fmaf(xe, kLog2e, -rp.x)), -rp.w);
+            float gg = __builtin_fmaf(rp.y, fast_exp2(__builtin_fmaf(xe, scale, -rp.x)), DU ? 0.f : -rp.w);
+            if constexpr (DU) gg = __builtin_fmaf(rp.z, fast_exp2(__builtin_fmaf(xe, kLog2e, -rp.w)), gg);
             gv[e] = decltype(INTERIOR)::value || cb + e < g.N ? gg : 0.f;
           }
           // packed to bf16; the 8-byte piece hc (of 16 per 128-byte row) lives at hc ^ (row & 15)
@@ -654,7 +711,7 @@ struct EpiGradT {
         for (int k = 0; k < n; ++k) v[k] = at & bit ? v[2 * k + 1] : v[2 * k];
       if (mine) {
         const float xe = HB ? v[0] + p.bias[p.v0 + lab] : v[0];
-        const float gg = __builtin_fmaf(rp.y, fast_exp2(__builtin_fmaf(xe, kLog2e, -rp.x)), -rp.w) - rp.z;
+        const float gg = __builtin_fmaf(rp.y, fast_exp2(__builtin_fmaf(xe, scale, -rp.x)), -rp.w) - rp.z;
         bf16_t* const t = ws + (i & 1) * kArea + r * 64 + (lc >> 6) * 2048 +
                           ((((int)(lc & 63) >> 2) ^ (r & 15)) << 2) + (lc & 3);
         *t = __builtin_bit_cast(bf16_t, (__bf16)gg);
@@ -692,7 +749,7 @@ struct EpiGradT {
         stage(i, rp, std::true_type{});
       else
         stage(i, rp, std::false_type{});
-      one_hot(i, rp, lab);
+      if constexpr (SM == kOneSoftmax) one_hot(i, rp, lab);
       if (i > 0) store(i - 1);
       rp = rp1;
       lab = lab1;
@@ -707,6 +764,14 @@ template <int BN>
 using EpiGrad = EpiGradT<BN, false>;
 template <int BN>
 using EpiGradBias = EpiGradT<BN, true>;
+template <int BN>
+using EpiGradTemp = EpiGradT<BN, false, kAtTemperature>;
+template <int BN>
+using EpiGradBiasTemp = EpiGradT<BN, true, kAtTemperature>;
+template <int BN>
+using EpiGradTwo = EpiGradT<BN, false, kTwoSoftmaxes>;
+template <int BN>
+using EpiGradBiasTwo = EpiGradT<BN, true, kTwoSoftmaxes>;
 
 struct AccParams {
   float* acc32;
@@ -1146,8 +1211,8 @@ __device__ __forceinline__ void dh_body(const GemmShape& g0, const AccParams& e0
 }
 
 // HB: with a bias.  AROW: the recompute reads H's rows through the row order.
-// KTAIL: d is no multiple of 64 (the recompute's K).
-template <bool HB, bool AROW, bool KTAIL>
+// KTAIL: d is no multiple of 64 (the recompute's K).  SM: EpiGradT's.
+template <bool HB, bool AROW, bool KTAIL, int SM = kOneSoftmax>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))) void band_kernel(BandLaunch p) {
   __shared__ __attribute__((aligned(16))) bf16_t smem[kLdsElems];
   // the populations in the launch's order, then the reduction
@@ -1178,10 +1243,18 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
     return;
   }
   if (pop == kPopGrad) {
-    if constexpr (HB)
+    if constexpr (SM == kOneSoftmax && HB)
       gemm_body<kBN, true, true, EpiGradBias, AROW, KTAIL>(p.gr, p.e_gr, b, p.nb_gr, smem);
-    else
+    else if constexpr (SM == kOneSoftmax)
       gemm_body<kBN, true, true, EpiGrad, AROW, KTAIL>(p.gr, p.e_gr, b, p.nb_gr, smem);
+    else if constexpr (SM == kAtTemperature && HB)
+      gemm_body<kBN, true, true, EpiGradBiasTemp, AROW, KTAIL>(p.gr, p.e_gr, b, p.nb_gr, smem);
+    else if constexpr (SM == kAtTemperature)
+      gemm_body<kBN, true, true, EpiGradTemp, AROW, KTAIL>(p.gr, p.e_gr, b, p.nb_gr, smem);
+    else if constexpr (HB)
+      gemm_body<kBN, true, true, EpiGradBiasTwo, AROW, KTAIL>(p.gr, p.e_gr, b, p.nb_gr, smem);
+    else
+      gemm_body<kBN, true, true, EpiGradTwo, AROW, KTAIL>(p.gr, p.e_gr, b, p.nb_gr, smem);
     return;
   }
   dh_reduce_body(p.red, b * (long)kThreads + threadIdx.x, (long)p.nb_red * kThreads);
@@ -2232,6 +2305,9 @@ struct BwdLayout {
   // null when unsplit
   float* dhpart;
   int dh_ks;
+  // SparseGrad's columns and values
+  int* col;
+  float* val;
   size_t bytes;
 };
 
@@ -2265,7 +2341,7 @@ int dh_splits(long N, long d, long Vb) {
 long ht_cols(long N) { return (long)align_up((size_t)N, kBK); }
 
 BwdLayout bwd_layout(void* ws, long N, long d, long V, long Vb, bool need_dh, bool need_dw, bool dh_f32,
-                     bool dw_f32) {
+                     bool dw_f32, int entries = 0) {
   Carver c(ws);
   BwdLayout L;
   L.N = N;
@@ -2297,6 +2373,8 @@ BwdLayout bwd_layout(void* ws, long N, long d, long V, long Vb, bool need_dh, bo
   // band launch writes the one buffer again
   L.dhpart = L.dh_ks > 1 ? c.take<float>((size_t)(dh_fold(L.dh_ks) && units > 1 ? 2 : 1) * L.dh_ks * L.Nb * d)
                          : nullptr;
+  L.col = entries ? c.take<int>((size_t)N * entries) : nullptr;
+  L.val = entries ? c.take<float>((size_t)N * entries) : nullptr;
   L.bytes = align_up(c.off, 256);
   return L;
 }
@@ -2413,7 +2491,7 @@ int zero_fill(void* p, size_t bytes, hipStream_t st) {
 // Each workgroup takes one tile, the finest grain for filling the CUs that the
 // long dW / dH tiles of a band launch leave idle.
 void grad_shape(const bf16_t* H, const bf16_t* W, const float* bias, const BwdLayout& L, bf16_t* G, long m0,
-                long rows, long d, long v0, long vb, GemmShape& g, GradParams& e, int& nb) {
+                long rows, long d, long v0, long vb, float scale, GemmShape& g, GradParams& e, int& nb) {
   const int gm = (int)ceil_div(rows, kBM);
   if (L.Hc || !L.idx) {
     g.A = (L.Hc ? L.Hc : H) + m0 * d;
@@ -2426,6 +2504,7 @@ void grad_shape(const bf16_t* H, const bf16_t* W, const float* bias, const BwdLa
   g.M = (int)rows; g.N = (int)vb; g.K = (int)d;
   g.live = L.live; g.dyn = L.live ? kDynM : kDynNone; g.live_base = (int)m0;
   e.bias = bias; e.rowp = L.rowp + m0; e.rowlab = L.rowlab + m0; e.G = G; e.ldg = L.Vb; e.v0 = (int)v0;
+  e.scale = scale;
   e.tiles_n = (int)ceil_div(vb, kBN);
   nb = gm * e.tiles_n;
 }
@@ -2456,7 +2535,15 @@ void order_populations(BandLaunch& p, long k_dw, long k_dh, long k_gr) {
   }
 }
 
-int launch_band(const BandLaunch& p, bool has_bias, hipStream_t st, int kind = CCE_KERNEL_BWD_BAND) {
+template <int SM>
+auto* pick_band(bool has_bias, bool arow, bool ktail) {
+  return ktail  ? (has_bias ? band_kernel<true, false, true, SM> : band_kernel<false, false, true, SM>)
+         : arow ? (has_bias ? band_kernel<true, true, false, SM> : band_kernel<false, true, false, SM>)
+                : (has_bias ? band_kernel<true, false, false, SM> : band_kernel<false, false, false, SM>);
+}
+
+int launch_band(const BandLaunch& p, bool has_bias, hipStream_t st, int kind = CCE_KERNEL_BWD_BAND,
+                int softmaxes = kOneSoftmax) {
   const int nb = p.nb_dw + p.nb_dw2 + p.nb_dh + p.nb_dh2 + p.nb_gr + p.nb_red;
   if (nb <= 0) return CCE_OK;
   int rc = CCE_OK;
@@ -2470,9 +2557,9 @@ int launch_band(const BandLaunch& p, bool has_bias, hipStream_t st, int kind = C
   hipEvent_t t0 = nullptr, t1 = nullptr;
   const bool timed = timing_begin(st, &t0, &t1);
   const bool arow = p.gr.arow != nullptr;
-  auto* const kernel = ktail ? (has_bias ? band_kernel<true, false, true> : band_kernel<false, false, true>)
-                       : arow ? (has_bias ? band_kernel<true, true, false> : band_kernel<false, true, false>)
-                              : (has_bias ? band_kernel<true, false, false> : band_kernel<false, false, false>);
+  auto* const kernel = softmaxes == kOneSoftmax      ? pick_band<kOneSoftmax>(has_bias, arow, ktail)
+                       : softmaxes == kAtTemperature ? pick_band<kAtTemperature>(has_bias, arow, ktail)
+                                                     : pick_band<kTwoSoftmaxes>(has_bias, arow, ktail);
   hipLaunchKernelGGL(kernel, dim3(nb), dim3(kThreads), 0, st, p);
   HIP_TRY(hipGetLastError());
   if (timed) {
@@ -2521,6 +2608,15 @@ int check_logits_args(long N, long V, int dtype, long ld, int reduction, float e
   if (smooth != CCE_SMOOTH_LOGV && smooth != CCE_SMOOTH_UNIFORM)
     return fail(CCE_ERR_INVALID_ARG, "smoothing_form must be CCE_SMOOTH_LOGV or CCE_SMOOTH_UNIFORM, got %d", smooth);
   return CCE_OK;
+}
+
+// The forward's GEMM, by the form of its A operand.
+template <template <int> class Epi>
+int launch_lse(const GemmShape& g, const LseParams& ep, int slots, hipStream_t st) {
+  constexpr int kKind = CCE_KERNEL_FWD_LSE;
+  if (!whole_slabs(g.K)) return launch_gemm<kBN, Epi, false, true>(g, ep, slots, st, kKind, true);
+  if (g.arow) return launch_gemm<kBN, Epi, true>(g, ep, slots, st, kKind, true);
+  return launch_gemm<kBN, Epi>(g, ep, slots, st, kKind, true);
 }
 
 int forward_run(const void* hidden, const void* weight, const void* labels, int labels_int64, const float* bias,
@@ -2593,16 +2689,9 @@ int forward_run(const void* hidden, const void* weight, const void* labels, int 
   ep.ldp = N;
   ep.splits = S;
   ep.tiles_n = (int)ceil_div(V, kBN);
-  constexpr int kKind = CCE_KERNEL_FWD_LSE;
-  if (!whole_slabs(d))
-    rc = bias ? launch_gemm<kBN, EpiLseBias, false, true>(g, ep, slots, st, kKind, true)
-              : launch_gemm<kBN, EpiLse, false, true>(g, ep, slots, st, kKind, true);
-  else if (g.arow)
-    rc = bias ? launch_gemm<kBN, EpiLseBias, true>(g, ep, slots, st, kKind, true)
-              : launch_gemm<kBN, EpiLse, true>(g, ep, slots, st, kKind, true);
-  else
-    rc = bias ? launch_gemm<kBN, EpiLseBias>(g, ep, slots, st, kKind, true)
-              : launch_gemm<kBN, EpiLse>(g, ep, slots, st, kKind, true);
+  ep.scale = kLog2e;
+  ep.ps1 = nullptr;
+  rc = bias ? launch_lse<EpiLseBias>(g, ep, slots, st) : launch_lse<EpiLse>(g, ep, slots, st);
   if (rc) return rc;
 
   const bool uniform = smoothing_form == CCE_SMOOTH_UNIFORM && label_smoothing > 0.f;
@@ -2629,133 +2718,38 @@ int forward_run(const void* hidden, const void* weight, const void* labels, int 
   return CCE_OK;
 }
 
-}  // namespace
+// Row coefficients and sparse columns of a gradient that is not the
+// cross-entropy's (distillation), in place of bwd_prep_kernel.
+struct SparseGrad {
+  float scale;  // GradParams
+  int softmaxes;  // EpiGradT
+  int entries;  // columns per row
+  // rowp and rowlab of the N rows in the GEMM's order (idx; null: as they are),
+  // their columns ([N][entries], -1: none) and the values of G there
+  int (*prep)(const SparseGrad& s, const int* idx, long N, float4* rowp, int* rowlab, int* col, float* val,
+              hipStream_t st);
+  const void* args;
+};
 
-// ---------------------------------------------------------------------------
-// Static scratch of cce_forward_noalloc: the forward's workspace for callers
-// that cannot allocate device memory.  Each device that runs the library holds
-// its own copy of this array (CCE_NOALLOC_SCRATCH_BYTES) until the process
-// ends.  In host code `scratch` names a host-side stand-in, not device memory:
-// the device address comes from hipGetSymbolAddress, once per device, and only
-// that address is passed to kernels.
-// ---------------------------------------------------------------------------
-static __device__ __align__(256) unsigned char scratch[CCE_NOALLOC_SCRATCH_BYTES];
-
-namespace {
-
-constexpr int kMaxDevices = 64;
-std::mutex g_scratch_mu;
-void* g_scratch_dev[kMaxDevices] = {};
-
-// Device address of `scratch` on the current device (looked up on the first
-// call per device and kept).
-int noalloc_scratch(void** out) {
-  int dev = -1;
-  HIP_TRY(hipGetDevice(&dev));
-  if (dev < 0 || dev >= kMaxDevices)
-    return fail(CCE_ERR_INVALID_ARG, "device ordinal %d outside [0, %d)", dev, kMaxDevices);
-  std::lock_guard<std::mutex> lk(g_scratch_mu);
-  if (!g_scratch_dev[dev]) {
-    void* p = nullptr;
-    HIP_TRY(hipGetSymbolAddress(&p, HIP_SYMBOL(scratch)));
-    if (!p) return fail(CCE_ERR_HIP, "hipGetSymbolAddress(scratch) returned a null address on device %d", dev);
-    g_scratch_dev[dev] = p;
+// G[m][col - v0] = val for the block's rows and the band's columns.
+__global__ __launch_bounds__(256) void sparse_grad_kernel(const int* __restrict__ col, const float* __restrict__ val,
+                                                          int entries, int rows, const int* __restrict__ live,
+                                                          int live_base, int v0, int vb, bf16_t* __restrict__ G,
+                                                          long ldg) {
+  if (live) rows = min(rows, live_rows(live, live_base));
+  const long total = (long)rows * entries;
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+    const unsigned c = (unsigned)(col[i] - v0);
+    if (c < (unsigned)vb) G[(i / entries) * ldg + c] = __builtin_bit_cast(bf16_t, (__bf16)val[i]);
   }
-  *out = g_scratch_dev[dev];
-  return CCE_OK;
 }
 
-}  // namespace
-
-// ===========================================================================
-// C ABI
-// ===========================================================================
-
-extern "C" {
-
-const char* cce_last_error(void) { return g_err; }
-
-int cce_abi_version(void) { return CCE_ABI_VERSION; }
-
-// The build passes the SHA-256 of this file and the header as bare hex digits.
-#ifndef CCE_SOURCE_HASH
-#define CCE_SOURCE_HASH unknown
-#endif
-#define CCE_STR2(x) #x
-#define CCE_STR(x) CCE_STR2(x)
-const char* cce_source_hash(void) { return CCE_STR(CCE_SOURCE_HASH); }
-
-int cce_forward_workspace_bytes(int64_t N, int64_t d, int64_t V, int reduction, int lse_rows, size_t* bytes) {
-  g_err[0] = 0;
-  if (!bytes) return fail(CCE_ERR_INVALID_ARG, "bytes must not be null");
-  int rc = check_dims(N, d, V);
-  if (rc) return rc;
-  if (reduction < CCE_REDUCTION_NONE || reduction > CCE_REDUCTION_SUM)
-    return fail(CCE_ERR_INVALID_ARG, "reduction must be 0 (none), 1 (mean) or 2 (sum), got %d", reduction);
-  if (lse_rows != CCE_LSE_ALL_ROWS && lse_rows != CCE_LSE_LABELLED_ROWS)
-    return fail(CCE_ERR_INVALID_ARG, "lse_rows must be CCE_LSE_ALL_ROWS or CCE_LSE_LABELLED_ROWS, got %d", lse_rows);
-  *bytes = fwd_layout(nullptr, N, d, V, reduction, lse_rows).bytes;
-  return CCE_OK;
-}
-
-int cce_backward_workspace_bytes(int64_t N, int64_t d, int64_t V, int64_t chunk_size, int need_grad_hidden,
-                                 int grad_hidden_dtype, int need_grad_weight, int grad_weight_dtype, size_t* bytes) {
-  g_err[0] = 0;
-  if (!bytes) return fail(CCE_ERR_INVALID_ARG, "bytes must not be null");
-  int rc = check_dims(N, d, V);
-  if (rc) return rc;
-  if ((need_grad_hidden && grad_hidden_dtype != CCE_DTYPE_BF16 && grad_hidden_dtype != CCE_DTYPE_F32) ||
-      (need_grad_weight && grad_weight_dtype != CCE_DTYPE_BF16 && grad_weight_dtype != CCE_DTYPE_F32))
-    return fail(CCE_ERR_INVALID_ARG, "gradient dtypes must be CCE_DTYPE_BF16 or CCE_DTYPE_F32");
-  *bytes = bwd_layout(nullptr, N, d, V, band_width(V, chunk_size, N), need_grad_hidden != 0,
-                      need_grad_weight != 0, grad_hidden_dtype == CCE_DTYPE_F32,
-                      grad_weight_dtype == CCE_DTYPE_F32).bytes;
-  return CCE_OK;
-}
-
-int cce_forward(const void* hidden, const void* weight, const void* labels, int labels_int64, const float* bias,
-                int64_t N, int64_t d, int64_t V, int64_t ignore_index, float label_smoothing, float z_loss_weight,
-                int smoothing_form, int reduction, int lse_rows, float* loss_out, float* lse_out, float* target_out,
-                int32_t* n_valid_out, void* workspace, size_t workspace_bytes, void* stream) {
-  g_err[0] = 0;
-  return forward_run(hidden, weight, labels, labels_int64, bias, N, d, V, ignore_index, label_smoothing,
-                     z_loss_weight, smoothing_form, reduction, lse_rows, loss_out, lse_out, target_out, n_valid_out,
-                     workspace, workspace_bytes, stream);
-}
-
-int cce_forward_noalloc(const void* hidden, const void* weight, const void* labels, int labels_int64,
-                        const float* bias, int64_t N, int64_t d, int64_t V, int64_t ignore_index,
-                        float label_smoothing, float z_loss_weight, int smoothing_form, int reduction, int lse_rows,
-                        float* loss_out, float* lse_out, float* target_out, int32_t* n_valid_out, void* stream) {
-  g_err[0] = 0;
-  int rc = check_dims(N, d, V);
-  if (rc) return rc;
-  if (reduction < CCE_REDUCTION_NONE || reduction > CCE_REDUCTION_SUM)
-    return fail(CCE_ERR_INVALID_ARG, "reduction must be 0 (none), 1 (mean) or 2 (sum), got %d", reduction);
-  if (lse_rows != CCE_LSE_ALL_ROWS && lse_rows != CCE_LSE_LABELLED_ROWS)
-    return fail(CCE_ERR_INVALID_ARG, "lse_rows must be CCE_LSE_ALL_ROWS or CCE_LSE_LABELLED_ROWS, got %d", lse_rows);
-  // the static scratch is fixed: the rows are read in place wherever the
-  // byte offsets into hidden allow, so no N x d copy takes scratch
-  const size_t need = fwd_layout(nullptr, N, d, V, reduction, lse_rows, true).bytes;
-  if (need > (size_t)CCE_NOALLOC_SCRATCH_BYTES)
-    return fail(CCE_ERR_WORKSPACE,
-                "cce_forward_noalloc: this problem (N=%ld d=%ld V=%ld) needs %zu bytes of scratch, more than the "
-                "%zu-byte static scratch; call cce_forward with a workspace instead",
-                (long)N, (long)d, (long)V, need, (size_t)CCE_NOALLOC_SCRATCH_BYTES);
-  void* ws = nullptr;
-  rc = noalloc_scratch(&ws);
-  if (rc) return rc;
-  return forward_run(hidden, weight, labels, labels_int64, bias, N, d, V, ignore_index, label_smoothing,
-                     z_loss_weight, smoothing_form, reduction, lse_rows, loss_out, lse_out, target_out, n_valid_out,
-                     ws, (size_t)CCE_NOALLOC_SCRATCH_BYTES, stream, true);
-}
-
-int cce_backward(const float* grad_out, const void* hidden, const void* weight, const void* labels, int labels_int64,
+int backward_run(const float* grad_out, const void* hidden, const void* weight, const void* labels, int labels_int64,
                  const float* bias, const float* lse, const int32_t* n_valid, int64_t N, int64_t d, int64_t V,
                  int64_t ignore_index, float label_smoothing, float z_loss_weight, int reduction, int64_t chunk_size,
                  void* grad_hidden, int grad_hidden_dtype, void* grad_weight, int grad_weight_dtype,
-                 float* grad_bias, void* workspace, size_t workspace_bytes, void* stream) {
-  g_err[0] = 0;
+                 float* grad_bias, void* workspace, size_t workspace_bytes, void* stream,
+                 const SparseGrad* sparse) {
   int rc = check_dims(N, d, V);
   if (rc) return rc;
   if (reduction < CCE_REDUCTION_NONE || reduction > CCE_REDUCTION_SUM)
@@ -2775,7 +2769,8 @@ int cce_backward(const float* grad_out, const void* hidden, const void* weight, 
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const bool dh_f32 = grad_hidden_dtype == CCE_DTYPE_F32, dw_f32 = grad_weight_dtype == CCE_DTYPE_F32;
   const long Vb = band_width(V, chunk_size, N);
-  const BwdLayout need = bwd_layout(nullptr, N, d, V, Vb, need_dh, need_dw, dh_f32, dw_f32);
+  const int entries = sparse ? sparse->entries : 0;
+  const BwdLayout need = bwd_layout(nullptr, N, d, V, Vb, need_dh, need_dw, dh_f32, dw_f32, entries);
   if (workspace_bytes < need.bytes || (need.bytes && !workspace))
     return fail(CCE_ERR_WORKSPACE, "workspace too small: need %zu bytes, got %zu", need.bytes, workspace_bytes);
   if (N == 0) {
@@ -2787,7 +2782,7 @@ int cce_backward(const float* grad_out, const void* hidden, const void* weight, 
     return CCE_OK;
   }
   if (!need_dh && !need_dw && !need_db) return CCE_OK;
-  BwdLayout L = bwd_layout(workspace, N, d, V, Vb, need_dh, need_dw, dh_f32, dw_f32);
+  BwdLayout L = bwd_layout(workspace, N, d, V, Vb, need_dh, need_dw, dh_f32, dw_f32, entries);
   if (L.ht_out) L.HT = static_cast<bf16_t*>(grad_hidden);
   if (L.hc_out) L.Hc = static_cast<bf16_t*>(grad_hidden);
   const long NT = ht_cols(N);  // row length of H^T
@@ -2807,10 +2802,15 @@ int cce_backward(const float* grad_out, const void* hidden, const void* weight, 
       HIP_TRY(hipGetLastError());
     }
   }
-  hipLaunchKernelGGL(bwd_prep_kernel, dim3((unsigned)ceil_div(N, 256)), dim3(256), 0, st, grad_out, lse, n_valid,
-                     labels, labels_int64, (int)N, (int)V, (long)ignore_index, label_smoothing, z_loss_weight,
-                     reduction, L.idx, L.rowp, L.rowlab);
-  HIP_TRY(hipGetLastError());
+  if (sparse) {
+    rc = sparse->prep(*sparse, L.idx, N, L.rowp, L.rowlab, L.col, L.val, st);
+    if (rc) return rc;
+  } else {
+    hipLaunchKernelGGL(bwd_prep_kernel, dim3((unsigned)ceil_div(N, 256)), dim3(256), 0, st, grad_out, lse, n_valid,
+                       labels, labels_int64, (int)N, (int)V, (long)ignore_index, label_smoothing, z_loss_weight,
+                       reduction, L.idx, L.rowp, L.rowlab);
+    HIP_TRY(hipGetLastError());
+  }
   if (need_dw) {
     hipLaunchKernelGGL(transpose_kernel, dim3((unsigned)ceil_div(NT, 64), (unsigned)ceil_div(d, 64)), dim3(256), 0,
                        st, L.Hc ? L.Hc : H, (long)d, (int)N, (int)d, L.HT, (long)NT, (int)NT,
@@ -2905,8 +2905,22 @@ int cce_backward(const float* grad_out, const void* hidden, const void* weight, 
     long v0, vb, m0, rows;
     band_cols(u / R, v0, vb);
     block_span(u % R, m0, rows);
-    grad_shape(H, W, bias, L, L.G[u & 1], m0, rows, d, v0, vb, g, e, nb);
+    grad_shape(H, W, bias, L, L.G[u & 1], m0, rows, d, v0, vb, sparse ? sparse->scale : kLog2e, g, e, nb);
   };
+
+  // the sparse columns of unit u over its dense gradient
+  auto sparse_unit = [&](long u) -> int {
+    if (!sparse) return CCE_OK;
+    long v0, vb, m0, rows;
+    band_cols(u / R, v0, vb);
+    block_span(u % R, m0, rows);
+    hipLaunchKernelGGL(sparse_grad_kernel, dim3((unsigned)std::min<long>(ceil_div(rows * entries, 256), 1024)),
+                       dim3(256), 0, st, L.col + m0 * entries, L.val + m0 * entries, entries, (int)rows, L.live,
+                       (int)m0, (int)v0, (int)vb, L.G[u & 1], Vb);
+    HIP_TRY(hipGetLastError());
+    return CCE_OK;
+  };
+  const int softmaxes = sparse ? sparse->softmaxes : kOneSoftmax;
 
   // launch u: dW and dH of unit u from G[u & 1] and the recompute of unit
   // u+1 into G[(u+1) & 1]; unit 0's recompute runs alone first.
@@ -2914,7 +2928,8 @@ int cce_backward(const float* grad_out, const void* hidden, const void* weight, 
   BandLaunch first = {};
   grad_unit(0, first.gr, first.e_gr, first.nb_gr);
   order_populations(first, 0, 0, d);
-  rc = launch_band(first, bias != nullptr, st, CCE_KERNEL_BWD_GRAD);
+  rc = launch_band(first, bias != nullptr, st, CCE_KERNEL_BWD_GRAD, softmaxes);
+  if (!rc) rc = sparse_unit(0);
   if (rc) return rc;
   // With 4 or more splits (very few rows) the band launches are short and the
   // reduction rides in the next launch, so the partials alternate between
@@ -2993,7 +3008,8 @@ int cce_backward(const float* grad_out, const void* hidden, const void* weight, 
     }
     if (u + 1 < units) grad_unit(u + 1, p.gr, p.e_gr, p.nb_gr);
     order_populations(p, rows, p.dh_kc, d);
-    rc = launch_band(p, bias != nullptr, st);
+    rc = launch_band(p, bias != nullptr, st, CCE_KERNEL_BWD_BAND, softmaxes);
+    if (!rc && u + 1 < units) rc = sparse_unit(u + 1);
     if (rc) return rc;
     if (need_dh && L.dhpart && (!fold || u + 1 == units)) {
       // this unit's partials (the last band's go to the output: mode 0, 3 or 4)
@@ -3030,6 +3046,143 @@ int cce_backward(const float* grad_out, const void* hidden, const void* weight, 
     HIP_TRY(hipGetLastError());
   }
   return CCE_OK;
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------------------
+// Static scratch of cce_forward_noalloc: the forward's workspace for callers
+// that cannot allocate device memory.  Each device that runs the library holds
+// its own copy of this array (CCE_NOALLOC_SCRATCH_BYTES) until the process
+// ends.  In host code `scratch` names a host-side stand-in, not device memory:
+// the device address comes from hipGetSymbolAddress, once per device, and only
+// that address is passed to kernels.
+// ---------------------------------------------------------------------------
+static __device__ __align__(256) unsigned char scratch[CCE_NOALLOC_SCRATCH_BYTES];
+
+namespace {
+
+constexpr int kMaxDevices = 64;
+std::mutex g_scratch_mu;
+void* g_scratch_dev[kMaxDevices] = {};
+
+// Device address of `scratch` on the current device (looked up on the first
+// call per device and kept).
+int noalloc_scratch(void** out) {
+  int dev = -1;
+  HIP_TRY(hipGetDevice(&dev));
+  if (dev < 0 || dev >= kMaxDevices)
+    return fail(CCE_ERR_INVALID_ARG, "device ordinal %d outside [0, %d)", dev, kMaxDevices);
+  std::lock_guard<std::mutex> lk(g_scratch_mu);
+  if (!g_scratch_dev[dev]) {
+    void* p = nullptr;
+    HIP_TRY(hipGetSymbolAddress(&p, HIP_SYMBOL(scratch)));
+    if (!p) return fail(CCE_ERR_HIP, "hipGetSymbolAddress(scratch) returned a null address on device %d", dev);
+    g_scratch_dev[dev] = p;
+  }
+  *out = g_scratch_dev[dev];
+  return CCE_OK;
+}
+
+#include "layer_norm.h"
+#include "top_logits.h"
+#include "distill.h"
+#include "distill_linear.h"
+
+}  // namespace
+
+// ===========================================================================
+// C ABI
+// ===========================================================================
+
+extern "C" {
+
+const char* cce_last_error(void) { return g_err; }
+
+int cce_abi_version(void) { return CCE_ABI_VERSION; }
+
+// The build passes the SHA-256 of this file and the header as bare hex digits.
+#ifndef CCE_SOURCE_HASH
+#define CCE_SOURCE_HASH unknown
+#endif
+#define CCE_STR2(x) #x
+#define CCE_STR(x) CCE_STR2(x)
+const char* cce_source_hash(void) { return CCE_STR(CCE_SOURCE_HASH); }
+
+int cce_forward_workspace_bytes(int64_t N, int64_t d, int64_t V, int reduction, int lse_rows, size_t* bytes) {
+  g_err[0] = 0;
+  if (!bytes) return fail(CCE_ERR_INVALID_ARG, "bytes must not be null");
+  int rc = check_dims(N, d, V);
+  if (rc) return rc;
+  if (reduction < CCE_REDUCTION_NONE || reduction > CCE_REDUCTION_SUM)
+    return fail(CCE_ERR_INVALID_ARG, "reduction must be 0 (none), 1 (mean) or 2 (sum), got %d", reduction);
+  if (lse_rows != CCE_LSE_ALL_ROWS && lse_rows != CCE_LSE_LABELLED_ROWS)
+    return fail(CCE_ERR_INVALID_ARG, "lse_rows must be CCE_LSE_ALL_ROWS or CCE_LSE_LABELLED_ROWS, got %d", lse_rows);
+  *bytes = fwd_layout(nullptr, N, d, V, reduction, lse_rows).bytes;
+  return CCE_OK;
+}
+
+int cce_backward_workspace_bytes(int64_t N, int64_t d, int64_t V, int64_t chunk_size, int need_grad_hidden,
+                                 int grad_hidden_dtype, int need_grad_weight, int grad_weight_dtype, size_t* bytes) {
+  g_err[0] = 0;
+  if (!bytes) return fail(CCE_ERR_INVALID_ARG, "bytes must not be null");
+  int rc = check_dims(N, d, V);
+  if (rc) return rc;
+  if ((need_grad_hidden && grad_hidden_dtype != CCE_DTYPE_BF16 && grad_hidden_dtype != CCE_DTYPE_F32) ||
+      (need_grad_weight && grad_weight_dtype != CCE_DTYPE_BF16 && grad_weight_dtype != CCE_DTYPE_F32))
+    return fail(CCE_ERR_INVALID_ARG, "gradient dtypes must be CCE_DTYPE_BF16 or CCE_DTYPE_F32");
+  *bytes = bwd_layout(nullptr, N, d, V, band_width(V, chunk_size, N), need_grad_hidden != 0,
+                      need_grad_weight != 0, grad_hidden_dtype == CCE_DTYPE_F32,
+                      grad_weight_dtype == CCE_DTYPE_F32).bytes;
+  return CCE_OK;
+}
+
+int cce_forward(const void* hidden, const void* weight, const void* labels, int labels_int64, const float* bias,
+                int64_t N, int64_t d, int64_t V, int64_t ignore_index, float label_smoothing, float z_loss_weight,
+                int smoothing_form, int reduction, int lse_rows, float* loss_out, float* lse_out, float* target_out,
+                int32_t* n_valid_out, void* workspace, size_t workspace_bytes, void* stream) {
+  g_err[0] = 0;
+  return forward_run(hidden, weight, labels, labels_int64, bias, N, d, V, ignore_index, label_smoothing,
+                     z_loss_weight, smoothing_form, reduction, lse_rows, loss_out, lse_out, target_out, n_valid_out,
+                     workspace, workspace_bytes, stream);
+}
+
+int cce_forward_noalloc(const void* hidden, const void* weight, const void* labels, int labels_int64,
+                        const float* bias, int64_t N, int64_t d, int64_t V, int64_t ignore_index,
+                        float label_smoothing, float z_loss_weight, int smoothing_form, int reduction, int lse_rows,
+                        float* loss_out, float* lse_out, float* target_out, int32_t* n_valid_out, void* stream) {
+  g_err[0] = 0;
+  int rc = check_dims(N, d, V);
+  if (rc) return rc;
+  if (reduction < CCE_REDUCTION_NONE || reduction > CCE_REDUCTION_SUM)
+    return fail(CCE_ERR_INVALID_ARG, "reduction must be 0 (none), 1 (mean) or 2 (sum), got %d", reduction);
+  if (lse_rows != CCE_LSE_ALL_ROWS && lse_rows != CCE_LSE_LABELLED_ROWS)
+    return fail(CCE_ERR_INVALID_ARG, "lse_rows must be CCE_LSE_ALL_ROWS or CCE_LSE_LABELLED_ROWS, got %d", lse_rows);
+  // the static scratch is fixed: the rows are read in place wherever the
+  // byte offsets into hidden allow, so no N x d copy takes scratch
+  const size_t need = fwd_layout(nullptr, N, d, V, reduction, lse_rows, true).bytes;
+  if (need > (size_t)CCE_NOALLOC_SCRATCH_BYTES)
+    return fail(CCE_ERR_WORKSPACE,
+                "cce_forward_noalloc: this problem (N=%ld d=%ld V=%ld) needs %zu bytes of scratch, more than the "
+                "%zu-byte static scratch; call cce_forward with a workspace instead",
+                (long)N, (long)d, (long)V, need, (size_t)CCE_NOALLOC_SCRATCH_BYTES);
+  void* ws = nullptr;
+  rc = noalloc_scratch(&ws);
+  if (rc) return rc;
+  return forward_run(hidden, weight, labels, labels_int64, bias, N, d, V, ignore_index, label_smoothing,
+                     z_loss_weight, smoothing_form, reduction, lse_rows, loss_out, lse_out, target_out, n_valid_out,
+                     ws, (size_t)CCE_NOALLOC_SCRATCH_BYTES, stream, true);
+}
+
+int cce_backward(const float* grad_out, const void* hidden, const void* weight, const void* labels, int labels_int64,
+                 const float* bias, const float* lse, const int32_t* n_valid, int64_t N, int64_t d, int64_t V,
+                 int64_t ignore_index, float label_smoothing, float z_loss_weight, int reduction, int64_t chunk_size,
+                 void* grad_hidden, int grad_hidden_dtype, void* grad_weight, int grad_weight_dtype,
+                 float* grad_bias, void* workspace, size_t workspace_bytes, void* stream) {
+  g_err[0] = 0;
+  return backward_run(grad_out, hidden, weight, labels, labels_int64, bias, lse, n_valid, N, d, V, ignore_index,
+                      label_smoothing, z_loss_weight, reduction, chunk_size, grad_hidden, grad_hidden_dtype,
+                      grad_weight, grad_weight_dtype, grad_bias, workspace, workspace_bytes, stream, nullptr);
 }
 
 int cce_logits_forward_workspace_bytes(int64_t N, int64_t V, int reduction, size_t* bytes) {
@@ -3204,6 +3357,210 @@ int cce_logits_forward_backward(const void* logits, int logits_dtype, int64_t ld
                      n_valid_out);
   HIP_TRY(hipGetLastError());
   return CCE_OK;
+}
+
+int cce_distill_logits_workspace_bytes(int64_t N, int64_t V, int reduction, size_t* bytes) {
+  g_err[0] = 0;
+  if (!bytes) return fail(CCE_ERR_INVALID_ARG, "bytes must not be null");
+  const int rc = check_logits_args(N, V, CCE_DTYPE_F32, V, reduction, 0.f, CCE_SMOOTH_LOGV);
+  if (rc) return rc;
+  *bytes = kd_layout(nullptr, N, V).bytes;
+  return CCE_OK;
+}
+
+int cce_distill_logits_forward(const void* logits, int logits_dtype, int64_t ld, const cce_teacher* teacher,
+                               const void* labels, int labels_int64, int64_t N, int64_t V, int64_t ignore_index,
+                               int reduction, float* loss_out, float* stats_out, int32_t* n_valid_out,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+  g_err[0] = 0;
+  int rc = check_logits_args(N, V, logits_dtype, ld, reduction, 0.f, CCE_SMOOTH_LOGV);
+  Teacher a;
+  if (!rc) rc = check_teacher(teacher, N, labels, ignore_index, labels_int64, a);
+  if (rc) return rc;
+  if (!n_valid_out || (!loss_out && (N > 0 || reduction != CCE_REDUCTION_NONE)) || (N > 0 && (!logits || !stats_out)))
+    return fail(CCE_ERR_INVALID_ARG, "logits, loss_out, stats_out and n_valid_out must not be null");
+  if (misaligned(stats_out) || misaligned(workspace))
+    return fail(CCE_ERR_INVALID_ARG, "stats_out and workspace must be 16-byte aligned");
+  const KdLayout need = kd_layout(nullptr, N, V);
+  if (workspace_bytes < need.bytes || !workspace)
+    return fail(CCE_ERR_WORKSPACE, "workspace too small: need %zu bytes, got %zu", need.bytes, workspace_bytes);
+  const KdLayout L = kd_layout(workspace, N, V);
+  return logits_type(logits_dtype, [&](auto t) {
+    typedef decltype(t) T;
+    auto* const run = two_softmaxes(a) ? kd_forward_run<T, true> : kd_forward_run<T, false>;
+    return run(static_cast<const T*>(logits), (long)ld, (long)N, (long)V, a, reduction, loss_out,
+               reinterpret_cast<float4*>(stats_out), n_valid_out, L, reinterpret_cast<hipStream_t>(stream));
+  });
+}
+
+int cce_distill_logits_backward(const float* grad_out, const void* logits, int logits_dtype, int64_t ld,
+                                const cce_teacher* teacher, const void* labels, int labels_int64, const float* stats,
+                                const int32_t* n_valid, int64_t N, int64_t V, int64_t ignore_index, int reduction,
+                                void* grad_logits, int64_t ld_grad, void* stream) {
+  g_err[0] = 0;
+  int rc = check_logits_args(N, V, logits_dtype, ld, reduction, 0.f, CCE_SMOOTH_LOGV);
+  Teacher a;
+  if (!rc) rc = check_teacher(teacher, N, labels, ignore_index, labels_int64, a);
+  if (rc) return rc;
+  if (ld_grad < V)
+    return fail(CCE_ERR_INVALID_ARG, "gradient row stride %ld is smaller than V = %ld", (long)ld_grad, (long)V);
+  if (N == 0) return CCE_OK;
+  if (!grad_out || !logits || !stats || !n_valid || !grad_logits)
+    return fail(CCE_ERR_INVALID_ARG, "grad_out, logits, stats, n_valid and grad_logits must not be null");
+  if (grad_logits == logits) return fail(CCE_ERR_INVALID_ARG, "grad_logits must not be the logits");
+  if (misaligned(stats)) return fail(CCE_ERR_INVALID_ARG, "stats must be 16-byte aligned");
+  return logits_type(logits_dtype, [&](auto t) {
+    typedef decltype(t) T;
+    auto* const run = two_softmaxes(a) ? kd_backward_run<T, true> : kd_backward_run<T, false>;
+    return run(grad_out, static_cast<const T*>(logits), (long)ld, (long)N, (long)V, a,
+               reinterpret_cast<const float4*>(stats), n_valid, reduction, static_cast<T*>(grad_logits), (long)ld_grad,
+               reinterpret_cast<hipStream_t>(stream));
+  });
+}
+
+int cce_distill_forward_workspace_bytes(int64_t N, int64_t d, int64_t V, int reduction, size_t* bytes) {
+  g_err[0] = 0;
+  if (!bytes) return fail(CCE_ERR_INVALID_ARG, "bytes must not be null");
+  const int rc = check_dims(N, d, V);
+  if (rc) return rc;
+  if (reduction < CCE_REDUCTION_NONE || reduction > CCE_REDUCTION_SUM)
+    return fail(CCE_ERR_INVALID_ARG, "reduction must be 0 (none), 1 (mean) or 2 (sum), got %d", reduction);
+  *bytes = distill_layout(nullptr, N, d, V, reduction).bytes;
+  return CCE_OK;
+}
+
+int cce_distill_forward(const void* hidden, const void* weight, const float* bias, const cce_teacher* teacher,
+                        const void* labels, int labels_int64, int64_t N, int64_t d, int64_t V, int64_t ignore_index,
+                        int reduction, float* loss_out, float* stats_out, float* entry_logits_out, int32_t* rows_out,
+                        int32_t* n_valid_out, void* workspace, size_t workspace_bytes, void* stream) {
+  g_err[0] = 0;
+  int rc = check_dims(N, d, V);
+  Teacher a;
+  if (!rc) rc = check_teacher(teacher, N, labels, ignore_index, labels_int64, a);
+  if (rc) return rc;
+  if (reduction < CCE_REDUCTION_NONE || reduction > CCE_REDUCTION_SUM)
+    return fail(CCE_ERR_INVALID_ARG, "reduction must be 0 (none), 1 (mean) or 2 (sum), got %d", reduction);
+  if (!n_valid_out || (!loss_out && (N > 0 || reduction != CCE_REDUCTION_NONE)) ||
+      (N > 0 && (!hidden || !weight || !stats_out || !entry_logits_out || !rows_out)))
+    return fail(CCE_ERR_INVALID_ARG,
+                "hidden, weight, loss_out, stats_out, entry_logits_out, rows_out and n_valid_out must not be null");
+  if (misaligned(hidden) || misaligned(weight) || misaligned(stats_out) || misaligned(workspace))
+    return fail(CCE_ERR_INVALID_ARG, "hidden, weight, stats_out and workspace must be 16-byte aligned");
+  const DistillLayout need = distill_layout(nullptr, N, d, V, reduction);
+  if (workspace_bytes < need.bytes || !workspace)
+    return fail(CCE_ERR_WORKSPACE, "workspace too small: need %zu bytes, got %zu", need.bytes, workspace_bytes);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (N == 0) {
+    rc = zero_fill(n_valid_out, sizeof(int32_t), st);
+    if (!rc && reduction != CCE_REDUCTION_NONE) rc = zero_fill(loss_out, sizeof(float), st);
+    return rc;
+  }
+  return distill_forward_run(static_cast<const bf16_t*>(hidden), static_cast<const bf16_t*>(weight), bias, (long)N,
+                             (long)d, (long)V, a, reduction, loss_out, reinterpret_cast<float2*>(stats_out),
+                             entry_logits_out, rows_out, n_valid_out, distill_layout(workspace, N, d, V, reduction),
+                             st);
+}
+
+int cce_distill_backward_workspace_bytes(int64_t N, int64_t d, int64_t V, int64_t entries, int64_t chunk_size,
+                                         int need_grad_hidden, int grad_hidden_dtype, int need_grad_weight,
+                                         int grad_weight_dtype, size_t* bytes) {
+  const int rc = cce_backward_workspace_bytes(N, d, V, chunk_size, need_grad_hidden, grad_hidden_dtype,
+                                              need_grad_weight, grad_weight_dtype, bytes);
+  if (rc) return rc;
+  if (entries < 1 || entries > kMaxEntries)
+    return fail(CCE_ERR_INVALID_ARG, "a teacher has 1 to %d entries per row (got %ld)", kMaxEntries, (long)entries);
+  *bytes = bwd_layout(nullptr, N, d, V, band_width(V, chunk_size, N), need_grad_hidden != 0, need_grad_weight != 0,
+                      grad_hidden_dtype == CCE_DTYPE_F32, grad_weight_dtype == CCE_DTYPE_F32, (int)entries + 1).bytes;
+  return CCE_OK;
+}
+
+int cce_distill_backward(const float* grad_out, const void* hidden, const void* weight, const float* bias,
+                         const cce_teacher* teacher, const float* stats, const float* entry_logits,
+                         const int32_t* rows, const int32_t* n_valid, int64_t N, int64_t d, int64_t V, int reduction,
+                         int64_t chunk_size, void* grad_hidden, int grad_hidden_dtype, void* grad_weight,
+                         int grad_weight_dtype, float* grad_bias, void* workspace, size_t workspace_bytes,
+                         void* stream) {
+  g_err[0] = 0;
+  DistillGrad p;
+  const int rc = check_teacher(teacher, N, rows, -1, 0, p.a);
+  if (rc) return rc;
+  if (N > 0 && (!stats || !entry_logits || !rows))
+    return fail(CCE_ERR_INVALID_ARG, "stats, entry_logits and rows must not be null");
+  if (N > 0 && V > INT_MAX) return check_dims(N, d, V);
+  p.grad_out = grad_out;
+  p.stats = reinterpret_cast<const float2*>(stats);
+  p.xk = entry_logits;
+  p.rows = rows;
+  p.n_valid = n_valid;
+  p.reduction = reduction;
+  p.V = (int)V;
+  SparseGrad s;
+  s.scale = kLog2e * p.a.inv_t;
+  s.softmaxes = softmaxes_of(p.a);
+  s.entries = p.a.K + 1;
+  s.prep = distill_prep;
+  s.args = &p;
+  return backward_run(grad_out, hidden, weight, rows, 0, bias, stats, n_valid, N, d, V, -1, 0.f, 0.f, reduction,
+                      chunk_size, grad_hidden, grad_hidden_dtype, grad_weight, grad_weight_dtype, grad_bias, workspace,
+                      workspace_bytes, stream, &s);
+}
+
+int cce_top_logits(const void* logits, int logits_dtype, int64_t ld, int64_t N, int64_t V, int64_t k, void* values_out,
+                   int64_t* indices_out, void* stream) {
+  g_err[0] = 0;
+  const int rc = check_top(N, V, k, logits_dtype, ld);
+  if (rc) return rc;
+  if (N == 0) return CCE_OK;
+  if (!logits || !values_out || !indices_out)
+    return fail(CCE_ERR_INVALID_ARG, "logits, values_out and indices_out must not be null");
+  return logits_type(logits_dtype, [&](auto t) {
+    typedef decltype(t) T;
+    hipLaunchKernelGGL(top_logits_kernel<T>, dim3((unsigned)N), dim3(256), 0, reinterpret_cast<hipStream_t>(stream),
+                       static_cast<const T*>(logits), (long)ld, (int)V, (int)k, static_cast<T*>(values_out),
+                       indices_out);
+    HIP_TRY(hipGetLastError());
+    return CCE_OK;
+  });
+}
+
+int cce_layer_norm_forward(const void* x, int dtype, int64_t ldx, const void* weight, const void* bias,
+                           int param_dtype, int64_t N, int64_t D, float eps, void* y_out, float* mean_out,
+                           float* rstd_out, void* stream) {
+  g_err[0] = 0;
+  const int rc = check_norm(N, D, dtype, ldx, param_dtype);
+  if (rc) return rc;
+  if (!(eps >= 0.f && eps < INFINITY)) return fail(CCE_ERR_INVALID_ARG, "eps must be finite and at least 0");
+  if (N == 0) return CCE_OK;
+  if (!x || !y_out || !mean_out || !rstd_out)
+    return fail(CCE_ERR_INVALID_ARG, "x, y_out, mean_out and rstd_out must not be null");
+  return norm_forward(x, dtype, ldx, weight, bias, param_dtype, N, D, eps, y_out, mean_out, rstd_out,
+                      reinterpret_cast<hipStream_t>(stream));
+}
+
+int cce_layer_norm_backward_workspace_bytes(int64_t N, int64_t D, size_t* bytes) {
+  g_err[0] = 0;
+  if (!bytes) return fail(CCE_ERR_INVALID_ARG, "bytes must not be null");
+  const int rc = check_norm(N, D, CCE_DTYPE_F32, D, CCE_DTYPE_F32);
+  if (rc) return rc;
+  *bytes = norm_layout(nullptr, N, D).bytes;
+  return CCE_OK;
+}
+
+int cce_layer_norm_backward(const void* grad_y, const void* x, int dtype, int64_t ldx, const void* weight,
+                            int param_dtype, const float* mean, const float* rstd, int64_t N, int64_t D, void* grad_x,
+                            void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
+                            void* stream) {
+  g_err[0] = 0;
+  const int rc = check_norm(N, D, dtype, ldx, param_dtype);
+  if (rc) return rc;
+  if (N > 0 && (!grad_y || !x || !mean || !rstd))
+    return fail(CCE_ERR_INVALID_ARG, "grad_y, x, mean and rstd must not be null");
+  if (misaligned(workspace)) return fail(CCE_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
+  const NormLayout need = norm_layout(nullptr, N, D);
+  if (workspace_bytes < need.bytes || !workspace)
+    return fail(CCE_ERR_WORKSPACE, "workspace too small: need %zu bytes, got %zu", need.bytes, workspace_bytes);
+  return norm_backward(grad_y, x, dtype, ldx, weight, param_dtype, mean, rstd, N, D, grad_x, grad_weight, grad_bias,
+                       norm_layout(workspace, N, D), reinterpret_cast<hipStream_t>(stream));
 }
 
 int cce_kernel_timing_enable(int enable) {

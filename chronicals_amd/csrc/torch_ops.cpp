@@ -22,6 +22,7 @@
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "../../include/chronicals_cce.h"
@@ -41,6 +42,17 @@ struct Api {
   decltype(&cce_logits_forward) logits_forward;
   decltype(&cce_logits_backward) logits_backward;
   decltype(&cce_logits_forward_backward) logits_forward_backward;
+  decltype(&cce_distill_logits_workspace_bytes) distill_logits_workspace_bytes;
+  decltype(&cce_distill_logits_forward) distill_logits_forward;
+  decltype(&cce_distill_logits_backward) distill_logits_backward;
+  decltype(&cce_distill_forward_workspace_bytes) distill_forward_workspace_bytes;
+  decltype(&cce_distill_forward) distill_forward;
+  decltype(&cce_distill_backward_workspace_bytes) distill_backward_workspace_bytes;
+  decltype(&cce_distill_backward) distill_backward;
+  decltype(&cce_top_logits) top_logits;
+  decltype(&cce_layer_norm_forward) layer_norm_forward;
+  decltype(&cce_layer_norm_backward_workspace_bytes) layer_norm_backward_workspace_bytes;
+  decltype(&cce_layer_norm_backward) layer_norm_backward;
 };
 
 Api g_api;
@@ -92,21 +104,25 @@ Tensor aligned(const Tensor& t) {
 
 bool is_label(const Tensor& t) { return t.scalar_type() == at::kLong || t.scalar_type() == at::kInt; }
 
-void check_operands(const Tensor& hidden, const Tensor& weight, const Tensor& labels, const optional<Tensor>& bias) {
+void check_head(const Tensor& hidden, const Tensor& weight, const optional<Tensor>& bias) {
   TORCH_CHECK(hidden.scalar_type() == at::kBFloat16 && weight.scalar_type() == at::kBFloat16,
               "cce ops take bf16 hidden and weight, got ", hidden.scalar_type(), " and ", weight.scalar_type());
   TORCH_CHECK(hidden.dim() == 2 && weight.dim() == 2 && hidden.size(1) == weight.size(1),
               "cce ops take hidden [N, d] and weight [V, d], got ", hidden.sizes(), " and ", weight.sizes());
-  TORCH_CHECK(labels.dim() == 1 && labels.size(0) == hidden.size(0) && is_label(labels),
-              "cce ops take int64/int32 labels [N], got ", labels.scalar_type(), " ", labels.sizes());
   TORCH_CHECK(hidden.is_contiguous(), "hidden must be contiguous");
   TORCH_CHECK(weight.is_contiguous(), "weight must be contiguous");
-  TORCH_CHECK(hidden.device() == weight.device() && hidden.device() == labels.device(),
-              "hidden, weight and labels must be on the same device");
+  TORCH_CHECK(hidden.device() == weight.device(), "hidden and weight must be on the same device");
   if (bias.has_value())
     TORCH_CHECK(bias->scalar_type() == at::kFloat && bias->dim() == 1 && bias->size(0) == weight.size(0) &&
                     bias->is_contiguous() && bias->device() == hidden.device(),
                 "bias must be a contiguous fp32 [V] tensor");
+}
+
+void check_operands(const Tensor& hidden, const Tensor& weight, const Tensor& labels, const optional<Tensor>& bias) {
+  check_head(hidden, weight, bias);
+  TORCH_CHECK(labels.dim() == 1 && labels.size(0) == hidden.size(0) && is_label(labels),
+              "cce ops take int64/int32 labels [N], got ", labels.scalar_type(), " ", labels.sizes());
+  TORCH_CHECK(hidden.device() == labels.device(), "hidden, weight and labels must be on the same device");
 }
 
 const float* bias_ptr(const optional<Tensor>& bias) {
@@ -267,6 +283,252 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> ce_logits_fwd_bwd(const Tensor& logit
   return {o.loss, o.lse, o.n_valid, dx};
 }
 
+// ---------------------------------------------------------------------------
+// Distillation, the teacher's top logits, layer norm
+// ---------------------------------------------------------------------------
+
+float* f32(const Tensor& t) { return static_cast<float*>(t.data_ptr()); }
+
+bool is_logits(const Tensor& t) {
+  return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf || t.scalar_type() == at::kFloat;
+}
+
+// What a forward kept, as it came.
+void check_kept(const Tensor& t, const char* name, at::ScalarType type, int64_t numel, const Tensor& student) {
+  TORCH_CHECK(t.scalar_type() == type && t.numel() == numel && t.is_contiguous() && t.device() == student.device(), name,
+              " must be the forward's output (", numel, " contiguous ", type, " values), got ", t.scalar_type(), " ",
+              t.sizes());
+}
+
+// A teacher's entries with what they need checked against N student rows.
+struct TeacherArgs {
+  cce_teacher t;
+  TeacherArgs(const Tensor& logits, const Tensor& indices, const Tensor& student, int64_t N, double temperature,
+              double distill_weight, double ce_weight) {
+    TORCH_CHECK(is_logits(logits), "teacher logits dtype ", logits.scalar_type(), " not supported (bf16, fp16, fp32)");
+    TORCH_CHECK(logits.dim() == 2 && logits.size(0) == N && indices.sizes() == logits.sizes() && is_label(indices),
+                "distill ops take teacher logits [N = ", N, ", K] and int64/int32 indices of the same shape, got ",
+                logits.sizes(), " and ", indices.scalar_type(), " ", indices.sizes());
+    TORCH_CHECK(logits.is_contiguous() && indices.is_contiguous(), "teacher logits and indices must be contiguous");
+    TORCH_CHECK(logits.device() == student.device() && indices.device() == student.device(),
+                "teacher logits and indices must be on the student's device");
+    t.logits = logits.data_ptr();
+    t.indices = indices.data_ptr();
+    t.entries = logits.size(1);
+    t.logits_dtype = logits_dtype(logits);
+    t.indices_int64 = indices.scalar_type() == at::kLong;
+    t.temperature = (float)temperature;
+    t.distill_weight = (float)distill_weight;
+    t.ce_weight = (float)ce_weight;
+  }
+};
+
+void check_row_labels(const optional<Tensor>& labels, const Tensor& student, int64_t N) {
+  if (!labels.has_value()) return;
+  TORCH_CHECK(labels->dim() == 1 && labels->size(0) == N && is_label(*labels) && labels->is_contiguous(),
+              "distill ops take contiguous int64/int32 labels [N = ", N, "], got ", labels->scalar_type(), " ",
+              labels->sizes());
+  TORCH_CHECK(labels->device() == student.device(), "labels must be on the student's device");
+}
+
+const void* label_ptr(const optional<Tensor>& labels) { return labels.has_value() ? labels->data_ptr() : nullptr; }
+int label_int64(const optional<Tensor>& labels) { return labels.has_value() && labels->scalar_type() == at::kLong; }
+
+void check_student_logits(const Tensor& logits) {
+  logits_dtype(logits);
+  TORCH_CHECK(logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1),
+              "distill ops take [N, V] logits with a contiguous last dimension, got shape ", logits.sizes(),
+              " strides ", logits.strides());
+}
+
+std::tuple<Tensor, Tensor, Tensor> distill_logits_fwd(const Tensor& logits, const Tensor& teacher_logits,
+                                                      const Tensor& teacher_indices, const optional<Tensor>& labels,
+                                                      double temperature, double distill_weight, double ce_weight,
+                                                      int64_t ignore_index, int64_t reduction) {
+  check_student_logits(logits);
+  const int64_t N = logits.size(0), V = logits.size(1);
+  check_row_labels(labels, logits, N);
+  const TeacherArgs teacher(teacher_logits, teacher_indices, logits, N, temperature, distill_weight, ce_weight);
+  const Api& a = api();
+  const c10::DeviceGuard guard(logits.device());
+  size_t bytes = 0;
+  check(a, a.distill_logits_workspace_bytes(N, V, (int)reduction, &bytes));
+  const auto opt = logits.options().dtype(at::kFloat);
+  const Tensor ws = at::empty({(int64_t)bytes}, logits.options().dtype(at::kByte));
+  Tensor loss = at::empty({reduction == CCE_REDUCTION_NONE ? N : 1}, opt), stats = at::empty({N, 4}, opt);
+  Tensor n_valid = at::empty({1}, logits.options().dtype(at::kInt));
+  check(a, a.distill_logits_forward(logits.data_ptr(), logits_dtype(logits), row_stride(logits), &teacher.t,
+                                    label_ptr(labels), label_int64(labels), N, V, ignore_index, (int)reduction,
+                                    f32(loss), f32(stats), static_cast<int32_t*>(n_valid.data_ptr()), ws.data_ptr(),
+                                    bytes, stream(logits.device())));
+  return {loss, stats, n_valid};
+}
+
+Tensor distill_logits_bwd(const Tensor& grad_out, const Tensor& logits, const Tensor& teacher_logits,
+                          const Tensor& teacher_indices, const optional<Tensor>& labels, const Tensor& stats,
+                          const Tensor& n_valid, double temperature, double distill_weight, double ce_weight,
+                          int64_t ignore_index, int64_t reduction) {
+  check_student_logits(logits);
+  const int64_t N = logits.size(0), V = logits.size(1);
+  check_row_labels(labels, logits, N);
+  const TeacherArgs teacher(teacher_logits, teacher_indices, logits, N, temperature, distill_weight, ce_weight);
+  const Api& a = api();
+  const c10::DeviceGuard guard(logits.device());
+  Tensor dx = at::empty(logits.sizes(), logits.options());
+  const Tensor g = grad_rows(grad_out);
+  check_kept(g, "grad_out", at::kFloat, reduction == CCE_REDUCTION_NONE ? N : 1, logits);
+  check_kept(stats, "stats", at::kFloat, 4 * N, logits);
+  check_kept(n_valid, "n_valid", at::kInt, 1, logits);
+  check(a, a.distill_logits_backward(f32(g), logits.data_ptr(), logits_dtype(logits), row_stride(logits), &teacher.t,
+                                     label_ptr(labels), label_int64(labels), f32(stats),
+                                     static_cast<const int32_t*>(n_valid.data_ptr()), N, V, ignore_index,
+                                     (int)reduction, dx.data_ptr(), row_stride(dx), stream(logits.device())));
+  return dx;
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> distill_fwd(
+    const Tensor& hidden_, const Tensor& weight_, const optional<Tensor>& bias, const Tensor& teacher_logits,
+    const Tensor& teacher_indices, const optional<Tensor>& labels, double temperature, double distill_weight,
+    double ce_weight, int64_t ignore_index, int64_t reduction) {
+  check_head(hidden_, weight_, bias);
+  const int64_t N = hidden_.size(0), d = hidden_.size(1), V = weight_.size(0);
+  check_row_labels(labels, hidden_, N);
+  const TeacherArgs teacher(teacher_logits, teacher_indices, hidden_, N, temperature, distill_weight, ce_weight);
+  const Api& a = api();
+  const c10::DeviceGuard guard(hidden_.device());
+  const Tensor hidden = aligned(hidden_), weight = aligned(weight_);
+  size_t bytes = 0;
+  check(a, a.distill_forward_workspace_bytes(N, d, V, (int)reduction, &bytes));
+  const auto opt = hidden.options().dtype(at::kFloat), i32 = hidden.options().dtype(at::kInt);
+  const Tensor ws = at::empty({(int64_t)bytes}, hidden.options().dtype(at::kByte));
+  Tensor loss = at::empty({reduction == CCE_REDUCTION_NONE ? N : 1}, opt), stats = at::empty({N, 2}, opt);
+  Tensor entry_logits = at::empty({N, teacher.t.entries + 1}, opt), rows = at::empty({N}, i32);
+  Tensor n_valid = at::empty({1}, i32);
+  check(a, a.distill_forward(hidden.data_ptr(), weight.data_ptr(), bias_ptr(bias), &teacher.t, label_ptr(labels),
+                             label_int64(labels), N, d, V, ignore_index, (int)reduction, f32(loss), f32(stats),
+                             f32(entry_logits), static_cast<int32_t*>(rows.data_ptr()),
+                             static_cast<int32_t*>(n_valid.data_ptr()), ws.data_ptr(), bytes,
+                             stream(hidden.device())));
+  return {loss, stats, entry_logits, rows, n_valid};
+}
+
+std::tuple<Tensor, Tensor, Tensor> distill_bwd(const Tensor& grad_out, const Tensor& hidden_, const Tensor& weight_,
+                                               const optional<Tensor>& bias, const Tensor& teacher_logits,
+                                               const Tensor& teacher_indices, const Tensor& stats,
+                                               const Tensor& entry_logits, const Tensor& rows, const Tensor& n_valid,
+                                               double temperature, double distill_weight, double ce_weight,
+                                               int64_t reduction, int64_t chunk_size, bool need_dh, bool need_dw,
+                                               bool need_db, bool dh_f32, bool dw_f32) {
+  check_head(hidden_, weight_, bias);
+  TORCH_CHECK(!need_db || bias.has_value(), "need_db requires a bias");
+  const int64_t N = hidden_.size(0), d = hidden_.size(1), V = weight_.size(0);
+  const TeacherArgs teacher(teacher_logits, teacher_indices, hidden_, N, temperature, distill_weight, ce_weight);
+  const Api& a = api();
+  const c10::DeviceGuard guard(hidden_.device());
+  const Tensor hidden = aligned(hidden_), weight = aligned(weight_);
+  const Tensor g = grad_rows(grad_out);
+  check_kept(g, "grad_out", at::kFloat, reduction == CCE_REDUCTION_NONE ? N : 1, hidden);
+  check_kept(stats, "stats", at::kFloat, 2 * N, hidden);
+  check_kept(entry_logits, "entry_logits", at::kFloat, N * (teacher.t.entries + 1), hidden);
+  check_kept(rows, "rows", at::kInt, N, hidden);
+  check_kept(n_valid, "n_valid", at::kInt, 1, hidden);
+  const auto opt = hidden.options().dtype(at::kFloat);
+  auto empty = [&](bool need, at::IntArrayRef size, bool f) {
+    return at::empty(need ? size : at::IntArrayRef{0}, f ? opt : hidden.options());
+  };
+  Tensor dh = empty(need_dh, {N, d}, dh_f32), dw = empty(need_dw, {V, d}, dw_f32), db = empty(need_db, {V}, true);
+  if (need_dh || need_dw || need_db) {
+    const int hdt = dh_f32 ? CCE_DTYPE_F32 : CCE_DTYPE_BF16, wdt = dw_f32 ? CCE_DTYPE_F32 : CCE_DTYPE_BF16;
+    size_t bytes = 0;
+    check(a, a.distill_backward_workspace_bytes(N, d, V, teacher.t.entries, chunk_size, need_dh, hdt, need_dw, wdt,
+                                                &bytes));
+    const Tensor ws = at::empty({(int64_t)bytes}, hidden.options().dtype(at::kByte));
+    check(a, a.distill_backward(f32(g), hidden.data_ptr(), weight.data_ptr(), bias_ptr(bias), &teacher.t, f32(stats),
+                                f32(entry_logits), static_cast<const int32_t*>(rows.data_ptr()),
+                                static_cast<const int32_t*>(n_valid.data_ptr()), N, d, V, (int)reduction, chunk_size,
+                                need_dh ? dh.data_ptr() : nullptr, hdt, need_dw ? dw.data_ptr() : nullptr, wdt,
+                                need_db ? f32(db) : nullptr, ws.data_ptr(), bytes, stream(hidden.device())));
+  }
+  return {dh, dw, db};
+}
+
+std::tuple<Tensor, Tensor> top_logits(const Tensor& logits, int64_t k) {
+  logits_dtype(logits);
+  TORCH_CHECK(logits.dim() == 2 && (logits.size(1) <= 1 || logits.stride(1) == 1),
+              "top_logits takes [N, V] logits with a contiguous last dimension, got shape ", logits.sizes(),
+              " strides ", logits.strides());
+  const Api& a = api();
+  const c10::DeviceGuard guard(logits.device());
+  const int64_t N = logits.size(0), V = logits.size(1);
+  TORCH_CHECK(k >= 1 && k <= std::min<int64_t>(V, CCE_MAX_TEACHER_ENTRIES), "k must be in [1, min(",
+              CCE_MAX_TEACHER_ENTRIES, ", V = ", V, ")], got ", k);
+  Tensor values = at::empty({N, k}, logits.options()), indices = at::empty({N, k}, logits.options().dtype(at::kLong));
+  check(a, a.top_logits(logits.data_ptr(), logits_dtype(logits), row_stride(logits), N, V, k, values.data_ptr(),
+                        static_cast<int64_t*>(indices.data_ptr()), stream(logits.device())));
+  return {values, indices};
+}
+
+// The parameters' type: that of the weight or, without one, of the bias.
+int check_norm(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias) {
+  TORCH_CHECK(is_logits(x), "layer_norm dtype ", x.scalar_type(), " not supported (bf16, fp16, fp32)");
+  TORCH_CHECK(x.dim() == 2 && (x.size(1) <= 1 || x.stride(1) == 1),
+              "layer_norm ops take [N, D] rows with a contiguous last dimension, got shape ", x.sizes(), " strides ",
+              x.strides());
+  at::ScalarType type = x.scalar_type();
+  for (const optional<Tensor>* p : {&bias, &weight}) {
+    if (!p->has_value()) continue;
+    const Tensor& t = **p;
+    TORCH_CHECK(t.dim() == 1 && t.size(0) == x.size(1) && t.is_contiguous() && t.device() == x.device(),
+                "weight and bias must be contiguous [D] tensors on the input's device, got ", t.sizes());
+    type = t.scalar_type();
+    TORCH_CHECK(type == x.scalar_type() || type == at::kFloat, "weight and bias must have the input's dtype or fp32, got ",
+                type);
+  }
+  TORCH_CHECK(!weight.has_value() || !bias.has_value() || weight->scalar_type() == bias->scalar_type(),
+              "weight and bias must have the same dtype");
+  return type == at::kFloat ? CCE_DTYPE_F32 : logits_dtype(x);
+}
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm_fwd(const Tensor& x, const optional<Tensor>& weight,
+                                                  const optional<Tensor>& bias, double eps) {
+  const int pdt = check_norm(x, weight, bias);
+  const Api& a = api();
+  const c10::DeviceGuard guard(x.device());
+  const int64_t N = x.size(0), D = x.size(1);
+  const auto opt = x.options().dtype(at::kFloat);
+  Tensor y = at::empty({N, D}, x.options()), mean = at::empty({N}, opt), rstd = at::empty({N}, opt);
+  check(a, a.layer_norm_forward(x.data_ptr(), logits_dtype(x), row_stride(x), label_ptr(weight), label_ptr(bias), pdt,
+                                N, D, (float)eps, y.data_ptr(), f32(mean), f32(rstd), stream(x.device())));
+  return {y, mean, rstd};
+}
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor& grad_y, const Tensor& x, const optional<Tensor>& weight,
+                                                  const Tensor& mean, const Tensor& rstd, bool param_f32, bool need_dx,
+                                                  bool need_dw, bool need_db) {
+  const int wdt = check_norm(x, weight, std::nullopt);
+  const int pdt = param_f32 ? CCE_DTYPE_F32 : logits_dtype(x);
+  TORCH_CHECK(!weight.has_value() || wdt == pdt, "param_f32 does not fit the weight's dtype");
+  TORCH_CHECK(grad_y.sizes() == x.sizes() && grad_y.scalar_type() == x.scalar_type() && grad_y.is_contiguous() &&
+                  grad_y.device() == x.device(),
+              "grad_y must be a contiguous tensor of the input's shape, dtype and device");
+  const int64_t N = x.size(0), D = x.size(1);
+  check_kept(mean, "mean", at::kFloat, N, x);
+  check_kept(rstd, "rstd", at::kFloat, N, x);
+  const Api& a = api();
+  const c10::DeviceGuard guard(x.device());
+  const auto popt = x.options().dtype(param_f32 ? at::kFloat : x.scalar_type());
+  Tensor dx = at::empty(need_dx ? x.sizes() : at::IntArrayRef{0}, x.options());
+  Tensor dw = at::empty({need_dw ? D : 0}, popt), db = at::empty({need_db ? D : 0}, popt);
+  size_t bytes = 0;
+  check(a, a.layer_norm_backward_workspace_bytes(N, D, &bytes));
+  const Tensor ws = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+  check(a, a.layer_norm_backward(grad_y.data_ptr(), x.data_ptr(), logits_dtype(x), row_stride(x), label_ptr(weight),
+                                 pdt, f32(mean), f32(rstd), N, D, need_dx ? dx.data_ptr() : nullptr,
+                                 need_dw ? dw.data_ptr() : nullptr, need_db ? db.data_ptr() : nullptr, ws.data_ptr(),
+                                 bytes, stream(x.device())));
+  return {dx, dw, db};
+}
+
 }  // namespace
 
 extern "C" {
@@ -288,6 +550,17 @@ int chronicals_torch_bind(void* handle) {
   get(a.logits_forward, "cce_logits_forward");
   get(a.logits_backward, "cce_logits_backward");
   get(a.logits_forward_backward, "cce_logits_forward_backward");
+  get(a.distill_logits_workspace_bytes, "cce_distill_logits_workspace_bytes");
+  get(a.distill_logits_forward, "cce_distill_logits_forward");
+  get(a.distill_logits_backward, "cce_distill_logits_backward");
+  get(a.distill_forward_workspace_bytes, "cce_distill_forward_workspace_bytes");
+  get(a.distill_forward, "cce_distill_forward");
+  get(a.distill_backward_workspace_bytes, "cce_distill_backward_workspace_bytes");
+  get(a.distill_backward, "cce_distill_backward");
+  get(a.top_logits, "cce_top_logits");
+  get(a.layer_norm_forward, "cce_layer_norm_forward");
+  get(a.layer_norm_backward_workspace_bytes, "cce_layer_norm_backward_workspace_bytes");
+  get(a.layer_norm_backward, "cce_layer_norm_backward");
   if (!ok) return 1;
   if (!g_bound.load(std::memory_order_acquire)) {
     g_api = a;
@@ -313,11 +586,20 @@ TORCH_LIBRARY_IMPL(chronicals_hip, CUDA, m) {
   m.impl("ce_logits_fwd", ce_logits_fwd);
   m.impl("ce_logits_bwd", ce_logits_bwd);
   m.impl("ce_logits_fwd_bwd", ce_logits_fwd_bwd);
+  m.impl("distill_logits_fwd", distill_logits_fwd);
+  m.impl("distill_logits_bwd", distill_logits_bwd);
+  m.impl("distill_fwd", distill_fwd);
+  m.impl("distill_bwd", distill_bwd);
+  m.impl("top_logits", top_logits);
+  m.impl("layer_norm_fwd", layer_norm_fwd);
+  m.impl("layer_norm_bwd", layer_norm_bwd);
 }
 
 // The operators have no derivative of their own (the autograd functions call
 // them): a backward through one raises.
 TORCH_LIBRARY_IMPL(chronicals_hip, Autograd, m) {
-  for (const char* op : {"cce_fwd", "cce_bwd", "ce_logits_fwd", "ce_logits_bwd", "ce_logits_fwd_bwd"})
+  for (const char* op : {"cce_fwd", "cce_bwd", "ce_logits_fwd", "ce_logits_bwd", "ce_logits_fwd_bwd",
+                         "distill_logits_fwd", "distill_logits_bwd", "distill_fwd", "distill_bwd", "top_logits",
+                         "layer_norm_fwd", "layer_norm_bwd"})
     m.impl(op, torch::autograd::autogradNotImplementedFallback());
 }

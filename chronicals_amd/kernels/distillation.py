@@ -1,0 +1,305 @@
+"""Distillation from a teacher's top logits, on MI355X.
+
+A teacher's answer for a token is kept as its K largest logits and their columns
+(``top_logits``).  The student is trained towards softmax(t / T) over those K, in
+the two forms that the cross-entropy has here:
+
+  distillation_loss, DistillationLoss
+      over student logits that exist (as ``chunked_cross_entropy_loss``): the
+      forward streams them once, the backward again, writing the gradient.
+  linear_distillation_loss, LinearDistillationLoss
+      from hidden states and the head's weight (as ``cut_cross_entropy``): the
+      student's N x V logits are never stored.
+
+Per row, with q = softmax(t / T) over the row's usable entries (t_k, i_k):
+
+  distill_weight * T^2 * sum_k q_k * (log q_k - log softmax(x / T)[i_k])
+    + ce_weight * (logsumexp(x) - x[label])
+
+so with ``ce_weight`` the labels' loss comes from the same passes.
+
+  * An entry whose index is outside [0, V) (use -1 as padding) or whose logit is
+    -inf takes no part, whatever else it holds; a row left without any has no
+    distillation term.  Entries that share an index add up there.
+  * ``labels``: a row labelled ``ignore_index`` gives no loss and a zero gradient.
+    A label outside [0, V) that is not ``ignore_index`` has no target logit.
+    Without labels (``ce_weight`` is 0 then) a row counts if it has a usable entry.
+  * 'mean' divides by the number of rows that count, at least 1; 'sum' adds them;
+    'none' returns one value per row, in the shape of the rows.
+  * K is at most 256, the temperature in [0.01, 1000].
+  * Losses are fp32.  Sums are added in a fixed order: the same bits on every run.
+  * Tensors must live on a HIP device; there is no CPU path.  The teacher's
+    tensors get no gradient, and gradients cannot be differentiated again.
+  * ``linear_distillation_loss`` computes in bf16 with fp32 accumulation (fp16 and
+    fp32 operands are rounded to bf16 at the boundary) and rounds the gradient of
+    the logits to bf16 once, as ``cut_cross_entropy`` does; gradients come back in
+    the input dtypes.
+
+The reference has no distillation; the argument order follows its losses.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from .. import _lib
+from .. import ops as _ops  # noqa: F401  (registers chronicals_hip::distill_* and top_logits)
+from .cut_cross_entropy import _as_bf16_rows, _reduction_code, get_optimal_chunk_size
+
+__all__ = [
+    "top_logits",
+    "distillation_loss",
+    "DistillationLoss",
+    "DistillationFunction",
+    "linear_distillation_loss",
+    "LinearDistillationLoss",
+    "LinearDistillationFunction",
+]
+
+MAX_ENTRIES = _lib.CCE_MAX_TEACHER_ENTRIES
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+_INTS = (torch.int64, torch.int32)
+
+
+def _check(cond: bool, msg: str) -> None:
+    if not cond:
+        raise RuntimeError(msg)
+
+
+def _logit_rows(logits: torch.Tensor) -> torch.Tensor:
+    """[..., V] as [N, V] with a contiguous last dimension and rows that do not overlap."""
+    x = logits.reshape(-1, logits.shape[-1])
+    if (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        x = x.contiguous()
+    return x
+
+
+def _check_student(x: torch.Tensor, name: str, what: str) -> None:
+    _check(x.is_cuda, f"chronicals_amd {what} runs only on HIP devices: {name} must be a device tensor (got "
+                      f"{x.device})")
+    _check(x.dim() >= 1 and x.shape[-1] >= 1, f"{name} must be [..., D] with D >= 1, got shape {tuple(x.shape)}")
+    _check(x.dtype in _FLOATS, f"{name} dtype {x.dtype} not supported (bf16, fp16, fp32)")
+
+
+def _teacher_rows(student: torch.Tensor, teacher_logits: torch.Tensor, teacher_indices: torch.Tensor,
+                  labels: Optional[torch.Tensor], temperature: float, ce_weight: float):
+    """The teacher's tensors as contiguous [N, K] and the labels as [N], for a student of shape [..., D]."""
+    lead = student.shape[:-1]
+    n = lead.numel()
+    _check(teacher_logits.dim() >= 1 and teacher_logits.shape[:-1] == lead,
+           f"teacher_logits must be [{', '.join(map(str, lead))}, K], got {tuple(teacher_logits.shape)}")
+    _check(teacher_indices.shape == teacher_logits.shape,
+           f"teacher_indices must have the shape {tuple(teacher_logits.shape)} of teacher_logits, got "
+           f"{tuple(teacher_indices.shape)}")
+    k = teacher_logits.shape[-1]
+    _check(1 <= k <= MAX_ENTRIES, f"a teacher has 1 to {MAX_ENTRIES} entries per row, got {k}")
+    _check(teacher_logits.dtype in _FLOATS, f"teacher_logits dtype {teacher_logits.dtype} not supported (bf16, fp16, "
+                                            "fp32)")
+    _check(teacher_indices.dtype in _INTS, f"teacher_indices must be int64 or int32, got {teacher_indices.dtype}")
+    _check(teacher_logits.device == student.device and teacher_indices.device == student.device,
+           "teacher_logits and teacher_indices must be on the student's device")
+    if not 1e-2 <= temperature <= 1e3:
+        raise ValueError(f"temperature must be in [0.01, 1000], got {temperature}")
+    if labels is None:
+        if ce_weight != 0.0:
+            raise ValueError("ce_weight needs labels")
+        lab = None
+    else:
+        _check(labels.dtype in _INTS, f"labels must be int64 or int32, got {labels.dtype}")
+        _check(labels.numel() == n, f"labels has {labels.numel()} elements but the student has {n} rows")
+        _check(labels.device == student.device, "labels must be on the student's device")
+        lab = labels.reshape(-1).contiguous()
+    return teacher_logits.detach().reshape(n, k).contiguous(), teacher_indices.reshape(n, k).contiguous(), lab
+
+
+def top_logits(logits: torch.Tensor, k: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The k largest of each row of [..., V] logits, largest first, and their indices (int64): [..., k] each.
+
+    Among equal values the lower index comes first; NaN is larger than any
+    number and -0 equals +0.  1 <= k <= min(V, 256).  Not differentiable: a
+    teacher's answer.
+    """
+    _check_student(logits, "logits", "top_logits")
+    V = logits.shape[-1]
+    if not 1 <= k <= min(V, MAX_ENTRIES):
+        raise ValueError(f"k must be in [1, min({MAX_ENTRIES}, V = {V})], got {k}")
+    values, indices = torch.ops.chronicals_hip.top_logits(_logit_rows(logits.detach()), int(k))
+    shape = (*logits.shape[:-1], k)
+    return values.view(shape), indices.view(shape)
+
+
+class DistillationFunction(torch.autograd.Function):
+    """apply(logits2d, teacher_logits, teacher_indices, labels, temperature, distill_weight, ce_weight, ignore_index,
+    reduction_code) -> loss (scalar, or [N] for 'none').  Keeps four floats per row beyond the inputs."""
+
+    @staticmethod
+    def forward(ctx, x, t, index, labels, temperature, distill_weight, ce_weight, ignore_index, red):
+        how = (float(temperature), float(distill_weight), float(ce_weight), int(ignore_index), int(red))
+        loss, stats, n_valid = torch.ops.chronicals_hip.distill_logits_fwd(x, t, index, labels, *how)
+        ctx.save_for_backward(x, t, index, labels, stats, n_valid)
+        ctx.how = how
+        return loss if red == _lib.CCE_REDUCTION_NONE else loss.view(())
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_output):
+        if not ctx.needs_input_grad[0]:
+            return (None,) * 9
+        x, t, index, labels, stats, n_valid = ctx.saved_tensors
+        dx = torch.ops.chronicals_hip.distill_logits_bwd(grad_output, x, t, index, labels, stats, n_valid, *ctx.how)
+        return (dx,) + (None,) * 8
+
+
+def distillation_loss(
+    logits: torch.Tensor,
+    teacher_logits: torch.Tensor,
+    teacher_indices: torch.Tensor,
+    labels: Optional[torch.Tensor] = None,
+    temperature: float = 1.0,
+    distill_weight: float = 1.0,
+    ce_weight: float = 0.0,
+    ignore_index: int = -100,
+    reduction: str = "mean",
+) -> torch.Tensor:
+    """Distillation loss over student logits [..., V] that exist (module docstring); differentiable in ``logits``.
+
+    teacher_logits and teacher_indices [..., K]; labels [...] or None.
+    """
+    red = _reduction_code(reduction)
+    _check_student(logits, "logits", "distillation_loss")
+    t, index, lab = _teacher_rows(logits, teacher_logits, teacher_indices, labels, temperature, ce_weight)
+    loss = DistillationFunction.apply(_logit_rows(logits), t, index, lab, temperature, distill_weight, ce_weight,
+                                      ignore_index, red)
+    return loss.view(logits.shape[:-1]) if red == _lib.CCE_REDUCTION_NONE else loss
+
+
+class DistillationLoss(nn.Module):
+    """Module form of distillation_loss."""
+
+    def __init__(self, temperature: float = 1.0, distill_weight: float = 1.0, ce_weight: float = 0.0,
+                 ignore_index: int = -100, reduction: str = "mean"):
+        super().__init__()
+        _reduction_code(reduction)
+        self.temperature = temperature
+        self.distill_weight = distill_weight
+        self.ce_weight = ce_weight
+        self.ignore_index = ignore_index
+        self.reduction = reduction
+
+    def forward(self, logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_indices: torch.Tensor,
+                labels: Optional[torch.Tensor] = None) -> torch.Tensor:
+        return distillation_loss(logits, teacher_logits, teacher_indices, labels, self.temperature,
+                                 self.distill_weight, self.ce_weight, self.ignore_index, self.reduction)
+
+    def extra_repr(self) -> str:
+        return (f"temperature={self.temperature}, distill_weight={self.distill_weight}, "
+                f"ce_weight={self.ce_weight}, ignore_index={self.ignore_index}, reduction={self.reduction!r}")
+
+
+class LinearDistillationFunction(torch.autograd.Function):
+    """apply(hidden, weight, bias, teacher_logits, teacher_indices, labels, chunk_size, temperature, distill_weight,
+    ce_weight, ignore_index, reduction_code) -> loss (scalar, or [N] for 'none').
+
+    Keeps the bf16 operands and, per row, K + 4 numbers of 32 bits.
+    """
+
+    @staticmethod
+    def forward(ctx, hidden, weight, bias, t, index, labels, chunk_size, temperature, distill_weight, ce_weight,
+                ignore_index, red):
+        h2 = _as_bf16_rows(hidden.detach().reshape(-1, hidden.shape[-1]))
+        w2 = _as_bf16_rows(weight.detach())
+        b32 = None if bias is None else bias.detach().to(torch.float32).contiguous()
+        how = (float(temperature), float(distill_weight), float(ce_weight))
+        loss, stats, entry_logits, rows, n_valid = torch.ops.chronicals_hip.distill_fwd(
+            h2, w2, b32, t, index, labels, *how, int(ignore_index), int(red))
+        ctx.save_for_backward(h2, w2, b32, t, index, stats, entry_logits, rows, n_valid)
+        ctx.cfg = (how, int(red), int(chunk_size))
+        ctx.shapes = (hidden.shape, hidden.dtype, weight.dtype, None if bias is None else bias.dtype)
+        return loss if red == _lib.CCE_REDUCTION_NONE else loss.view(())
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_output):
+        h2, w2, b32, t, index, stats, entry_logits, rows, n_valid = ctx.saved_tensors
+        how, red, chunk_size = ctx.cfg
+        hshape, hdtype, wdtype, bdtype = ctx.shapes
+        need_dh, need_dw, need_db = ctx.needs_input_grad[:3]
+        if not (need_dh or need_dw or need_db):
+            return (None,) * 12
+        dh, dw, db = torch.ops.chronicals_hip.distill_bwd(
+            grad_output, h2, w2, b32, t, index, stats, entry_logits, rows, n_valid, *how, red, chunk_size, need_dh,
+            need_dw, need_db, hdtype != torch.bfloat16, wdtype != torch.bfloat16)
+        return (dh.view(hshape).to(hdtype) if need_dh else None, dw.to(wdtype) if need_dw else None,
+                db.to(bdtype) if need_db else None) + (None,) * 9
+
+
+def linear_distillation_loss(
+    hidden: torch.Tensor,
+    weight: torch.Tensor,
+    teacher_logits: torch.Tensor,
+    teacher_indices: torch.Tensor,
+    labels: Optional[torch.Tensor] = None,
+    bias: Optional[torch.Tensor] = None,
+    chunk_size: int = 8192,
+    temperature: float = 1.0,
+    distill_weight: float = 1.0,
+    ce_weight: float = 0.0,
+    ignore_index: int = -100,
+    reduction: str = "mean",
+) -> torch.Tensor:
+    """Fused lm_head projection + distillation loss without materialising logits (module docstring).
+
+    hidden [..., d], weight [V, d], bias [V] or None, teacher_logits and
+    teacher_indices [..., K], labels [...] or None; differentiable in hidden,
+    weight and bias.  d is a multiple of 8.  ``chunk_size`` bounds the backward's
+    vocabulary band, as in ``cut_cross_entropy``.
+    """
+    red = _reduction_code(reduction)
+    _check_student(hidden, "hidden", "linear_distillation_loss")
+    _check(weight.dim() == 2, f"weight must be [vocab_size, hidden_dim], got shape {tuple(weight.shape)}")
+    _check(weight.device == hidden.device, "hidden and weight must be on the same device")
+    _check(weight.dtype in _FLOATS, f"weight dtype {weight.dtype} not supported (bf16, fp16, fp32)")
+    _check(hidden.shape[-1] == weight.shape[1],
+           f"hidden last dim {hidden.shape[-1]} does not match weight hidden_dim {weight.shape[1]}")
+    if bias is not None:
+        _check(bias.dim() == 1 and bias.shape[0] == weight.shape[0],
+               f"bias must be [vocab_size={weight.shape[0]}], got {tuple(bias.shape)}")
+        _check(bias.device == hidden.device, "bias must be on the same device as hidden")
+    t, index, lab = _teacher_rows(hidden, teacher_logits, teacher_indices, labels, temperature, ce_weight)
+    loss = LinearDistillationFunction.apply(hidden, weight, bias, t, index, lab, chunk_size, temperature,
+                                            distill_weight, ce_weight, ignore_index, red)
+    return loss.view(hidden.shape[:-1]) if red == _lib.CCE_REDUCTION_NONE else loss
+
+
+class LinearDistillationLoss(nn.Module):
+    """Module form of linear_distillation_loss; ``chunk_size=None`` picks ``get_optimal_chunk_size`` per call, as
+    CutCrossEntropyLoss does."""
+
+    def __init__(self, chunk_size: Optional[int] = None, temperature: float = 1.0, distill_weight: float = 1.0,
+                 ce_weight: float = 0.0, ignore_index: int = -100, reduction: str = "mean"):
+        super().__init__()
+        _reduction_code(reduction)
+        self.chunk_size = chunk_size
+        self.temperature = temperature
+        self.distill_weight = distill_weight
+        self.ce_weight = ce_weight
+        self.ignore_index = ignore_index
+        self.reduction = reduction
+
+    def forward(self, hidden: torch.Tensor, weight: torch.Tensor, teacher_logits: torch.Tensor,
+                teacher_indices: torch.Tensor, labels: Optional[torch.Tensor] = None,
+                bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+        chunk = self.chunk_size
+        if chunk is None:
+            chunk = get_optimal_chunk_size(weight.shape[0], weight.shape[1])
+        return linear_distillation_loss(hidden, weight, teacher_logits, teacher_indices, labels, bias, chunk,
+                                        self.temperature, self.distill_weight, self.ce_weight, self.ignore_index,
+                                        self.reduction)
+
+    def extra_repr(self) -> str:
+        return (f"chunk_size={self.chunk_size}, temperature={self.temperature}, "
+                f"distill_weight={self.distill_weight}, ce_weight={self.ce_weight}, "
+                f"ignore_index={self.ignore_index}, reduction={self.reduction!r}")

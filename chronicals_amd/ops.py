@@ -42,7 +42,8 @@ from . import _lib
 from . import build as _build
 
 __all__ = ["cce_fwd", "cce_bwd", "ce_logits_fwd", "ce_logits_bwd", "ce_logits_bwd_", "ce_logits_fwd_bwd",
-           "ce_logits_fwd_bwd_"]
+           "ce_logits_fwd_bwd_", "distill_logits_fwd", "distill_logits_bwd", "distill_fwd", "distill_bwd", "top_logits",
+           "layer_norm_fwd", "layer_norm_bwd"]
 
 _SCHEMAS = (
     "cce_fwd(Tensor hidden, Tensor weight, Tensor labels, Tensor? bias, SymInt ignore_index, float label_smoothing, "
@@ -57,6 +58,23 @@ _SCHEMAS = (
     "float label_smoothing, float z_loss_weight, SymInt smoothing_form, SymInt reduction, bool f32_grad) -> Tensor",
     "ce_logits_fwd_bwd(Tensor logits, Tensor labels, SymInt ignore_index, float label_smoothing, float z_loss_weight, "
     "SymInt smoothing_form, SymInt reduction, bool grad_mean, bool f32_grad) -> (Tensor, Tensor, Tensor, Tensor)",
+    "distill_logits_fwd(Tensor logits, Tensor teacher_logits, Tensor teacher_indices, Tensor? labels, "
+    "float temperature, float distill_weight, float ce_weight, SymInt ignore_index, SymInt reduction) "
+    "-> (Tensor, Tensor, Tensor)",
+    "distill_logits_bwd(Tensor grad_out, Tensor logits, Tensor teacher_logits, Tensor teacher_indices, "
+    "Tensor? labels, Tensor stats, Tensor n_valid, float temperature, float distill_weight, float ce_weight, "
+    "SymInt ignore_index, SymInt reduction) -> Tensor",
+    "distill_fwd(Tensor hidden, Tensor weight, Tensor? bias, Tensor teacher_logits, Tensor teacher_indices, "
+    "Tensor? labels, float temperature, float distill_weight, float ce_weight, SymInt ignore_index, "
+    "SymInt reduction) -> (Tensor, Tensor, Tensor, Tensor, Tensor)",
+    "distill_bwd(Tensor grad_out, Tensor hidden, Tensor weight, Tensor? bias, Tensor teacher_logits, "
+    "Tensor teacher_indices, Tensor stats, Tensor entry_logits, Tensor rows, Tensor n_valid, float temperature, "
+    "float distill_weight, float ce_weight, SymInt reduction, SymInt chunk_size, bool need_dh, bool need_dw, "
+    "bool need_db, bool dh_f32, bool dw_f32) -> (Tensor, Tensor, Tensor)",
+    "top_logits(Tensor logits, SymInt k) -> (Tensor, Tensor)",
+    "layer_norm_fwd(Tensor x, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor, Tensor)",
+    "layer_norm_bwd(Tensor grad_y, Tensor x, Tensor? weight, Tensor mean, Tensor rstd, bool param_f32, "
+    "bool need_dx, bool need_dw, bool need_db) -> (Tensor, Tensor, Tensor)",
 )
 _LIBRARY = torch.library.Library("chronicals_hip", "FRAGMENT")
 for _s in _SCHEMAS:
@@ -259,8 +277,77 @@ def _ce_logits_fwd_bwd__fake(logits, labels, ignore_index, label_smoothing, z_lo
                                reduction)
 
 
+# ---------------------------------------------------------------------------
+# Distillation from a teacher's top logits (cce_distill_*), the teacher's top
+# logits (cce_top_logits) and layer norm (cce_layer_norm_*); all in C++.
+#
+# teacher_logits [N, K] (bf16, fp16, fp32) and teacher_indices [N, K] (int64,
+# int32) are contiguous; the students' operands are those of ce_logits_* and
+# cce_*.  What a forward returns beside the loss is for the backward of the same
+# operands.  layer_norm_* take [N, D] rows with a contiguous last dimension.
+# ---------------------------------------------------------------------------
+
+def _loss_fake(x, reduction):
+    return x.new_empty((x.shape[0],) if reduction == _lib.CCE_REDUCTION_NONE else (1,), dtype=torch.float32)
+
+
+@torch.library.register_fake("chronicals_hip::distill_logits_fwd", lib=_LIBRARY)
+def _distill_logits_fwd_fake(logits, teacher_logits, teacher_indices, labels, temperature, distill_weight, ce_weight,
+                             ignore_index, reduction):
+    return (_loss_fake(logits, reduction), logits.new_empty((logits.shape[0], 4), dtype=torch.float32),
+            logits.new_empty((1,), dtype=torch.int32))
+
+
+@torch.library.register_fake("chronicals_hip::distill_logits_bwd", lib=_LIBRARY)
+def _distill_logits_bwd_fake(grad_out, logits, *args):
+    return logits.new_empty(tuple(logits.shape))
+
+
+@torch.library.register_fake("chronicals_hip::distill_fwd", lib=_LIBRARY)
+def _distill_fwd_fake(hidden, weight, bias, teacher_logits, teacher_indices, labels, temperature, distill_weight,
+                      ce_weight, ignore_index, reduction):
+    N, K = teacher_logits.shape
+    return (_loss_fake(hidden, reduction), hidden.new_empty((N, 2), dtype=torch.float32),
+            hidden.new_empty((N, K + 1), dtype=torch.float32), hidden.new_empty((N,), dtype=torch.int32),
+            hidden.new_empty((1,), dtype=torch.int32))
+
+
+@torch.library.register_fake("chronicals_hip::distill_bwd", lib=_LIBRARY)
+def _distill_bwd_fake(grad_out, hidden, weight, bias, teacher_logits, teacher_indices, stats, entry_logits, rows,
+                      n_valid, temperature, distill_weight, ce_weight, reduction, chunk_size, need_dh, need_dw, need_db,
+                      dh_f32, dw_f32):
+    return _cce_bwd_fake(grad_out, hidden, weight, rows, stats, n_valid, bias, -1, 0.0, 0.0, reduction, chunk_size,
+                         need_dh, need_dw, need_db, dh_f32, dw_f32)
+
+
+@torch.library.register_fake("chronicals_hip::top_logits", lib=_LIBRARY)
+def _top_logits_fake(logits, k):
+    shape = (logits.shape[0], k)
+    return logits.new_empty(shape), logits.new_empty(shape, dtype=torch.int64)
+
+
+@torch.library.register_fake("chronicals_hip::layer_norm_fwd", lib=_LIBRARY)
+def _layer_norm_fwd_fake(x, weight, bias, eps):
+    rows = (x.shape[0],)
+    return x.new_empty(tuple(x.shape)), x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
+
+
+@torch.library.register_fake("chronicals_hip::layer_norm_bwd", lib=_LIBRARY)
+def _layer_norm_bwd_fake(grad_y, x, weight, mean, rstd, param_f32, need_dx, need_dw, need_db):
+    params = torch.float32 if param_f32 else x.dtype
+    return (x.new_empty(tuple(x.shape) if need_dx else (0,)), x.new_empty((x.shape[1] if need_dw else 0,), dtype=params),
+            x.new_empty((x.shape[1] if need_db else 0,), dtype=params))
+
+
 cce_fwd = torch.ops.chronicals_hip.cce_fwd
 cce_bwd = torch.ops.chronicals_hip.cce_bwd
 ce_logits_fwd = torch.ops.chronicals_hip.ce_logits_fwd
 ce_logits_bwd = torch.ops.chronicals_hip.ce_logits_bwd
 ce_logits_fwd_bwd = torch.ops.chronicals_hip.ce_logits_fwd_bwd
+distill_logits_fwd = torch.ops.chronicals_hip.distill_logits_fwd
+distill_logits_bwd = torch.ops.chronicals_hip.distill_logits_bwd
+distill_fwd = torch.ops.chronicals_hip.distill_fwd
+distill_bwd = torch.ops.chronicals_hip.distill_bwd
+top_logits = torch.ops.chronicals_hip.top_logits
+layer_norm_fwd = torch.ops.chronicals_hip.layer_norm_fwd
+layer_norm_bwd = torch.ops.chronicals_hip.layer_norm_bwd

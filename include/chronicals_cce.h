@@ -43,7 +43,7 @@
 extern "C" {
 #endif
 
-#define CCE_ABI_VERSION 7
+#define CCE_ABI_VERSION 8
 
 #define CCE_OK 0
 #define CCE_ERR_INVALID_ARG 1
@@ -260,6 +260,95 @@ int cce_logits_forward_backward(const void* logits, int logits_dtype, int64_t ld
                                 float* loss_out, float* lse_out, int32_t* n_valid_out, void* grad_logits,
                                 int grad_dtype, int64_t ld_grad, void* workspace, size_t workspace_bytes,
                                 void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Distillation from a teacher's top logits.  No reference counterpart.
+ *
+ * Row n of a teacher has `entries` entries: the logit t_k at column i_k of the
+ * student's vocabulary.  An entry whose column is outside [0, V) (padding: -1)
+ * or whose logit is -inf takes no part.  With the temperature T and over the
+ * usable entries
+ *   q      = softmax(t / T)
+ *   row[n] = distill_weight * T^2 * sum_k q_k * (log q_k - log softmax(x / T)[i_k])
+ *          + ce_weight * (logsumexp(x) - x[label])
+ * The first term is 0 for a row without a usable entry; x[label] is left out for
+ * a label outside [0, V) that is not ignore_index.  A row counts if its label is
+ * not ignore_index or, where labels is NULL (ce_weight must be 0 then), if it
+ * has a usable entry; the others give 0 and a zero gradient, whatever they hold.
+ * 'mean' divides by the number of rows that count, at least 1.  Entries of one
+ * row may share a column: their q add up there.
+ */
+#define CCE_MAX_TEACHER_ENTRIES 256
+
+typedef struct cce_teacher {
+  const void* logits;  /* [N][entries], contiguous */
+  const void* indices; /* [N][entries], contiguous, int64 or int32 */
+  int64_t entries;     /* 1 .. CCE_MAX_TEACHER_ENTRIES */
+  int logits_dtype;    /* CCE_DTYPE_* */
+  int indices_int64;
+  float temperature; /* 0.01 .. 1000 */
+  float distill_weight;
+  float ce_weight;
+} cce_teacher;
+
+/* Over student logits that exist: [N][ld], of logits_dtype.  The forward's
+ * stats_out [N][4] (16-byte aligned) is what the backward reads beside the inputs;
+ * grad_logits has the logits' dtype, any row stride, and is not the logits. */
+int cce_distill_logits_workspace_bytes(int64_t N, int64_t V, int reduction, size_t* bytes);
+int cce_distill_logits_forward(const void* logits, int logits_dtype, int64_t ld, const cce_teacher* teacher,
+                               const void* labels, int labels_int64, int64_t N, int64_t V, int64_t ignore_index,
+                               int reduction, float* loss_out, float* stats_out, int32_t* n_valid_out,
+                               void* workspace, size_t workspace_bytes, void* stream);
+int cce_distill_logits_backward(const float* grad_out, const void* logits, int logits_dtype, int64_t ld,
+                                const cce_teacher* teacher, const void* labels, int labels_int64, const float* stats,
+                                const int32_t* n_valid, int64_t N, int64_t V, int64_t ignore_index, int reduction,
+                                void* grad_logits, int64_t ld_grad, void* stream);
+
+/* Fused with the head's product, x = hidden . weight^T + bias, operands as
+ * cce_forward's and cce_backward's.  The forward keeps for the backward
+ * stats_out [N][2], entry_logits_out [N][entries + 1] and rows_out [N]; the
+ * backward takes the same teacher, and no labels. */
+int cce_distill_forward_workspace_bytes(int64_t N, int64_t d, int64_t V, int reduction, size_t* bytes);
+int cce_distill_forward(const void* hidden, const void* weight, const float* bias, const cce_teacher* teacher,
+                        const void* labels, int labels_int64, int64_t N, int64_t d, int64_t V, int64_t ignore_index,
+                        int reduction, float* loss_out, float* stats_out, float* entry_logits_out, int32_t* rows_out,
+                        int32_t* n_valid_out, void* workspace, size_t workspace_bytes, void* stream);
+int cce_distill_backward_workspace_bytes(int64_t N, int64_t d, int64_t V, int64_t entries, int64_t chunk_size,
+                                         int need_grad_hidden, int grad_hidden_dtype, int need_grad_weight,
+                                         int grad_weight_dtype, size_t* bytes);
+int cce_distill_backward(const float* grad_out, const void* hidden, const void* weight, const float* bias,
+                         const cce_teacher* teacher, const float* stats, const float* entry_logits,
+                         const int32_t* rows, const int32_t* n_valid, int64_t N, int64_t d, int64_t V, int reduction,
+                         int64_t chunk_size, void* grad_hidden, int grad_hidden_dtype, void* grad_weight,
+                         int grad_weight_dtype, float* grad_bias, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/*
+ * The k largest logits of each row, largest first (values_out [N][k], of the
+ * logits' dtype, bit by bit) and their columns (indices_out [N][k]); among equal
+ * values the lower column first.  NaN is larger than any number, -0 equals +0.
+ * 1 <= k <= min(V, CCE_MAX_TEACHER_ENTRIES).
+ */
+int cce_top_logits(const void* logits, int logits_dtype, int64_t ld, int64_t N, int64_t V, int64_t k, void* values_out,
+                   int64_t* indices_out, void* stream);
+
+/*
+ * Layer norm over rows of D elements, D <= 2^20:
+ *   y = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(var + eps)
+ * with fp32 statistics (mean_out, rstd_out [N]).  x has the row stride ldx, y_out
+ * and the gradients are contiguous, of x's dtype; weight and bias (either may be
+ * NULL) and their gradients are of param_dtype, which is x's or fp32.  The
+ * backward leaves out the gradients whose pointer is NULL.  No reference
+ * counterpart.
+ */
+int cce_layer_norm_forward(const void* x, int dtype, int64_t ldx, const void* weight, const void* bias,
+                           int param_dtype, int64_t N, int64_t D, float eps, void* y_out, float* mean_out,
+                           float* rstd_out, void* stream);
+int cce_layer_norm_backward_workspace_bytes(int64_t N, int64_t D, size_t* bytes);
+int cce_layer_norm_backward(const void* grad_y, const void* x, int dtype, int64_t ldx, const void* weight,
+                            int param_dtype, const float* mean, const float* rstd, int64_t N, int64_t D, void* grad_x,
+                            void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
+                            void* stream);
 
 /*
  * Per-kernel timing for measurement tools (no counterpart in the reference).
