@@ -140,7 +140,11 @@ SIGNATURES = {
         _vp, _i32, _vp, _i32, _vp,           # grad_hidden, dtype, grad_weight, dtype, grad_bias
         _vp, _sz, _vp,                       # workspace, workspace_bytes, stream
     ]),
-    "cce_top_logits": (_i32, [_vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "cce_top_logits_workspace_bytes": (_i32, [_i64, _i64, _i64, _size_out]),
+    "cce_top_logits": (_i32, [
+        _vp, _i32, _i64, _i64, _i64, _i64,   # logits, dtype, ld, N, V, k
+        _vp, _vp, _vp, _sz, _vp,             # values_out, indices_out, workspace, workspace_bytes, stream
+    ]),
     "cce_layer_norm_forward": (_i32, [
         _vp, _i32, _i64, _vp, _vp, _i32,     # x, dtype, ldx, weight, bias, param_dtype
         _i64, _i64, _f32, _vp, _vp, _vp, _vp,  # N, D, eps, y_out, mean_out, rstd_out, stream

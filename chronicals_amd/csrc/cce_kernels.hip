@@ -3505,21 +3505,31 @@ int cce_distill_backward(const float* grad_out, const void* hidden, const void* 
                       workspace_bytes, stream, &s);
 }
 
+int cce_top_logits_workspace_bytes(int64_t N, int64_t V, int64_t k, size_t* bytes) {
+  g_err[0] = 0;
+  if (!bytes) return fail(CCE_ERR_INVALID_ARG, "bytes must not be null");
+  const int rc = check_top(N, V, k, CCE_DTYPE_F32, V);
+  if (rc) return rc;
+  *bytes = top_bytes(N, V, k);
+  return CCE_OK;
+}
+
 int cce_top_logits(const void* logits, int logits_dtype, int64_t ld, int64_t N, int64_t V, int64_t k, void* values_out,
-                   int64_t* indices_out, void* stream) {
+                   int64_t* indices_out, void* workspace, size_t workspace_bytes, void* stream) {
   g_err[0] = 0;
   const int rc = check_top(N, V, k, logits_dtype, ld);
   if (rc) return rc;
   if (N == 0) return CCE_OK;
   if (!logits || !values_out || !indices_out)
     return fail(CCE_ERR_INVALID_ARG, "logits, values_out and indices_out must not be null");
+  if (misaligned(workspace)) return fail(CCE_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
+  const size_t need = top_bytes(N, V, k);
+  if (workspace_bytes < need || (need && !workspace))
+    return fail(CCE_ERR_WORKSPACE, "workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
   return logits_type(logits_dtype, [&](auto t) {
     typedef decltype(t) T;
-    hipLaunchKernelGGL(top_logits_kernel<T>, dim3((unsigned)N), dim3(256), 0, reinterpret_cast<hipStream_t>(stream),
-                       static_cast<const T*>(logits), (long)ld, (int)V, (int)k, static_cast<T*>(values_out),
-                       indices_out);
-    HIP_TRY(hipGetLastError());
-    return CCE_OK;
+    return top_run(static_cast<const T*>(logits), (long)ld, (long)N, (long)V, (long)k, static_cast<T*>(values_out),
+                   indices_out, static_cast<uint64_t*>(workspace), reinterpret_cast<hipStream_t>(stream));
   });
 }
 

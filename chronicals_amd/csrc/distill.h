@@ -106,14 +106,6 @@ __device__ inline float entries_at(const Entries& e, int K, int c) {
 // Over logits that exist
 // ---------------------------------------------------------------------------
 
-// Columns of split s of S of a row of V: whole multiples of 64, so that every
-// split starts on the row's alignment.
-__device__ inline void split_span(int V, int S, int s, int& c0, int& c1) {
-  const int per = ((V + S - 1) / S + 63) / 64 * 64;
-  c0 = min((int)min((long)s * per, (long)V), V);
-  c1 = (int)min((long)c0 + per, (long)V);
-}
-
 // Running maximum of x and sums of exp((x - m) / T) and, with DU, exp(x - m).
 // The differences are taken before they are scaled: with x at its type's lowest
 // value, m * log2(e) would pass the range of fp32.

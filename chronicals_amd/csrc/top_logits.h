@@ -60,15 +60,18 @@ __device__ int kth_key(F&& key, int m, int k, uint32_t* hist, uint32_t& tau) {
   return k;
 }
 
-// Candidates in LDS, as (key, position) pairs that are all different.
+// A candidate: its key above the complement of its column, so that a larger one
+// comes first and among equal keys the lower column.  All are different.
+__device__ inline uint64_t candidate(uint32_t key, int at) { return (uint64_t)key << 32 | (uint32_t)~at; }
+__device__ inline int column(uint64_t c) { return (int)~(uint32_t)c; }
+
+// Candidates in LDS.
 struct TopList {
-  uint32_t* key;
-  int* at;
+  uint64_t* c;
   int* count;
 };
 
-// The k largest of m keys into `list`, in no order; equal keys by the lower
-// position first.
+// The k largest of m keys into `list`, in no order.
 template <int BITS, typename F>
 __device__ void top_exact(F&& key, int m, int k, uint32_t* hist, const TopList& list) {
   __shared__ int wave_count[4];
@@ -79,11 +82,7 @@ __device__ void top_exact(F&& key, int m, int k, uint32_t* hist, const TopList& 
   __syncthreads();
   for (int i = tid; i < m; i += 256) {
     const uint32_t v = key(i);
-    if (v > tau) {
-      const int p = atomicAdd(list.count, 1);
-      list.key[p] = v;
-      list.at[p] = i;
-    }
+    if (v > tau) list.c[atomicAdd(list.count, 1)] = candidate(v, i);
   }
   // those equal to tau in order of their positions, 256 at a time
   int done = 0;
@@ -99,43 +98,274 @@ __device__ void top_exact(F&& key, int m, int k, uint32_t* hist, const TopList& 
       if (v < w) p += wave_count[v];
       done += wave_count[v];
     }
-    if (eq && p < equal) {
-      list.key[k - equal + p] = tau;
-      list.at[k - equal + p] = i;
-    }
+    if (eq && p < equal) list.c[k - equal + p] = candidate(tau, i);
   }
   __syncthreads();
   if (tid == 0) *list.count = k;
   __syncthreads();
 }
 
-// Calls f(rank, position) for the candidates of rank below k, one thread each.
+// Calls f(rank, candidate) for the candidates of rank below k, one thread each.
 template <typename F>
 __device__ void top_ranked(const TopList& list, int k, F&& f) {
   const int m = *list.count;
   for (int i = threadIdx.x; i < m; i += 256) {
-    const uint32_t v = list.key[i];
-    const int at = list.at[i];
+    const uint64_t v = list.c[i];
     int rank = 0;
-    for (int j = 0; j < m; ++j) rank += list.key[j] > v || (list.key[j] == v && list.at[j] < at);
-    if (rank < k) f(rank, at);
+#pragma unroll 8
+    for (int j = 0; j < m; ++j) rank += list.c[j] > v;
+    if (rank < k) f(rank, v);
   }
 }
 
-// One workgroup per row.
+// The largest of some elements, as unsigned integers that order as the values do:
+// 0 for -inf, past +inf's the NaN of either sign, -0 one below +0.  From the bits
+// b: b ^ 0x7f.. for negative ones, less -inf's.  The 16-bit types keep two, of the
+// even and the odd elements (packed operations).
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short w16x2 __attribute__((ext_vector_type(2)));
 template <typename T>
-__global__ __launch_bounds__(256) void top_logits_kernel(const T* __restrict__ X, long ld, int V, int k,
-                                                         T* __restrict__ values, int64_t* __restrict__ indices) {
-  __shared__ uint32_t hist[256], ckey[kTopMax];
-  __shared__ int cat[kTopMax], count;
-  const TopList list = {ckey, cat, &count};
-  const long n = blockIdx.x;
-  const T* const row = X + n * ld;
+struct GroupMax {
+  static constexpr int kParts = 2, kBits = 16;
+  static constexpr uint32_t kInf = std::is_same<T, uint16_t>::value ? 0x7f80 : 0x7c00;  // +inf's bits
+  static constexpr uint32_t kZero = kInf + 1;                                          // +0
+  w16x2 v = {0, 0};
+  __device__ inline void add(const u32x4& raw) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t r = raw[i];  // a bit_cast of the vector's element itself takes element 0
+      const s16x2 b = __builtin_bit_cast(s16x2, r);
+      const w16x2 p = __builtin_bit_cast(w16x2, (s16x2)(b ^ (s16x2)((b >> 15) & (short)0x7fff))) + (unsigned short)kZero;
+      v = __builtin_elementwise_max(v, p);
+    }
+  }
+  __device__ inline uint32_t part(int i) const { return v[i]; }
+  static __device__ inline T value(uint32_t p) {
+    const short b = (short)(p - kZero);
+    return __builtin_bit_cast(T, (short)(b ^ ((b >> 15) & 0x7fff)));
+  }
+};
+template <>
+struct GroupMax<float> {
+  static constexpr int kParts = 1, kBits = 32;
+  static constexpr uint32_t kInf = 0x7f800000u, kZero = kInf + 1;
+  uint32_t v = 0;
+  __device__ inline void add(const u32x4& raw) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v = max(v, (raw[i] ^ (uint32_t)((int)raw[i] >> 31) >> 1) + kZero);
+  }
+  __device__ inline uint32_t part(int) const { return v; }
+  static __device__ inline float value(uint32_t p) {
+    const uint32_t b = p - kZero;
+    return __uint_as_float(b ^ (uint32_t)((int)b >> 31) >> 1);
+  }
+};
+
+constexpr int kTopCandidates = 2048;
+
+// The k largest of row[0, V) into `list` (at least those k, at most
+// kTopCandidates), by one pass over HBM and a second look at a few of its lines.
+//
+// Pass 1 keeps the largest of each of 1024 or 2048 groups: a thread's chunks at
+// each place of its four loads in flight.  Each group's largest is an element,
+// so at least k elements reach the k-th largest of these maxima, tau.  Pass 2
+// reads the groups that reach it again (about k of them, from the caches) and
+// collects their elements from tau on: for values in no particular order about
+// k more or less, 66 to 300 for k = 64 to 256.  A row with more than
+// kTopCandidates there (long ties), or with fewer chunks than k, goes by
+// top_exact, whose passes over the row are three to five.
+//
+// Bound by HBM: k = 64 of 2048 x 151936 bf16 takes 128 us, 4.9 TB/s (a large copy
+// reaches 4.9); by top_exact alone it took 1550 us.  Of that 144 -> 136 us came
+// from non-temporal loads in pass 1 and 136 -> 128 from eight workgroups per CU
+// instead of seven.
+template <typename T>
+__device__ void top_of_row(const T* row, int V, int k, uint32_t* hist, uint16_t* groups, const TopList& list) {
+  constexpr int U = 4, NP = GroupMax<T>::kParts;
+  __shared__ int counts[2][4], ngroups;
+  const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
+  const RowSplit<T> sp(row, V);
+  if (sp.chunks >= k) {
+    const u32x4* const body = reinterpret_cast<const u32x4*>(row + sp.head);
+    GroupMax<T> g[U];
+    int c = tid;
+    for (; c + (U - 1) * 256 < sp.chunks; c += U * 256) {
+      u32x4 raw[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = __builtin_nontemporal_load(body + c + u * 256);
+#pragma unroll
+      for (int u = 0; u < U; ++u) g[u].add(raw[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (c + u * 256 < sp.chunks) g[u].add(body[c + u * 256]);
+    // tau: the largest integer that k groups reach, bit by bit from the top.  Of
+    // fp32's the lowest 12 bits stay 0: what lies in between is hardly ever a
+    // candidate more, and each bit costs a barrier
+    uint32_t tau = 0;
+    for (int bit = GroupMax<T>::kBits - 1; bit >= (GroupMax<T>::kBits == 32 ? 12 : 0); --bit) {
+      const uint32_t next = tau | 1u << bit;
+      int n = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < NP; ++i) n += __popcll(__ballot(g[u].part(i) >= next));
+      int* const at = counts[bit & 1];
+      if (l == 0) at[w] = n;
+      __syncthreads();
+      if (at[0] + at[1] + at[2] + at[3] >= k) tau = next;
+    }
+    // the lowest integer of the same key: NaN are equal, and so are zeros
+    constexpr uint32_t kInf = GroupMax<T>::kInf + GroupMax<T>::kZero;
+    const uint32_t from = key_of(GroupMax<T>::value(tau));
+    tau = tau > kInf ? kInf + 1 : tau == GroupMax<T>::kZero ? tau - 1 : tau;
+    if (tid == 0) *list.count = ngroups = 0;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      bool reach = false;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) reach = reach || g[u].part(i) >= tau;
+      if (reach) groups[atomicAdd(&ngroups, 1)] = (uint16_t)(u * 256 + tid);
+    }
+    __syncthreads();
+    auto take = [&](T x, int at) {
+      const uint32_t key = key_of(x);
+      if (key < from) return;
+      const int p = atomicAdd(list.count, 1);
+      if (p < kTopCandidates) list.c[p] = candidate(key, at);
+    };
+    const int rounds = (sp.chunks + U * 256 - 1) / (U * 256), items = ngroups * rounds;
+    for (int i0 = 0; i0 < items; i0 += U * 256) {
+      u32x4 raw[U];
+      int at[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * 256 + tid;
+        at[u] = -1;
+        if (i < items) {
+          // neighbouring threads take neighbouring groups of one round
+          const int chunk = (i / ngroups) * (U * 256) + groups[i % ngroups];
+          if (chunk < sp.chunks) {
+            at[u] = sp.head + chunk * RowSplit<T>::E;
+            raw[u] = body[chunk];
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (at[u] < 0) continue;
+        const T* v = reinterpret_cast<const T*>(&raw[u]);
+#pragma unroll
+        for (int e = 0; e < RowSplit<T>::E; ++e) take(v[e], at[u] + e);
+      }
+    }
+    if (tid < sp.head) take(row[tid], tid);
+    if (tid < V - sp.tail_start) take(row[sp.tail_start + tid], sp.tail_start + tid);
+    __syncthreads();
+    const bool fits = *list.count <= kTopCandidates;
+    __syncthreads();
+    if (fits) return;
+  }
   top_exact<kKeyBits<T>>([&](int i) { return key_of(row[i]); }, V, k, hist, list);
-  top_ranked(list, k, [&](int rank, int at) {
-    values[n * k + rank] = row[at];
-    indices[n * k + rank] = at;
+}
+
+// Columns of split s of S of a row of V: whole multiples of 64, so that every
+// split starts on the row's alignment.
+__device__ inline void split_span(int V, int S, int s, int& c0, int& c1) {
+  const int per = ((V + S - 1) / S + 63) / 64 * 64;
+  c0 = min((int)min((long)s * per, (long)V), V);
+  c1 = (int)min((long)c0 + per, (long)V);
+}
+
+// One workgroup per row and split of S.  One split: the row's answer.  More: the
+// split's k largest, in order, at part[(n * S + s) * k], or all of it where it has
+// no more than k columns, and zeros (less than any candidate) behind.
+template <typename T>
+__global__ __launch_bounds__(256) void top_logits_kernel(const T* __restrict__ X, long ld, int V, int S, int k,
+                                                         T* __restrict__ values, int64_t* __restrict__ indices,
+                                                         uint64_t* __restrict__ part) {
+  __shared__ uint32_t hist[256];
+  __shared__ uint64_t cands[kTopCandidates];
+  __shared__ uint16_t groups[1024];  // 16 bits: eight workgroups per CU fit with 20 KB each
+  __shared__ int count;
+  const TopList list = {cands, &count};
+  const long n = blockIdx.x / S;
+  int c0, c1;
+  split_span(V, S, blockIdx.x % S, c0, c1);
+  const T* const row = X + n * ld + c0;
+  const int m = min(k, c1 - c0);
+  if (m > 0) top_of_row(row, c1 - c0, m, hist, groups, list);
+  if (S == 1) {
+    top_ranked(list, k, [&](int rank, uint64_t c) {
+      values[n * k + rank] = row[column(c)];
+      indices[n * k + rank] = column(c);
+    });
+    return;
+  }
+  uint64_t* const out = part + (long)blockIdx.x * k;
+  if (m > 0) top_ranked(list, m, [&](int rank, uint64_t c) { out[rank] = candidate(c >> 32, c0 + column(c)); });
+  for (int i = m + threadIdx.x; i < k; i += 256) out[i] = 0;
+}
+
+// The k largest of a row from those of its S splits.  S * ceil(k / S) candidates
+// reach the smallest of the splits' ceil(k / S)-th ones, so no other counts.
+template <typename T>
+__global__ __launch_bounds__(256) void top_join_kernel(const T* __restrict__ X, long ld, int S, int k,
+                                                       const uint64_t* __restrict__ part, T* __restrict__ values,
+                                                       int64_t* __restrict__ indices) {
+  constexpr int kE = kTopCandidates / 256;
+  __shared__ uint64_t cands[kTopCandidates], low[4];
+  __shared__ int count;
+  const TopList list = {cands, &count};
+  const long n = blockIdx.x;
+  const int tid = threadIdx.x;
+  const uint64_t* const p = part + n * S * k;
+  uint64_t c[kE], tau = ~0ull;
+  for (int s = tid; s < S; s += 256) tau = min(tau, p[s * k + (k + S - 1) / S - 1]);
+#pragma unroll
+  for (int e = 0; e < kE; ++e) c[e] = e * 256 + tid < S * k ? p[e * 256 + tid] : 0;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) tau = min(tau, (uint64_t)__shfl_xor((unsigned long long)tau, o));
+  if ((tid & 63) == 0) low[tid >> 6] = tau;
+  if (tid == 0) count = 0;
+  __syncthreads();
+  tau = min(min(low[0], low[1]), min(low[2], low[3]));
+#pragma unroll
+  for (int e = 0; e < kE; ++e)
+    if (c[e] >= tau && c[e] != 0) cands[atomicAdd(&count, 1)] = c[e];
+  __syncthreads();
+  top_ranked(list, k, [&](int rank, uint64_t v) {
+    values[n * k + rank] = X[n * ld + column(v)];
+    indices[n * k + rank] = column(v);
   });
+}
+
+// Workgroups per row: about four per CU where there are few rows, with at least
+// 2048 columns each, and no more candidates than one workgroup can join.  k = 128
+// of 16 x 128256 fp32: one workgroup per row by top_exact 528 us, 16 of them and
+// their join 22 us (11 each, most of it latencies).
+int top_splits(long N, long V, long k) {
+  const long s = std::min({ceil_div(1024, std::max<long>(N, 1)), V / 2048, kTopCandidates / std::max<long>(k, 1)});
+  return (int)std::max<long>(s, 1);
+}
+
+size_t top_bytes(long N, long V, long k) {
+  const int S = top_splits(N, V, k);
+  return S > 1 ? (size_t)N * S * k * sizeof(uint64_t) : 0;
+}
+
+template <typename T>
+int top_run(const T* X, long ld, long N, long V, long k, T* values, int64_t* indices, uint64_t* part, hipStream_t st) {
+  const int S = top_splits(N, V, k);
+  hipLaunchKernelGGL(top_logits_kernel<T>, dim3((unsigned)(N * S)), dim3(256), 0, st, X, ld, (int)V, S, (int)k, values,
+                     indices, part);
+  HIP_TRY(hipGetLastError());
+  if (S > 1) {
+    hipLaunchKernelGGL(top_join_kernel<T>, dim3((unsigned)N), dim3(256), 0, st, X, ld, S, (int)k, part, values, indices);
+    HIP_TRY(hipGetLastError());
+  }
+  return CCE_OK;
 }
 
 int check_top(int64_t N, int64_t V, int64_t k, int dtype, int64_t ld) {

@@ -49,6 +49,7 @@ struct Api {
   decltype(&cce_distill_forward) distill_forward;
   decltype(&cce_distill_backward_workspace_bytes) distill_backward_workspace_bytes;
   decltype(&cce_distill_backward) distill_backward;
+  decltype(&cce_top_logits_workspace_bytes) top_logits_workspace_bytes;
   decltype(&cce_top_logits) top_logits;
   decltype(&cce_layer_norm_forward) layer_norm_forward;
   decltype(&cce_layer_norm_backward_workspace_bytes) layer_norm_backward_workspace_bytes;
@@ -463,8 +464,11 @@ std::tuple<Tensor, Tensor> top_logits(const Tensor& logits, int64_t k) {
   TORCH_CHECK(k >= 1 && k <= std::min<int64_t>(V, CCE_MAX_TEACHER_ENTRIES), "k must be in [1, min(",
               CCE_MAX_TEACHER_ENTRIES, ", V = ", V, ")], got ", k);
   Tensor values = at::empty({N, k}, logits.options()), indices = at::empty({N, k}, logits.options().dtype(at::kLong));
+  size_t bytes = 0;
+  check(a, a.top_logits_workspace_bytes(N, V, k, &bytes));
+  const Tensor ws = at::empty({(int64_t)bytes}, logits.options().dtype(at::kByte));
   check(a, a.top_logits(logits.data_ptr(), logits_dtype(logits), row_stride(logits), N, V, k, values.data_ptr(),
-                        static_cast<int64_t*>(indices.data_ptr()), stream(logits.device())));
+                        static_cast<int64_t*>(indices.data_ptr()), ws.data_ptr(), bytes, stream(logits.device())));
   return {values, indices};
 }
 
@@ -557,6 +561,7 @@ int chronicals_torch_bind(void* handle) {
   get(a.distill_forward, "cce_distill_forward");
   get(a.distill_backward_workspace_bytes, "cce_distill_backward_workspace_bytes");
   get(a.distill_backward, "cce_distill_backward");
+  get(a.top_logits_workspace_bytes, "cce_top_logits_workspace_bytes");
   get(a.top_logits, "cce_top_logits");
   get(a.layer_norm_forward, "cce_layer_norm_forward");
   get(a.layer_norm_backward_workspace_bytes, "cce_layer_norm_backward_workspace_bytes");

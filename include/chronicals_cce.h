@@ -329,8 +329,9 @@ int cce_distill_backward(const float* grad_out, const void* hidden, const void* 
  * values the lower column first.  NaN is larger than any number, -0 equals +0.
  * 1 <= k <= min(V, CCE_MAX_TEACHER_ENTRIES).
  */
+int cce_top_logits_workspace_bytes(int64_t N, int64_t V, int64_t k, size_t* bytes);
 int cce_top_logits(const void* logits, int logits_dtype, int64_t ld, int64_t N, int64_t V, int64_t k, void* values_out,
-                   int64_t* indices_out, void* stream);
+                   int64_t* indices_out, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Layer norm over rows of D elements, D <= 2^20:

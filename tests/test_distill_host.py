@@ -189,9 +189,10 @@ def test_c_operands(lib):
     assert back(P, P, P, None, t, P, P, P, P, 4, 64, 1 << 33, 1, 0, P, 0, P, 0, None, P, 1 << 30, None) == bad
     top = lib.cce_top_logits
     for V, k in ((100, 0), (100, 101), (1000, 257), (0, 1)):
-        assert top(P, 1, V, 4, V, k, P, P, None) == bad
-    assert top(P, 1, 99, 4, 100, 3, P, P, None) == bad
-    assert top(None, 1, 100, 4, 100, 3, P, P, None) == bad
+        assert top(P, 1, V, 4, V, k, P, P, P, 1 << 30, None) == bad
+    assert top(P, 1, 99, 4, 100, 3, P, P, P, 1 << 30, None) == bad
+    assert top(None, 1, 100, 4, 100, 3, P, P, P, 1 << 30, None) == bad
+    assert top(P, 1, 1 << 17, 4, 1 << 17, 3, P, P, P, 8, None) == small
     norm, back = lib.cce_layer_norm_forward, lib.cce_layer_norm_backward
     assert norm(P, 0, 63, P, P, 0, 4, 64, 1e-5, P, P, P, None) == bad
     assert norm(P, 0, 64, P, P, 2, 4, 64, 1e-5, P, P, P, None) == bad
@@ -219,6 +220,9 @@ def test_c_workspaces(lib):
     kd = size(lib.cce_distill_backward_workspace_bytes, 4096, 896, 151936, 64, 8192, 1, 0, 1, 0)
     assert 4096 * 65 * 8 <= kd - ce <= 4096 * 65 * 8 + 1024
     assert size(lib.cce_layer_norm_backward_workspace_bytes, 0, 64) > 0
+    # the splits' candidates where there are few rows, nothing else
+    assert size(lib.cce_top_logits_workspace_bytes, 4096, 151936, 64) == 0
+    assert 0 < size(lib.cce_top_logits_workspace_bytes, 3, 151936, 64) <= 3 * 2048 * 8
     out = ctypes.c_size_t(0)
     assert lib.cce_distill_backward_workspace_bytes(8, 64, 100, 257, 0, 1, 0, 1, 0, ctypes.byref(out)) != 0
     assert lib.cce_distill_forward_workspace_bytes(8, 60, 100, 1, ctypes.byref(out)) != 0
