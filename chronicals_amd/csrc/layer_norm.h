@@ -9,6 +9,197 @@
 // to the type of x, dw and db to the type of w.  All of it is bound by HBM: the
 // forward reads x and writes y, the backward reads x and dy and writes dx.
 
+//
+// Rows of whole 16-byte chunks at 16-byte addresses stay in registers: TR threads
+// hold up to C chunks each, a wave per row up to 256 chunks, then a workgroup of
+// 256 or 1024.  A workgroup goes on to further rows with the parameters in its
+// registers, and in the backward with its share of dw and db there too.  What
+// does not fit (odd sizes or strides, more than 4096 chunks) goes by the kernels
+// below, which read a row two or three times.
+
+// Parameter c, fp32 or of type T.
+template <typename T>
+__device__ inline float load_param(const void* p, int f32, long c) {
+  return f32 ? static_cast<const float*>(p)[c] : elem_to_f32(static_cast<const T*>(p)[c]);
+}
+
+// Sums of two values over the TR threads of a row (fixed order).
+template <int TR>
+__device__ inline void row_sums(float& a, float& b, float (*red)[2]) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    a += __shfl_xor(a, o);
+    b += __shfl_xor(b, o);
+  }
+  if constexpr (TR > 64) {
+    __syncthreads();  // red may still be read by the sum before
+    if ((threadIdx.x & 63) == 0) {
+      red[threadIdx.x >> 6][0] = a;
+      red[threadIdx.x >> 6][1] = b;
+    }
+    __syncthreads();
+    a = b = 0.f;
+#pragma unroll
+    for (int w = 0; w < TR / 64; ++w) {
+      a += red[w][0];
+      b += red[w][1];
+    }
+  }
+}
+
+// The chunks of a row that thread t of TR holds, as fp32: chunk t + c * TR.
+template <typename T, int TR, int C>
+struct RowRegs {
+  static constexpr int E = 16 / sizeof(T);
+  float v[C][E];
+  __device__ inline void load(const T* row, int chunks, int t) {
+    u32x4 raw[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (t + c * TR < chunks) raw[c] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(row) + t + c * TR);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const T* e = reinterpret_cast<const T*>(&raw[c]);
+#pragma unroll
+      for (int i = 0; i < E; ++i) v[c][i] = t + c * TR < chunks ? elem_to_f32(e[i]) : 0.f;
+    }
+  }
+  __device__ inline void load_params(const void* p, int f32, int chunks, int t, float none) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        v[c][i] = p && t + c * TR < chunks ? load_param<T>(p, f32, (t + c * TR) * E + i) : none;
+  }
+  __device__ inline void store(T* row, int chunks, int t) const {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      u32x4 raw;
+      T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+      for (int i = 0; i < E; ++i) e[i] = f32_to_elem<T>(v[c][i]);
+      if (t + c * TR < chunks) __builtin_nontemporal_store(raw, reinterpret_cast<u32x4*>(row) + t + c * TR);
+    }
+  }
+};
+
+template <typename T, int TR, int C>
+__global__ __launch_bounds__(TR < 256 ? 256 : TR) void layer_norm_fwd_rows_kernel(
+    const T* __restrict__ X, long ldx, const void* __restrict__ w, const void* __restrict__ b, int param_f32, long N,
+    int D, float eps, T* __restrict__ Y, float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+  typedef RowRegs<T, TR, C> Row;
+  constexpr int kRows = TR < 256 ? 256 / TR : 1;  // rows of a workgroup at a time
+  __shared__ float red[TR / 64][2];
+  const int t = threadIdx.x % TR, chunks = D / Row::E;
+  const float inv = 1.f / (float)D;
+  Row wr, br;
+  wr.load_params(w, param_f32, chunks, t, 1.f);
+  br.load_params(b, param_f32, chunks, t, 0.f);
+  for (long n = (long)blockIdx.x * kRows + threadIdx.x / TR; n < N; n += (long)gridDim.x * kRows) {
+    Row x;
+    x.load(X + n * ldx, chunks, t);
+    float s = 0.f, q = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < Row::E; ++i) s += x.v[c][i];
+    row_sums<TR>(s, q, red);
+    const float mean = s * inv;
+    s = q = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < Row::E; ++i) {
+        x.v[c][i] = t + c * TR < chunks ? x.v[c][i] - mean : 0.f;
+        s += x.v[c][i] * x.v[c][i];
+      }
+    row_sums<TR>(s, q, red);
+    const float rstd = 1.f / sqrtf(s * inv + eps);
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < Row::E; ++i) x.v[c][i] = __builtin_fmaf(x.v[c][i] * rstd, wr.v[c][i], br.v[c][i]);
+    x.store(Y + n * D, chunks, t);
+    if (t == 0) {
+      mean_out[n] = mean;
+      rstd_out[n] = rstd;
+    }
+  }
+}
+
+// dx, and the workgroup's sums of dw and db over its rows at part[blockIdx.x].
+template <typename T, int TR, int C>
+__global__ __launch_bounds__(TR < 256 ? 256 : TR) void layer_norm_bwd_rows_kernel(
+    const T* __restrict__ dY, const T* __restrict__ X, long ldx, const void* __restrict__ w, int param_f32,
+    const float* __restrict__ mean, const float* __restrict__ rstd, long N, int D, T* __restrict__ dX,
+    float* __restrict__ dw, float* __restrict__ db) {
+  typedef RowRegs<T, TR, C> Row;
+  constexpr int kRows = TR < 256 ? 256 / TR : 1, E = Row::E;
+  __shared__ float red[TR / 64][2];
+  const int t = threadIdx.x % TR, chunks = D / E;
+  const float inv = 1.f / (float)D;
+  Row wr;
+  wr.load_params(w, param_f32, chunks, t, 1.f);
+  float sw[C][E] = {}, sb[C][E] = {};
+  for (long n = (long)blockIdx.x * kRows + threadIdx.x / TR; n < N; n += (long)gridDim.x * kRows) {
+    Row x, g;
+    x.load(X + n * ldx, chunks, t);
+    g.load(dY + n * D, chunks, t);
+    const float mu = mean[n], r = rstd[n];
+    float sa = 0.f, san = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        // past the row's end g is 0, so x there does not count
+        x.v[c][i] = (x.v[c][i] - mu) * r;
+        sw[c][i] = __builtin_fmaf(g.v[c][i], x.v[c][i], sw[c][i]);
+        sb[c][i] += g.v[c][i];
+        g.v[c][i] *= wr.v[c][i];
+        sa += g.v[c][i];
+        san = __builtin_fmaf(g.v[c][i], x.v[c][i], san);
+      }
+    if (!dX) continue;
+    row_sums<TR>(sa, san, red);
+    sa *= inv;
+    san *= inv;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < E; ++i) x.v[c][i] = r * (g.v[c][i] - sa - x.v[c][i] * san);
+    x.store(dX + n * D, chunks, t);
+  }
+  if (!dw) return;
+  // the rows' sums within the workgroup, one after the other
+  if constexpr (kRows > 1) {
+    __shared__ float sums[2][TR * C * E];
+    for (int k = 0; k < kRows; ++k) {
+      if (threadIdx.x / TR == k) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int i = 0; i < E; ++i) {
+            const int at = (c * E + i) * TR + t;
+            sums[0][at] = sw[c][i] = k ? sums[0][at] + sw[c][i] : sw[c][i];
+            sums[1][at] = sb[c][i] = k ? sums[1][at] + sb[c][i] : sb[c][i];
+          }
+      }
+      __syncthreads();
+    }
+    if (threadIdx.x / TR != kRows - 1) return;
+  }
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    if (t + c * TR >= chunks) continue;
+    const long at = (long)blockIdx.x * D + (t + c * TR) * E;
+#pragma unroll
+    for (int i = 0; i < E; i += 4) {
+      *reinterpret_cast<f32x4*>(dw + at + i) = f32x4{sw[c][i], sw[c][i + 1], sw[c][i + 2], sw[c][i + 3]};
+      *reinterpret_cast<f32x4*>(db + at + i) = f32x4{sb[c][i], sb[c][i + 1], sb[c][i + 2], sb[c][i + 3]};
+    }
+  }
+}
+
 // One workgroup per row: three passes over the row (its second and third reads
 // come from the caches).
 template <typename T, typename W>
@@ -86,20 +277,28 @@ __global__ __launch_bounds__(256) void layer_norm_parts_kernel(const T* __restri
   db[(long)blockIdx.y * D + c] = sb;
 }
 
-// The parts' sums, in order, rounded to the parameters' type.
+// The parts' sums, rounded to the parameters' type: blockIdx.y 0: dw, 1: db.  16
+// columns per workgroup, each by 16 threads that take every 16th part.
 template <typename W>
 __global__ __launch_bounds__(256) void layer_norm_join_kernel(const float* __restrict__ pw, const float* __restrict__ pb,
                                                               int parts, int D, W* __restrict__ dw,
                                                               W* __restrict__ db) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= D) return;
-  float sw = 0.f, sb = 0.f;
-  for (int p = 0; p < parts; ++p) {
-    sw += pw[(long)p * D + c];
-    sb += pb[(long)p * D + c];
+  __shared__ float sums[16][17];
+  W* const out = blockIdx.y ? db : dw;
+  if (!out) return;
+  const float* const p = blockIdx.y ? pb : pw;
+  const int x = threadIdx.x & 15, g = threadIdx.x >> 4, c = blockIdx.x * 16 + x;
+  float s = 0.f;
+  if (c < D) {
+#pragma unroll 8
+    for (int k = g; k < parts; k += 16) s += p[(long)k * D + c];
   }
-  if (dw) dw[c] = f32_to_elem<W>(sw);
-  if (db) db[c] = f32_to_elem<W>(sb);
+  sums[g][x] = s;
+  __syncthreads();
+  if (g != 0 || c >= D) return;
+#pragma unroll
+  for (int k = 1; k < 16; ++k) s += sums[k][x];
+  out[c] = f32_to_elem<W>(s);
 }
 
 constexpr long kNormMaxD = 1L << 20;
@@ -117,16 +316,19 @@ int check_norm(int64_t N, int64_t D, int dtype, int64_t ldx, int wdtype) {
 
 struct NormLayout {
   int parts;
-  long rows;
   float *dw, *db;
   size_t bytes;
 };
 
+// Workgroups that share out the rows of a backward, each with its part of dw and
+// db: enough to fill the card, few enough that the parts are little next to the
+// rows.
+constexpr long kNormParts = 1024;
+
 NormLayout norm_layout(void* ws, long N, long D) {
   Carver c(ws);
   NormLayout L;
-  L.rows = std::max<long>(64, ceil_div(std::max<long>(N, 1), 256));
-  L.parts = (int)ceil_div(std::max<long>(N, 1), L.rows);
+  L.parts = (int)std::max<long>(1, std::min(kNormParts, ceil_div(N, 4)));
   L.dw = c.take<float>((size_t)L.parts * D);
   L.db = c.take<float>((size_t)L.parts * D);
   L.bytes = align_up(c.off, 256);
@@ -141,14 +343,51 @@ int norm_types(int dtype, int wdtype, F&& f) {
   return f(0.f, 0.f);
 }
 
+// Whether rows of D elements of `size` bytes from p on, ld apart, are whole
+// chunks at 16-byte addresses.
+bool whole_chunks(const void* p, long ld, long D, size_t size) {
+  return !misaligned(p) && D * size % 16 == 0 && ld * size % 16 == 0;
+}
+
+// Calls f(TR, C) as integral constants for rows of so many chunks; false: too many.
+template <typename F>
+bool norm_shape(long chunks, F&& f) {
+  auto by = [&](auto tr) {
+    constexpr int TR = decltype(tr)::value;
+    if (chunks <= TR * 2)
+      f(tr, std::integral_constant<int, 2>{});
+    else
+      f(tr, std::integral_constant<int, 4>{});
+  };
+  if (chunks <= 64 * 4)
+    by(std::integral_constant<int, 64>{});
+  else if (chunks <= 256 * 4)
+    by(std::integral_constant<int, 256>{});
+  else if (chunks <= 1024 * 4)
+    by(std::integral_constant<int, 1024>{});
+  else
+    return false;
+  return true;
+}
+
 int norm_forward(const void* x, int dtype, int64_t ldx, const void* weight, const void* bias, int wdtype, int64_t N,
                  int64_t D, float eps, void* y, float* mean, float* rstd, hipStream_t st) {
   return norm_types(dtype, wdtype, [&](auto t, auto w) {
     typedef decltype(t) T;
     typedef decltype(w) W;
-    hipLaunchKernelGGL((layer_norm_fwd_kernel<T, W>), dim3((unsigned)N), dim3(256), 0, st, static_cast<const T*>(x),
-                       (long)ldx, static_cast<const W*>(weight), static_cast<const W*>(bias), (int)D, eps,
-                       static_cast<T*>(y), mean, rstd);
+    const bool in_registers =
+        whole_chunks(x, N > 1 ? ldx : D, D, sizeof(T)) && whole_chunks(y, D, D, sizeof(T)) &&
+        norm_shape(D * (long)sizeof(T) / 16, [&](auto tr, auto c) {
+          constexpr int TR = decltype(tr)::value, kRows = TR < 256 ? 256 / TR : 1;
+          const unsigned grid = (unsigned)std::min<long>(ceil_div(N, kRows), 2048);
+          hipLaunchKernelGGL((layer_norm_fwd_rows_kernel<T, TR, decltype(c)::value>), dim3(grid), dim3(std::max(TR, 256)),
+                             0, st, static_cast<const T*>(x), (long)ldx, weight, bias, (int)(wdtype == CCE_DTYPE_F32),
+                             (long)N, (int)D, eps, static_cast<T*>(y), mean, rstd);
+        });
+    if (!in_registers)
+      hipLaunchKernelGGL((layer_norm_fwd_kernel<T, W>), dim3((unsigned)N), dim3(256), 0, st, static_cast<const T*>(x),
+                         (long)ldx, static_cast<const W*>(weight), static_cast<const W*>(bias), (int)D, eps,
+                         static_cast<T*>(y), mean, rstd);
     HIP_TRY(hipGetLastError());
     return CCE_OK;
   });
@@ -160,18 +399,31 @@ int norm_backward(const void* dy, const void* x, int dtype, int64_t ldx, const v
   return norm_types(dtype, wdtype, [&](auto t, auto w) {
     typedef decltype(t) T;
     typedef decltype(w) W;
-    if (dx && N > 0) {
+    const bool params = dw || db;
+    const bool in_registers =
+        whole_chunks(x, N > 1 ? ldx : D, D, sizeof(T)) && whole_chunks(dy, D, D, sizeof(T)) && !misaligned(dx) &&
+        norm_shape(D * (long)sizeof(T) / 16, [&](auto tr, auto c) {
+          constexpr int TR = decltype(tr)::value;
+          hipLaunchKernelGGL((layer_norm_bwd_rows_kernel<T, TR, decltype(c)::value>), dim3((unsigned)L.parts),
+                             dim3(std::max(TR, 256)), 0, st, static_cast<const T*>(dy), static_cast<const T*>(x),
+                             (long)ldx, weight, (int)(wdtype == CCE_DTYPE_F32), mean, rstd, (long)N, (int)D,
+                             static_cast<T*>(dx), params ? L.dw : nullptr, L.db);
+        });
+    HIP_TRY(hipGetLastError());
+    if (!in_registers && dx && N > 0) {
       hipLaunchKernelGGL((layer_norm_dx_kernel<T, W>), dim3((unsigned)N), dim3(256), 0, st, static_cast<const T*>(dy),
                          static_cast<const T*>(x), (long)ldx, static_cast<const W*>(weight), mean, rstd, (int)D,
                          static_cast<T*>(dx));
       HIP_TRY(hipGetLastError());
     }
-    if (!dw && !db) return CCE_OK;
-    hipLaunchKernelGGL(layer_norm_parts_kernel<T>, dim3((unsigned)ceil_div(D, 256), (unsigned)L.parts), dim3(256), 0,
-                       st, static_cast<const T*>(dy), static_cast<const T*>(x), (long)ldx, mean, rstd, (long)N, (int)D,
-                       L.rows, L.dw, L.db);
-    HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL(layer_norm_join_kernel<W>, dim3((unsigned)ceil_div(D, 256)), dim3(256), 0, st, L.dw, L.db,
+    if (!params) return CCE_OK;
+    if (!in_registers) {
+      hipLaunchKernelGGL(layer_norm_parts_kernel<T>, dim3((unsigned)ceil_div(D, 256), (unsigned)L.parts), dim3(256), 0,
+                         st, static_cast<const T*>(dy), static_cast<const T*>(x), (long)ldx, mean, rstd, (long)N, (int)D,
+                         ceil_div(N, (long)L.parts), L.dw, L.db);
+      HIP_TRY(hipGetLastError());
+    }
+    hipLaunchKernelGGL(layer_norm_join_kernel<W>, dim3((unsigned)ceil_div(D, 16), 2), dim3(256), 0, st, L.dw, L.db,
                        L.parts, (int)D, static_cast<W*>(dw), static_cast<W*>(db));
     HIP_TRY(hipGetLastError());
     return CCE_OK;

@@ -4,7 +4,11 @@
 // Python take longer than the kernels of a small call: 16 rows of fp32 logits,
 // V 151936, forward and backward (43 us of kernels) took 179 us with Python
 // operators over ctypes and take 87 us with these; 64 rows of d 896 against
-// V 32000 went from 222 to 143 us.
+// V 32000 went from 222 to 143 us.  Layer norm and the distillation losses have
+// their autograd functions here too: a backward in Python waits for the
+// interpreter's lock in the autograd thread.  Forward and backward with a Python
+// function / so: layer norm of 16384 x 896 106 / 76 us, the fused distillation of
+// 64 rows against V 32000 154 / 119 us.
 //
 // ops.py defines the schemas and the fake (meta) implementations; the kernels
 // are registered here.  The C functions come from the library that the Python
@@ -15,11 +19,13 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -533,6 +539,162 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor& grad_y, const Te
   return {dx, dw, db};
 }
 
+// ---------------------------------------------------------------------------
+// Differentiable operators: autograd functions over the ones above, which they
+// call through the dispatcher, so that a trace sees those.  The gradients are
+// kernels' results and have none of their own.
+// ---------------------------------------------------------------------------
+using c10::SymInt;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+template <typename Sig>
+c10::TypedOperatorHandle<Sig> find(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Sig>();
+}
+
+// [..., D] as [N, D] with a contiguous last dimension and rows that do not overlap.
+Tensor as_rows(const Tensor& t) {
+  const Tensor r = t.dim() == 2 ? t : t.reshape_symint({SymInt(-1), t.sym_size(-1)});
+  if ((r.sym_size(1) > 1 && r.sym_stride(1) != 1) || (r.sym_size(0) > 1 && r.sym_stride(0) < r.sym_size(1)))
+    return r.contiguous();
+  return r;
+}
+
+optional<Tensor> given(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : std::nullopt; }
+optional<Tensor> contiguous(const optional<Tensor>& t) { return t.has_value() ? optional<Tensor>(t->contiguous()) : t; }
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const optional<Tensor>& weight,
+                        const optional<Tensor>& bias, double eps) {
+    static const auto fwd =
+        find<std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const optional<Tensor>&, const optional<Tensor>&, double)>(
+            "chronicals_hip::layer_norm_fwd");
+    const Tensor rows = as_rows(x);
+    const auto [y, mean, rstd] = fwd.call(rows, weight, bias, eps);
+    ctx->save_for_backward({rows, weight.value_or(Tensor()), mean, rstd});
+    const optional<Tensor>& p = weight.has_value() ? weight : bias;
+    ctx->saved_data["param_f32"] = p.has_value() && p->scalar_type() == at::kFloat;
+    ctx->saved_data["bias"] = bias.has_value();
+    return y.view_symint(x.sym_sizes());
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    static const auto bwd =
+        find<std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const optional<Tensor>&, const Tensor&,
+                                                const Tensor&, bool, bool, bool, bool)>("chronicals_hip::layer_norm_bwd");
+    const auto saved = ctx->get_saved_variables();
+    // absent inputs have no edge
+    const bool has_w = saved[1].defined(), need_dx = ctx->needs_input_grad(0),
+               need_dw = has_w && ctx->needs_input_grad(1),
+               need_db = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(has_w ? 2 : 1);
+    if (!need_dx && !need_dw && !need_db) return variable_list(4);
+    const Tensor g = grads[0].reshape_symint(saved[0].sym_sizes()).contiguous();
+    const auto [dx, dw, db] = bwd.call(g, saved[0], given(saved[1]), saved[2], saved[3],
+                                       ctx->saved_data["param_f32"].toBool(), need_dx, need_dw, need_db);
+    return {need_dx ? dx.view_symint(grads[0].sym_sizes()) : Tensor(), need_dw ? dw : Tensor(), need_db ? db : Tensor(),
+            Tensor()};
+  }
+};
+
+Tensor layer_norm(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias, double eps) {
+  return LayerNorm::apply(x, contiguous(weight), contiguous(bias), eps);
+}
+
+// The teacher's tensors are contiguous [N, K], labels contiguous [N] or undefined.
+struct DistillLogits : torch::autograd::Function<DistillLogits> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& logits, const Tensor& t, const Tensor& index,
+                        const optional<Tensor>& labels, double temperature, double distill_weight, double ce_weight,
+                        int64_t ignore_index, int64_t reduction) {
+    static const auto fwd =
+        find<std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const optional<Tensor>&, double,
+                                                double, double, SymInt, SymInt)>("chronicals_hip::distill_logits_fwd");
+    const Tensor x = as_rows(logits);
+    const auto [loss, stats, n_valid] =
+        fwd.call(x, t, index, labels, temperature, distill_weight, ce_weight, ignore_index, reduction);
+    ctx->save_for_backward({x, t, index, labels.value_or(Tensor()), stats, n_valid});
+    ctx->saved_data["how"] = std::vector<double>{temperature, distill_weight, ce_weight};
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->saved_data["reduction"] = reduction;
+    ctx->saved_data["dim"] = logits.dim();
+    if (logits.dim() != 2) ctx->saved_data["shape"] = logits.sym_sizes();
+    return reduction == CCE_REDUCTION_NONE ? loss : loss.reshape(at::IntArrayRef());
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    static const auto bwd =
+        find<Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const optional<Tensor>&, const Tensor&,
+                    const Tensor&, double, double, double, SymInt, SymInt)>("chronicals_hip::distill_logits_bwd");
+    variable_list out(9);
+    if (!ctx->needs_input_grad(0)) return out;
+    const auto s = ctx->get_saved_variables();
+    const auto how = ctx->saved_data["how"].toDoubleVector();
+    out[0] = bwd.call(grads[0], s[0], s[1], s[2], given(s[3]), s[4], s[5], how[0], how[1], how[2],
+                      ctx->saved_data["ignore_index"].toInt(), ctx->saved_data["reduction"].toInt());
+    if (ctx->saved_data["dim"].toInt() != 2) out[0] = out[0].view_symint(ctx->saved_data["shape"].toSymIntVector());
+    return out;
+  }
+};
+
+Tensor distill_logits(const Tensor& logits, const Tensor& t, const Tensor& index, const optional<Tensor>& labels,
+                      double temperature, double distill_weight, double ce_weight, int64_t ignore_index,
+                      int64_t reduction) {
+  return DistillLogits::apply(logits, t, index, labels, temperature, distill_weight, ce_weight,
+                              ignore_index, reduction);
+}
+
+struct DistillLinear : torch::autograd::Function<DistillLinear> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const optional<Tensor>& bias,
+                        const Tensor& t, const Tensor& index, const optional<Tensor>& labels, int64_t chunk_size,
+                        double temperature, double distill_weight, double ce_weight, int64_t ignore_index,
+                        int64_t reduction) {
+    static const auto fwd = find<std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>(
+        const Tensor&, const Tensor&, const optional<Tensor>&, const Tensor&, const Tensor&, const optional<Tensor>&, double,
+        double, double, SymInt, SymInt)>("chronicals_hip::distill_fwd");
+    // fp16 and fp32 operands are rounded to bf16, the GEMMs' type
+    const Tensor h = as_rows(hidden).to(at::kBFloat16).contiguous(), w = weight.to(at::kBFloat16).contiguous();
+    const Tensor b = bias.has_value() ? bias->to(at::kFloat).contiguous() : Tensor();
+    const auto [loss, stats, entry_logits, rows, n_valid] = fwd.call(
+        h, w, given(b), t, index, labels, temperature, distill_weight, ce_weight, ignore_index, reduction);
+    ctx->save_for_backward({h, w, b, t, index, stats, entry_logits, rows, n_valid});
+    ctx->saved_data["how"] = std::vector<double>{temperature, distill_weight, ce_weight};
+    ctx->saved_data["reduction"] = reduction;
+    ctx->saved_data["chunk_size"] = chunk_size;
+    ctx->saved_data["shape"] = hidden.sym_sizes();
+    ctx->saved_data["hidden"] = (int64_t)hidden.scalar_type();
+    ctx->saved_data["weight"] = (int64_t)weight.scalar_type();
+    if (bias.has_value()) ctx->saved_data["bias"] = (int64_t)bias->scalar_type();
+    return reduction == CCE_REDUCTION_NONE ? loss : loss.reshape(at::IntArrayRef());
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    static const auto bwd = find<std::tuple<Tensor, Tensor, Tensor>(
+        const Tensor&, const Tensor&, const Tensor&, const optional<Tensor>&, const Tensor&, const Tensor&, const Tensor&,
+        const Tensor&, const Tensor&, const Tensor&, double, double, double, SymInt, SymInt, bool, bool, bool, bool,
+        bool)>("chronicals_hip::distill_bwd");
+    variable_list out(12);
+    const auto s = ctx->get_saved_variables();
+    const bool need_dh = ctx->needs_input_grad(0), need_dw = ctx->needs_input_grad(1),
+               need_db = s[2].defined() && ctx->needs_input_grad(2);
+    if (!need_dh && !need_dw && !need_db) return out;
+    auto& kept = ctx->saved_data;
+    const auto how = kept["how"].toDoubleVector();
+    const auto htype = (at::ScalarType)kept["hidden"].toInt(), wtype = (at::ScalarType)kept["weight"].toInt();
+    // bf16 inputs get bf16 gradients, fp16 and fp32 inputs get them from fp32
+    const auto [dh, dw, db] =
+        bwd.call(grads[0], s[0], s[1], given(s[2]), s[3], s[4], s[5], s[6], s[7], s[8], how[0], how[1], how[2],
+                 kept["reduction"].toInt(), kept["chunk_size"].toInt(), need_dh, need_dw, need_db,
+                 htype != at::kBFloat16, wtype != at::kBFloat16);
+    if (need_dh) out[0] = dh.view_symint(kept["shape"].toSymIntVector()).to(htype);
+    if (need_dw) out[1] = dw.to(wtype);
+    if (need_db) out[2] = db.to((at::ScalarType)kept["bias"].toInt());
+    return out;
+  }
+};
+
+Tensor distill_linear(const Tensor& hidden, const Tensor& weight, const optional<Tensor>& bias, const Tensor& t,
+                      const Tensor& index, const optional<Tensor>& labels, int64_t chunk_size, double temperature,
+                      double distill_weight, double ce_weight, int64_t ignore_index, int64_t reduction) {
+  return DistillLinear::apply(hidden, weight, bias, t, index, labels, chunk_size, temperature, distill_weight, ce_weight, ignore_index, reduction);
+}
+
 }  // namespace
 
 extern "C" {
@@ -600,7 +762,13 @@ TORCH_LIBRARY_IMPL(chronicals_hip, CUDA, m) {
   m.impl("layer_norm_bwd", layer_norm_bwd);
 }
 
-// The operators have no derivative of their own (the autograd functions call
+TORCH_LIBRARY_IMPL(chronicals_hip, CompositeImplicitAutograd, m) {
+  m.impl("layer_norm", layer_norm);
+  m.impl("distill_logits", distill_logits);
+  m.impl("distill_linear", distill_linear);
+}
+
+// The operators on HIP tensors have no derivative of their own (the autograd functions call
 // them): a backward through one raises.
 TORCH_LIBRARY_IMPL(chronicals_hip, Autograd, m) {
   for (const char* op : {"cce_fwd", "cce_bwd", "ce_logits_fwd", "ce_logits_bwd", "ce_logits_fwd_bwd",

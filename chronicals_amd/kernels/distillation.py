@@ -43,30 +43,26 @@ from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from .. import ops as _ops  # noqa: F401  (registers chronicals_hip::distill_* and top_logits)
-from .cut_cross_entropy import _as_bf16_rows, _reduction_code, get_optimal_chunk_size
+from .. import ops as _ops
+from .cut_cross_entropy import _reduction_code, get_optimal_chunk_size
 
 __all__ = [
     "top_logits",
     "distillation_loss",
     "DistillationLoss",
-    "DistillationFunction",
     "linear_distillation_loss",
     "LinearDistillationLoss",
-    "LinearDistillationFunction",
 ]
+
+_top_logits = _ops.top_logits.default
+_distill_logits = _ops.distill_logits.default
+_distill_linear = _ops.distill_linear.default
 
 MAX_ENTRIES = _lib.CCE_MAX_TEACHER_ENTRIES
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 _INTS = (torch.int64, torch.int32)
-
-
-def _check(cond: bool, msg: str) -> None:
-    if not cond:
-        raise RuntimeError(msg)
 
 
 def _logit_rows(logits: torch.Tensor) -> torch.Tensor:
@@ -78,41 +74,48 @@ def _logit_rows(logits: torch.Tensor) -> torch.Tensor:
 
 
 def _check_student(x: torch.Tensor, name: str, what: str) -> None:
-    _check(x.is_cuda, f"chronicals_amd {what} runs only on HIP devices: {name} must be a device tensor (got "
-                      f"{x.device})")
-    _check(x.dim() >= 1 and x.shape[-1] >= 1, f"{name} must be [..., D] with D >= 1, got shape {tuple(x.shape)}")
-    _check(x.dtype in _FLOATS, f"{name} dtype {x.dtype} not supported (bf16, fp16, fp32)")
+    if not x.is_cuda:
+        raise RuntimeError(f"chronicals_amd {what} runs only on HIP devices: {name} must be a device tensor (got "
+                           f"{x.device})")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise RuntimeError(f"{name} must be [..., D] with D >= 1, got shape {tuple(x.shape)}")
+    if x.dtype not in _FLOATS:
+        raise RuntimeError(f"{name} dtype {x.dtype} not supported (bf16, fp16, fp32)")
 
 
 def _teacher_rows(student: torch.Tensor, teacher_logits: torch.Tensor, teacher_indices: torch.Tensor,
                   labels: Optional[torch.Tensor], temperature: float, ce_weight: float):
     """The teacher's tensors as contiguous [N, K] and the labels as [N], for a student of shape [..., D]."""
-    lead = student.shape[:-1]
-    n = lead.numel()
-    _check(teacher_logits.dim() >= 1 and teacher_logits.shape[:-1] == lead,
-           f"teacher_logits must be [{', '.join(map(str, lead))}, K], got {tuple(teacher_logits.shape)}")
-    _check(teacher_indices.shape == teacher_logits.shape,
-           f"teacher_indices must have the shape {tuple(teacher_logits.shape)} of teacher_logits, got "
-           f"{tuple(teacher_indices.shape)}")
-    k = teacher_logits.shape[-1]
-    _check(1 <= k <= MAX_ENTRIES, f"a teacher has 1 to {MAX_ENTRIES} entries per row, got {k}")
-    _check(teacher_logits.dtype in _FLOATS, f"teacher_logits dtype {teacher_logits.dtype} not supported (bf16, fp16, "
-                                            "fp32)")
-    _check(teacher_indices.dtype in _INTS, f"teacher_indices must be int64 or int32, got {teacher_indices.dtype}")
-    _check(teacher_logits.device == student.device and teacher_indices.device == student.device,
-           "teacher_logits and teacher_indices must be on the student's device")
+    shape = teacher_logits.shape
+    if teacher_logits.dim() < 1 or shape[:-1] != student.shape[:-1]:
+        raise RuntimeError(f"teacher_logits must be {[*student.shape[:-1], 'K']}, got {tuple(shape)}")
+    if teacher_indices.shape != shape:
+        raise RuntimeError(f"teacher_indices must have the shape {tuple(shape)} of teacher_logits, got "
+                           f"{tuple(teacher_indices.shape)}")
+    if not 1 <= shape[-1] <= MAX_ENTRIES:
+        raise RuntimeError(f"a teacher has 1 to {MAX_ENTRIES} entries per row, got {shape[-1]}")
+    if teacher_logits.dtype not in _FLOATS:
+        raise RuntimeError(f"teacher_logits dtype {teacher_logits.dtype} not supported (bf16, fp16, fp32)")
+    if teacher_indices.dtype not in _INTS:
+        raise RuntimeError(f"teacher_indices must be int64 or int32, got {teacher_indices.dtype}")
+    if teacher_logits.device != student.device or teacher_indices.device != student.device:
+        raise RuntimeError("teacher_logits and teacher_indices must be on the student's device")
     if not 1e-2 <= temperature <= 1e3:
         raise ValueError(f"temperature must be in [0.01, 1000], got {temperature}")
+    n = shape[:-1].numel()
     if labels is None:
         if ce_weight != 0.0:
             raise ValueError("ce_weight needs labels")
-        lab = None
     else:
-        _check(labels.dtype in _INTS, f"labels must be int64 or int32, got {labels.dtype}")
-        _check(labels.numel() == n, f"labels has {labels.numel()} elements but the student has {n} rows")
-        _check(labels.device == student.device, "labels must be on the student's device")
-        lab = labels.reshape(-1).contiguous()
-    return teacher_logits.detach().reshape(n, k).contiguous(), teacher_indices.reshape(n, k).contiguous(), lab
+        if labels.dtype not in _INTS:
+            raise RuntimeError(f"labels must be int64 or int32, got {labels.dtype}")
+        if labels.numel() != n:
+            raise RuntimeError(f"labels has {labels.numel()} elements but the student has {n} rows")
+        if labels.device != student.device:
+            raise RuntimeError("labels must be on the student's device")
+        labels = labels.reshape(-1).contiguous()
+    return (teacher_logits.detach().reshape(n, shape[-1]).contiguous(),
+            teacher_indices.reshape(n, shape[-1]).contiguous(), labels)
 
 
 def top_logits(logits: torch.Tensor, k: int) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -126,31 +129,9 @@ def top_logits(logits: torch.Tensor, k: int) -> Tuple[torch.Tensor, torch.Tensor
     V = logits.shape[-1]
     if not 1 <= k <= min(V, MAX_ENTRIES):
         raise ValueError(f"k must be in [1, min({MAX_ENTRIES}, V = {V})], got {k}")
-    values, indices = torch.ops.chronicals_hip.top_logits(_logit_rows(logits.detach()), int(k))
+    values, indices = _top_logits(_logit_rows(logits.detach()), int(k))
     shape = (*logits.shape[:-1], k)
     return values.view(shape), indices.view(shape)
-
-
-class DistillationFunction(torch.autograd.Function):
-    """apply(logits2d, teacher_logits, teacher_indices, labels, temperature, distill_weight, ce_weight, ignore_index,
-    reduction_code) -> loss (scalar, or [N] for 'none').  Keeps four floats per row beyond the inputs."""
-
-    @staticmethod
-    def forward(ctx, x, t, index, labels, temperature, distill_weight, ce_weight, ignore_index, red):
-        how = (float(temperature), float(distill_weight), float(ce_weight), int(ignore_index), int(red))
-        loss, stats, n_valid = torch.ops.chronicals_hip.distill_logits_fwd(x, t, index, labels, *how)
-        ctx.save_for_backward(x, t, index, labels, stats, n_valid)
-        ctx.how = how
-        return loss if red == _lib.CCE_REDUCTION_NONE else loss.view(())
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_output):
-        if not ctx.needs_input_grad[0]:
-            return (None,) * 9
-        x, t, index, labels, stats, n_valid = ctx.saved_tensors
-        dx = torch.ops.chronicals_hip.distill_logits_bwd(grad_output, x, t, index, labels, stats, n_valid, *ctx.how)
-        return (dx,) + (None,) * 8
 
 
 def distillation_loss(
@@ -171,8 +152,7 @@ def distillation_loss(
     red = _reduction_code(reduction)
     _check_student(logits, "logits", "distillation_loss")
     t, index, lab = _teacher_rows(logits, teacher_logits, teacher_indices, labels, temperature, ce_weight)
-    loss = DistillationFunction.apply(_logit_rows(logits), t, index, lab, temperature, distill_weight, ce_weight,
-                                      ignore_index, red)
+    loss = _distill_logits(logits, t, index, lab, temperature, distill_weight, ce_weight, ignore_index, red)
     return loss.view(logits.shape[:-1]) if red == _lib.CCE_REDUCTION_NONE else loss
 
 
@@ -199,43 +179,6 @@ class DistillationLoss(nn.Module):
                 f"ce_weight={self.ce_weight}, ignore_index={self.ignore_index}, reduction={self.reduction!r}")
 
 
-class LinearDistillationFunction(torch.autograd.Function):
-    """apply(hidden, weight, bias, teacher_logits, teacher_indices, labels, chunk_size, temperature, distill_weight,
-    ce_weight, ignore_index, reduction_code) -> loss (scalar, or [N] for 'none').
-
-    Keeps the bf16 operands and, per row, K + 4 numbers of 32 bits.
-    """
-
-    @staticmethod
-    def forward(ctx, hidden, weight, bias, t, index, labels, chunk_size, temperature, distill_weight, ce_weight,
-                ignore_index, red):
-        h2 = _as_bf16_rows(hidden.detach().reshape(-1, hidden.shape[-1]))
-        w2 = _as_bf16_rows(weight.detach())
-        b32 = None if bias is None else bias.detach().to(torch.float32).contiguous()
-        how = (float(temperature), float(distill_weight), float(ce_weight))
-        loss, stats, entry_logits, rows, n_valid = torch.ops.chronicals_hip.distill_fwd(
-            h2, w2, b32, t, index, labels, *how, int(ignore_index), int(red))
-        ctx.save_for_backward(h2, w2, b32, t, index, stats, entry_logits, rows, n_valid)
-        ctx.cfg = (how, int(red), int(chunk_size))
-        ctx.shapes = (hidden.shape, hidden.dtype, weight.dtype, None if bias is None else bias.dtype)
-        return loss if red == _lib.CCE_REDUCTION_NONE else loss.view(())
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_output):
-        h2, w2, b32, t, index, stats, entry_logits, rows, n_valid = ctx.saved_tensors
-        how, red, chunk_size = ctx.cfg
-        hshape, hdtype, wdtype, bdtype = ctx.shapes
-        need_dh, need_dw, need_db = ctx.needs_input_grad[:3]
-        if not (need_dh or need_dw or need_db):
-            return (None,) * 12
-        dh, dw, db = torch.ops.chronicals_hip.distill_bwd(
-            grad_output, h2, w2, b32, t, index, stats, entry_logits, rows, n_valid, *how, red, chunk_size, need_dh,
-            need_dw, need_db, hdtype != torch.bfloat16, wdtype != torch.bfloat16)
-        return (dh.view(hshape).to(hdtype) if need_dh else None, dw.to(wdtype) if need_dw else None,
-                db.to(bdtype) if need_db else None) + (None,) * 9
-
-
 def linear_distillation_loss(
     hidden: torch.Tensor,
     weight: torch.Tensor,
@@ -259,18 +202,22 @@ def linear_distillation_loss(
     """
     red = _reduction_code(reduction)
     _check_student(hidden, "hidden", "linear_distillation_loss")
-    _check(weight.dim() == 2, f"weight must be [vocab_size, hidden_dim], got shape {tuple(weight.shape)}")
-    _check(weight.device == hidden.device, "hidden and weight must be on the same device")
-    _check(weight.dtype in _FLOATS, f"weight dtype {weight.dtype} not supported (bf16, fp16, fp32)")
-    _check(hidden.shape[-1] == weight.shape[1],
-           f"hidden last dim {hidden.shape[-1]} does not match weight hidden_dim {weight.shape[1]}")
+    if weight.dim() != 2:
+        raise RuntimeError(f"weight must be [vocab_size, hidden_dim], got shape {tuple(weight.shape)}")
+    if weight.device != hidden.device:
+        raise RuntimeError("hidden and weight must be on the same device")
+    if weight.dtype not in _FLOATS:
+        raise RuntimeError(f"weight dtype {weight.dtype} not supported (bf16, fp16, fp32)")
+    if hidden.shape[-1] != weight.shape[1]:
+        raise RuntimeError(f"hidden last dim {hidden.shape[-1]} does not match weight hidden_dim {weight.shape[1]}")
     if bias is not None:
-        _check(bias.dim() == 1 and bias.shape[0] == weight.shape[0],
-               f"bias must be [vocab_size={weight.shape[0]}], got {tuple(bias.shape)}")
-        _check(bias.device == hidden.device, "bias must be on the same device as hidden")
+        if bias.dim() != 1 or bias.shape[0] != weight.shape[0]:
+            raise RuntimeError(f"bias must be [vocab_size={weight.shape[0]}], got {tuple(bias.shape)}")
+        if bias.device != hidden.device:
+            raise RuntimeError("bias must be on the same device as hidden")
     t, index, lab = _teacher_rows(hidden, teacher_logits, teacher_indices, labels, temperature, ce_weight)
-    loss = LinearDistillationFunction.apply(hidden, weight, bias, t, index, lab, chunk_size, temperature,
-                                            distill_weight, ce_weight, ignore_index, red)
+    loss = _distill_linear(hidden, weight, bias, t, index, lab, chunk_size, temperature, distill_weight, ce_weight,
+                           ignore_index, red)
     return loss.view(hidden.shape[:-1]) if red == _lib.CCE_REDUCTION_NONE else loss
 
 

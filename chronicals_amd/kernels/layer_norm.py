@@ -11,7 +11,7 @@ the parameters'.
   * x is bf16, fp16 or fp32 of any shape; rows may be strided (a last dimension
     that is not contiguous is copied).  weight and bias are [D], either or both,
     of x's dtype or fp32, both alike.
-  * The gradients are written by HIP kernels and cannot be differentiated again.
+  * Its gradients are kernels' results and cannot be differentiated again.
 
 The reference has no layer norm of its own; the models that it fine-tunes bring
 torch's.
@@ -22,45 +22,12 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
-from .. import ops as _ops  # noqa: F401  (registers chronicals_hip::layer_norm_*)
+from .. import ops as _ops
 
-__all__ = ["layer_norm", "LayerNorm", "LayerNormFunction"]
+__all__ = ["layer_norm", "LayerNorm"]
 
-
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """[..., D] as [N, D] with a contiguous last dimension and rows that do not overlap."""
-    r = x.reshape(-1, x.shape[-1])
-    if (r.shape[1] > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and r.stride(0) < r.shape[1]):
-        r = r.contiguous()
-    return r
-
-
-class LayerNormFunction(torch.autograd.Function):
-    """apply(x, weight, bias, eps) -> y; keeps x and the rows' fp32 statistics."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        rows = _rows(x)
-        w = None if weight is None else weight.contiguous()
-        b = None if bias is None else bias.contiguous()
-        y, mean, rstd = torch.ops.chronicals_hip.layer_norm_fwd(rows, w, b, float(eps))
-        ctx.save_for_backward(rows, w, mean, rstd)
-        ctx.param_f32 = any(p is not None and p.dtype == torch.float32 for p in (w, b))
-        return y.view(x.shape)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_y):
-        rows, w, mean, rstd = ctx.saved_tensors
-        need_dx, need_dw, need_db = ctx.needs_input_grad[:3]
-        if not (need_dx or need_dw or need_db):
-            return None, None, None, None
-        g = grad_y.reshape(rows.shape).contiguous()
-        dx, dw, db = torch.ops.chronicals_hip.layer_norm_bwd(g, rows, w, mean, rstd, ctx.param_f32, need_dx, need_dw,
-                                                             need_db)
-        return (dx.view(grad_y.shape) if need_dx else None, dw if need_dw else None, db if need_db else None, None)
+_layer_norm = _ops.layer_norm.default
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -86,7 +53,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
             raise RuntimeError(f"{name} must have x's dtype {x.dtype} or fp32, got {p.dtype}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise RuntimeError(f"weight and bias must have the same dtype, got {weight.dtype} and {bias.dtype}")
-    return LayerNormFunction.apply(x, weight, bias, eps)
+    return _layer_norm(x, weight, bias, eps)
 
 
 class LayerNorm(nn.Module):

@@ -43,7 +43,7 @@ from . import build as _build
 
 __all__ = ["cce_fwd", "cce_bwd", "ce_logits_fwd", "ce_logits_bwd", "ce_logits_bwd_", "ce_logits_fwd_bwd",
            "ce_logits_fwd_bwd_", "distill_logits_fwd", "distill_logits_bwd", "distill_fwd", "distill_bwd", "top_logits",
-           "layer_norm_fwd", "layer_norm_bwd"]
+           "layer_norm_fwd", "layer_norm_bwd", "layer_norm", "distill_logits", "distill_linear"]
 
 _SCHEMAS = (
     "cce_fwd(Tensor hidden, Tensor weight, Tensor labels, Tensor? bias, SymInt ignore_index, float label_smoothing, "
@@ -76,8 +76,17 @@ _SCHEMAS = (
     "layer_norm_bwd(Tensor grad_y, Tensor x, Tensor? weight, Tensor mean, Tensor rstd, bool param_f32, "
     "bool need_dx, bool need_dw, bool need_db) -> (Tensor, Tensor, Tensor)",
 )
+# differentiable, made of the operators above
+_COMPOSITE = (
+    "layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps) -> Tensor",
+    "distill_logits(Tensor logits, Tensor teacher_logits, Tensor teacher_indices, Tensor? labels, float temperature, "
+    "float distill_weight, float ce_weight, int ignore_index, int reduction) -> Tensor",
+    "distill_linear(Tensor hidden, Tensor weight, Tensor? bias, Tensor teacher_logits, Tensor teacher_indices, "
+    "Tensor? labels, int chunk_size, float temperature, float distill_weight, float ce_weight, int ignore_index, "
+    "int reduction) -> Tensor",
+)
 _LIBRARY = torch.library.Library("chronicals_hip", "FRAGMENT")
-for _s in _SCHEMAS:
+for _s in _SCHEMAS + _COMPOSITE:
     _LIBRARY.define(_s, tags=(torch.Tag.pt2_compliant_tag,))
 
 
@@ -115,6 +124,8 @@ def _unbuilt(name: str):
 if not _load_kernels():
     for _s in _SCHEMAS:
         _LIBRARY.impl(_s.split("(", 1)[0], _unbuilt(_s.split("(", 1)[0]), "CUDA")
+    for _s in _COMPOSITE:
+        _LIBRARY.impl(_s.split("(", 1)[0], _unbuilt(_s.split("(", 1)[0]), "CompositeImplicitAutograd")
 
 
 def _stream(device: torch.device) -> int:
@@ -285,6 +296,8 @@ def _ce_logits_fwd_bwd__fake(logits, labels, ignore_index, label_smoothing, z_lo
 # int32) are contiguous; the students' operands are those of ce_logits_* and
 # cce_*.  What a forward returns beside the loss is for the backward of the same
 # operands.  layer_norm_* take [N, D] rows with a contiguous last dimension.
+# layer_norm, distill_logits and distill_linear are the differentiable ones over
+# these, for tensors of any leading shape.
 # ---------------------------------------------------------------------------
 
 def _loss_fake(x, reduction):
@@ -351,3 +364,6 @@ distill_bwd = torch.ops.chronicals_hip.distill_bwd
 top_logits = torch.ops.chronicals_hip.top_logits
 layer_norm_fwd = torch.ops.chronicals_hip.layer_norm_fwd
 layer_norm_bwd = torch.ops.chronicals_hip.layer_norm_bwd
+layer_norm = torch.ops.chronicals_hip.layer_norm
+distill_logits = torch.ops.chronicals_hip.distill_logits
+distill_linear = torch.ops.chronicals_hip.distill_linear

@@ -127,6 +127,28 @@ def test_fakes():
     assert dx.dtype == torch.bfloat16 and dw.shape == (50,) and dw.dtype == torch.float32 and db.shape == (0,)
 
 
+def test_differentiable_operators_trace():
+    """A trace of forward and backward holds the operators underneath, with sizes that stay symbolic."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    ops = torch.ops.chronicals_hip
+
+    def f(x, h, w, b, t, i, lab):
+        n = ops.layer_norm(h, w[0], None, 1e-5)
+        loss = ops.distill_linear(n, w, b, t, i, lab, 8192, 2.0, 0.5, 0.5, -100, 1)
+        loss = loss + ops.distill_logits(x, t, i, None, 1.0, 1.0, 0.0, -100, 1)
+        return torch.autograd.grad(loss, [x, h, w, b])
+
+    def leaf(*shape):
+        return meta(*shape).requires_grad_(True)
+    args = (leaf(3, 4, 50), leaf(3, 4, 16), leaf(50, 16), leaf(50), meta(12, 5), meta(12, 5, dtype=torch.int64),
+            meta(12, dtype=torch.int64))
+    for mode in ("fake", "symbolic"):
+        graph = make_fx(f, tracing_mode=mode)(*args).graph
+        called = [str(n.target) for n in graph.nodes if "chronicals_hip" in str(n.target)]
+        assert sorted(c.split(".")[1] for c in called) == ["distill_bwd", "distill_fwd", "distill_logits_bwd",
+                                                           "distill_logits_fwd", "layer_norm_bwd", "layer_norm_fwd"]
+
+
 # ---------------------------------------------------------------------------
 # the C entry points: refusals come before any call to the device
 # ---------------------------------------------------------------------------
