@@ -10,18 +10,16 @@
 // forward reads x and writes y, the backward reads x and dy and writes dx.
 
 //
-// Rows of whole 16-byte chunks at 16-byte addresses stay in registers: TR threads
-// hold up to C chunks each, a wave per row up to 256 chunks, then a workgroup of
-// 256 or 1024.  A workgroup goes on to further rows with the parameters in its
-// registers, and in the backward with its share of dw and db there too.  What
-// does not fit (odd sizes or strides, more than 4096 chunks) goes by the kernels
-// below, which read a row two or three times.
+// Rows stay in registers: TR threads hold up to C chunks of 16 bytes each, a wave
+// per row up to 256 chunks, then a workgroup of 256 or 1024.  A workgroup goes on
+// to further rows with the parameters in its registers, and in the backward with
+// its share of dw and db there too.  Rows need no alignment (16-byte accesses at
+// the element's), and a last chunk that is not whole goes element by element.
+// Longer rows go by the kernels below, which read them two or three times.
 
-// Parameter c, fp32 or of type T.
-template <typename T>
-__device__ inline float load_param(const void* p, int f32, long c) {
-  return f32 ? static_cast<const float*>(p)[c] : elem_to_f32(static_cast<const T*>(p)[c]);
-}
+// Sixteen bytes at any element.
+typedef u32x4 loose_u32x4 __attribute__((aligned(2)));
+typedef f32x4 loose_f32x4 __attribute__((aligned(4)));
 
 // Sums of two values over the TR threads of a row (fixed order).
 template <int TR>
@@ -47,39 +45,76 @@ __device__ inline void row_sums(float& a, float& b, float (*red)[2]) {
   }
 }
 
-// The chunks of a row that thread t of TR holds, as fp32: chunk t + c * TR.
+// The chunks of a row of D elements that thread t of TR holds, as fp32: chunk t +
+// c * TR.  Elements past the row's end are 0.
 template <typename T, int TR, int C>
 struct RowRegs {
   static constexpr int E = 16 / sizeof(T);
   float v[C][E];
-  __device__ inline void load(const T* row, int chunks, int t) {
-    u32x4 raw[C];
+  static __device__ inline int first(int c, int t) { return (t + c * TR) * E; }
+  // a row's whole chunks on their way
+  struct Raw {
+    u32x4 v[C];
+    __device__ inline void issue(const T* row, int D, int t) {
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-      if (t + c * TR < chunks) raw[c] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(row) + t + c * TR);
+      for (int c = 0; c < C; ++c) {
+        v[c] = u32x4{0u, 0u, 0u, 0u};
+        if (first(c, t) + E <= D)
+          v[c] = __builtin_nontemporal_load(reinterpret_cast<const loose_u32x4*>(row + first(c, t)));
+      }
+    }
+  };
+  __device__ inline void take(const Raw& raw, const T* row, int D, int t) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const T* e = reinterpret_cast<const T*>(&raw[c]);
+      const T* e = reinterpret_cast<const T*>(&raw.v[c]);
 #pragma unroll
-      for (int i = 0; i < E; ++i) v[c][i] = t + c * TR < chunks ? elem_to_f32(e[i]) : 0.f;
+      for (int i = 0; i < E; ++i) v[c][i] = elem_to_f32(e[i]);
+    }
+    tail(D, t, [&](float& x, int at) { x = elem_to_f32(row[at]); });
+  }
+  // f(value, position) for the elements of a last chunk that is not whole
+  template <typename F>
+  __device__ inline void tail(int D, int t, F&& f) {
+    if (D % E == 0) return;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      if (first(c, t) >= D || first(c, t) + E <= D) continue;
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (first(c, t) + i < D) f(v[c][i], first(c, t) + i);
     }
   }
-  __device__ inline void load_params(const void* p, int f32, int chunks, int t, float none) {
+  // parameters, fp32 or of type T (null: `none`)
+  __device__ inline void load_params(const void* p, int f32, int D, int t, float none) {
+    if (p && !f32) {
+      Raw raw;
+      raw.issue(static_cast<const T*>(p), D, t);
+      take(raw, static_cast<const T*>(p), D, t);
+      return;
+    }
+    const float* const q = static_cast<const float*>(p);
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-      for (int i = 0; i < E; ++i)
-        v[c][i] = p && t + c * TR < chunks ? load_param<T>(p, f32, (t + c * TR) * E + i) : none;
+      for (int i = 0; i < E; i += 4) {
+        f32x4 e = {none, none, none, none};
+        if (p && first(c, t) + E <= D) e = *reinterpret_cast<const loose_f32x4*>(q + first(c, t) + i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[c][i + k] = e[k];
+      }
+    if (p) tail(D, t, [&](float& x, int at) { x = q[at]; });
   }
-  __device__ inline void store(T* row, int chunks, int t) const {
+  __device__ inline void store(T* row, int D, int t) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       u32x4 raw;
       T* e = reinterpret_cast<T*>(&raw);
 #pragma unroll
       for (int i = 0; i < E; ++i) e[i] = f32_to_elem<T>(v[c][i]);
-      if (t + c * TR < chunks) __builtin_nontemporal_store(raw, reinterpret_cast<u32x4*>(row) + t + c * TR);
+      if (first(c, t) + E <= D) __builtin_nontemporal_store(raw, reinterpret_cast<loose_u32x4*>(row + first(c, t)));
     }
+    tail(D, t, [&](float& x, int at) { row[at] = f32_to_elem<T>(x); });
   }
 };
 
@@ -90,14 +125,16 @@ __global__ __launch_bounds__(TR < 256 ? 256 : TR) void layer_norm_fwd_rows_kerne
   typedef RowRegs<T, TR, C> Row;
   constexpr int kRows = TR < 256 ? 256 / TR : 1;  // rows of a workgroup at a time
   __shared__ float red[TR / 64][2];
-  const int t = threadIdx.x % TR, chunks = D / Row::E;
+  const int t = threadIdx.x % TR;
   const float inv = 1.f / (float)D;
   Row wr, br;
-  wr.load_params(w, param_f32, chunks, t, 1.f);
-  br.load_params(b, param_f32, chunks, t, 0.f);
+  wr.load_params(w, param_f32, D, t, 1.f);
+  br.load_params(b, param_f32, D, t, 0.f);
   for (long n = (long)blockIdx.x * kRows + threadIdx.x / TR; n < N; n += (long)gridDim.x * kRows) {
     Row x;
-    x.load(X + n * ldx, chunks, t);
+    typename Row::Raw raw;
+    raw.issue(X + n * ldx, D, t);
+    x.take(raw, X + n * ldx, D, t);
     float s = 0.f, q = 0.f;
 #pragma unroll
     for (int c = 0; c < C; ++c)
@@ -110,7 +147,7 @@ __global__ __launch_bounds__(TR < 256 ? 256 : TR) void layer_norm_fwd_rows_kerne
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int i = 0; i < Row::E; ++i) {
-        x.v[c][i] = t + c * TR < chunks ? x.v[c][i] - mean : 0.f;
+        x.v[c][i] = Row::first(c, t) + i < D ? x.v[c][i] - mean : 0.f;
         s += x.v[c][i] * x.v[c][i];
       }
     row_sums<TR>(s, q, red);
@@ -119,7 +156,7 @@ __global__ __launch_bounds__(TR < 256 ? 256 : TR) void layer_norm_fwd_rows_kerne
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int i = 0; i < Row::E; ++i) x.v[c][i] = __builtin_fmaf(x.v[c][i] * rstd, wr.v[c][i], br.v[c][i]);
-    x.store(Y + n * D, chunks, t);
+    x.store(Y + n * D, D, t);
     if (t == 0) {
       mean_out[n] = mean;
       rstd_out[n] = rstd;
@@ -136,16 +173,30 @@ __global__ __launch_bounds__(TR < 256 ? 256 : TR) void layer_norm_bwd_rows_kerne
   typedef RowRegs<T, TR, C> Row;
   constexpr int kRows = TR < 256 ? 256 / TR : 1, E = Row::E;
   __shared__ float red[TR / 64][2];
-  const int t = threadIdx.x % TR, chunks = D / E;
+  const int t = threadIdx.x % TR;
   const float inv = 1.f / (float)D;
   Row wr;
-  wr.load_params(w, param_f32, chunks, t, 1.f);
+  wr.load_params(w, param_f32, D, t, 1.f);
   float sw[C][E] = {}, sb[C][E] = {};
-  for (long n = (long)blockIdx.x * kRows + threadIdx.x / TR; n < N; n += (long)gridDim.x * kRows) {
+  const long step = (long)gridDim.x * kRows;
+  long n = (long)blockIdx.x * kRows + threadIdx.x / TR;
+  typename Row::Raw raw_x, raw_g;
+  float next_mu = 0.f, next_r = 0.f;
+  auto issue = [&](long m) {
+    raw_x.issue(X + m * ldx, D, t);
+    raw_g.issue(dY + m * D, D, t);
+    next_mu = mean[m];
+    next_r = rstd[m];
+  };
+  constexpr bool kAhead = TR < 1024;  // 1024 threads have no registers for it
+  if (kAhead && n < N) issue(n);
+  for (; n < N; n += step) {
+    if (!kAhead) issue(n);
     Row x, g;
-    x.load(X + n * ldx, chunks, t);
-    g.load(dY + n * D, chunks, t);
-    const float mu = mean[n], r = rstd[n];
+    x.take(raw_x, X + n * ldx, D, t);
+    g.take(raw_g, dY + n * D, D, t);
+    const float mu = next_mu, r = next_r;
+    if (kAhead && n + step < N) issue(n + step);  // the next row, while this one is worked on
     float sa = 0.f, san = 0.f;
 #pragma unroll
     for (int c = 0; c < C; ++c)
@@ -167,7 +218,7 @@ __global__ __launch_bounds__(TR < 256 ? 256 : TR) void layer_norm_bwd_rows_kerne
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int i = 0; i < E; ++i) x.v[c][i] = r * (g.v[c][i] - sa - x.v[c][i] * san);
-    x.store(dX + n * D, chunks, t);
+    x.store(dX + n * D, D, t);
   }
   if (!dw) return;
   // the rows' sums within the workgroup, one after the other
@@ -188,16 +239,25 @@ __global__ __launch_bounds__(TR < 256 ? 256 : TR) void layer_norm_bwd_rows_kerne
     }
     if (threadIdx.x / TR != kRows - 1) return;
   }
+  dw += (long)blockIdx.x * D;
+  db += (long)blockIdx.x * D;
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    if (t + c * TR >= chunks) continue;
-    const long at = (long)blockIdx.x * D + (t + c * TR) * E;
+  for (int c = 0; c < C; ++c)
 #pragma unroll
     for (int i = 0; i < E; i += 4) {
-      *reinterpret_cast<f32x4*>(dw + at + i) = f32x4{sw[c][i], sw[c][i + 1], sw[c][i + 2], sw[c][i + 3]};
-      *reinterpret_cast<f32x4*>(db + at + i) = f32x4{sb[c][i], sb[c][i + 1], sb[c][i + 2], sb[c][i + 3]};
+      const int at = Row::first(c, t) + i;
+      if (at + 4 <= D) {
+        *reinterpret_cast<loose_f32x4*>(dw + at) = f32x4{sw[c][i], sw[c][i + 1], sw[c][i + 2], sw[c][i + 3]};
+        *reinterpret_cast<loose_f32x4*>(db + at) = f32x4{sb[c][i], sb[c][i + 1], sb[c][i + 2], sb[c][i + 3]};
+        continue;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (at + k < D) {
+          dw[at + k] = sw[c][i + k];
+          db[at + k] = sb[c][i + k];
+        }
     }
-  }
 }
 
 // One workgroup per row: three passes over the row (its second and third reads
@@ -314,23 +374,32 @@ int check_norm(int64_t N, int64_t D, int dtype, int64_t ldx, int wdtype) {
   return CCE_OK;
 }
 
+// Workgroups of a forward.
+constexpr long kNormGroups = 1024;
+
+// Workgroups of a backward, each with a part of dw and db: enough to fill the
+// card, few enough that the parts are little next to the rows, which with a wave
+// per row they are from 32 rows each on (8192 x 2048 bf16: 256 parts 31 us, 512
+// 37; 16384 x 896: 34, 26; 65536 x 896 with 256, 512, 768: 118, 81, 73; a
+// workgroup per row, 8192 x 4096: 69, 53, 51, and of 1024 threads, 2048 x 16384:
+// 60, 78, 78).
+constexpr long kNormParts = 768;
+long norm_parts(long N, int threads) {
+  const long parts = threads == 64 ? std::min(std::max(N / 32, 256L), kNormParts) : threads == 256 ? 512 : 256;
+  return std::max<long>(1, std::min(parts, threads == 64 ? ceil_div(N, 4) : N));
+}
+
 struct NormLayout {
-  int parts;
   float *dw, *db;
   size_t bytes;
 };
 
-// Workgroups that share out the rows of a backward, each with its part of dw and
-// db: enough to fill the card, few enough that the parts are little next to the
-// rows.
-constexpr long kNormParts = 1024;
-
 NormLayout norm_layout(void* ws, long N, long D) {
   Carver c(ws);
   NormLayout L;
-  L.parts = (int)std::max<long>(1, std::min(kNormParts, ceil_div(N, 4)));
-  L.dw = c.take<float>((size_t)L.parts * D);
-  L.db = c.take<float>((size_t)L.parts * D);
+  const size_t parts = (size_t)std::max<long>(1, std::min(N, kNormParts));
+  L.dw = c.take<float>(parts * D);
+  L.db = c.take<float>(parts * D);
   L.bytes = align_up(c.off, 256);
   return L;
 }
@@ -343,47 +412,47 @@ int norm_types(int dtype, int wdtype, F&& f) {
   return f(0.f, 0.f);
 }
 
-// Whether rows of D elements of `size` bytes from p on, ld apart, are whole
-// chunks at 16-byte addresses.
-bool whole_chunks(const void* p, long ld, long D, size_t size) {
-  return !misaligned(p) && D * size % 16 == 0 && ld * size % 16 == 0;
-}
-
-// Calls f(TR, C) as integral constants for rows of so many chunks; false: too many.
-template <typename F>
-bool norm_shape(long chunks, F&& f) {
+// Calls f(TR, C) as integral constants for rows of D elements of E to a chunk;
+// false: more than kMost.
+template <int E, int kMost, typename F>
+bool norm_shape(long D, F&& f) {
+  const long chunks = ceil_div(D, E);
   auto by = [&](auto tr) {
     constexpr int TR = decltype(tr)::value;
-    if (chunks <= TR * 2)
-      f(tr, std::integral_constant<int, 2>{});
-    else
-      f(tr, std::integral_constant<int, 4>{});
+    if constexpr (TR * 2 * E < kMost) {
+      if (chunks > TR * 2) return f(tr, std::integral_constant<int, 4>{});
+    }
+    f(tr, std::integral_constant<int, 2>{});
   };
+  if (D > kMost) return false;
   if (chunks <= 64 * 4)
     by(std::integral_constant<int, 64>{});
   else if (chunks <= 256 * 4)
     by(std::integral_constant<int, 256>{});
-  else if (chunks <= 1024 * 4)
-    by(std::integral_constant<int, 1024>{});
   else
-    return false;
+    by(std::integral_constant<int, 1024>{});
   return true;
 }
+
+// The longest rows that stay in registers: 1024 threads with four chunks each, in
+// the backward with 16 elements each.  Past that it spills: 1024 x 20000 bf16 175
+// us, by the kernels for longer rows 134 (the forward 29, by those 100).
+template <typename T>
+constexpr int kNormFwdD = 1024 * 4 * 16 / (int)sizeof(T);
+constexpr int kNormBwdD = 1024 * 16;
 
 int norm_forward(const void* x, int dtype, int64_t ldx, const void* weight, const void* bias, int wdtype, int64_t N,
                  int64_t D, float eps, void* y, float* mean, float* rstd, hipStream_t st) {
   return norm_types(dtype, wdtype, [&](auto t, auto w) {
     typedef decltype(t) T;
     typedef decltype(w) W;
-    const bool in_registers =
-        whole_chunks(x, N > 1 ? ldx : D, D, sizeof(T)) && whole_chunks(y, D, D, sizeof(T)) &&
-        norm_shape(D * (long)sizeof(T) / 16, [&](auto tr, auto c) {
-          constexpr int TR = decltype(tr)::value, kRows = TR < 256 ? 256 / TR : 1;
-          const unsigned grid = (unsigned)std::min<long>(ceil_div(N, kRows), 2048);
-          hipLaunchKernelGGL((layer_norm_fwd_rows_kernel<T, TR, decltype(c)::value>), dim3(grid), dim3(std::max(TR, 256)),
-                             0, st, static_cast<const T*>(x), (long)ldx, weight, bias, (int)(wdtype == CCE_DTYPE_F32),
-                             (long)N, (int)D, eps, static_cast<T*>(y), mean, rstd);
-        });
+    const bool in_registers = norm_shape<16 / sizeof(T), kNormFwdD<T>>(D, [&](auto tr, auto c) {
+      constexpr int TR = decltype(tr)::value, kRows = TR < 256 ? 256 / TR : 1;
+      const unsigned grid = (unsigned)std::min<long>(ceil_div(N, kRows), kNormGroups);
+      hipLaunchKernelGGL((layer_norm_fwd_rows_kernel<T, TR, decltype(c)::value>), dim3(grid), dim3(std::max(TR, 256)), 0,
+                         st, static_cast<const T*>(x), (long)ldx, weight, bias, (int)(wdtype == CCE_DTYPE_F32), (long)N,
+                         (int)D, eps, static_cast<T*>(y), mean, rstd);
+    });
     if (!in_registers)
       hipLaunchKernelGGL((layer_norm_fwd_kernel<T, W>), dim3((unsigned)N), dim3(256), 0, st, static_cast<const T*>(x),
                          (long)ldx, static_cast<const W*>(weight), static_cast<const W*>(bias), (int)D, eps,
@@ -400,15 +469,15 @@ int norm_backward(const void* dy, const void* x, int dtype, int64_t ldx, const v
     typedef decltype(t) T;
     typedef decltype(w) W;
     const bool params = dw || db;
-    const bool in_registers =
-        whole_chunks(x, N > 1 ? ldx : D, D, sizeof(T)) && whole_chunks(dy, D, D, sizeof(T)) && !misaligned(dx) &&
-        norm_shape(D * (long)sizeof(T) / 16, [&](auto tr, auto c) {
-          constexpr int TR = decltype(tr)::value;
-          hipLaunchKernelGGL((layer_norm_bwd_rows_kernel<T, TR, decltype(c)::value>), dim3((unsigned)L.parts),
-                             dim3(std::max(TR, 256)), 0, st, static_cast<const T*>(dy), static_cast<const T*>(x),
-                             (long)ldx, weight, (int)(wdtype == CCE_DTYPE_F32), mean, rstd, (long)N, (int)D,
-                             static_cast<T*>(dx), params ? L.dw : nullptr, L.db);
-        });
+    long parts = norm_parts(N, 256);
+    const bool in_registers = norm_shape<16 / sizeof(T), kNormBwdD>(D, [&](auto tr, auto c) {
+      constexpr int TR = decltype(tr)::value;
+      parts = norm_parts(N, TR);
+      hipLaunchKernelGGL((layer_norm_bwd_rows_kernel<T, TR, decltype(c)::value>), dim3((unsigned)parts),
+                         dim3(std::max(TR, 256)), 0, st, static_cast<const T*>(dy), static_cast<const T*>(x), (long)ldx,
+                         weight, (int)(wdtype == CCE_DTYPE_F32), mean, rstd, (long)N, (int)D, static_cast<T*>(dx),
+                         params ? L.dw : nullptr, L.db);
+    });
     HIP_TRY(hipGetLastError());
     if (!in_registers && dx && N > 0) {
       hipLaunchKernelGGL((layer_norm_dx_kernel<T, W>), dim3((unsigned)N), dim3(256), 0, st, static_cast<const T*>(dy),
@@ -418,13 +487,13 @@ int norm_backward(const void* dy, const void* x, int dtype, int64_t ldx, const v
     }
     if (!params) return CCE_OK;
     if (!in_registers) {
-      hipLaunchKernelGGL(layer_norm_parts_kernel<T>, dim3((unsigned)ceil_div(D, 256), (unsigned)L.parts), dim3(256), 0,
+      hipLaunchKernelGGL(layer_norm_parts_kernel<T>, dim3((unsigned)ceil_div(D, 256), (unsigned)parts), dim3(256), 0,
                          st, static_cast<const T*>(dy), static_cast<const T*>(x), (long)ldx, mean, rstd, (long)N, (int)D,
-                         ceil_div(N, (long)L.parts), L.dw, L.db);
+                         ceil_div(N, parts), L.dw, L.db);
       HIP_TRY(hipGetLastError());
     }
     hipLaunchKernelGGL(layer_norm_join_kernel<W>, dim3((unsigned)ceil_div(D, 16), 2), dim3(256), 0, st, L.dw, L.db,
-                       L.parts, (int)D, static_cast<W*>(dw), static_cast<W*>(db));
+                       (int)parts, (int)D, static_cast<W*>(dw), static_cast<W*>(db));
     HIP_TRY(hipGetLastError());
     return CCE_OK;
   });
