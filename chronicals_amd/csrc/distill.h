@@ -31,6 +31,7 @@ struct Teacher {
   float kd;     // kd T^2, the loss's factor
   float kdg;    // kd T, the gradient's
   float ce;
+  int squares;  // T = 2^squares for 1 and 2: exp(x) is exp(x / T) squared so often; 0: T is another
 };
 
 __device__ inline float load_teacher(const Teacher& a, long i) {
@@ -117,15 +118,30 @@ struct KdSums {
     if constexpr (DU) s1 *= fast_exp2((m - mn) * kLog2e);
     m = mn;
   }
+  // SQ: Teacher::squares
+  template <int SQ>
   __device__ inline void add(float x, float scale) {
-    st += fast_exp2((x - m) * scale);
-    if constexpr (DU) s1 += fast_exp2((x - m) * kLog2e);
+    const float e = fast_exp2((x - m) * scale);
+    st += e;
+    if constexpr (DU) {
+      if constexpr (SQ == 0)
+        s1 += fast_exp2((x - m) * kLog2e);
+      else if constexpr (SQ == 1)
+        s1 = __builtin_fmaf(e, e, s1);
+      else
+        s1 = __builtin_fmaf(e * e, e * e, s1);
+    }
   }
   __device__ inline void merge(float m2, float st2, float s12, float scale) {
     const float mn = fmaxf(m, m2);
     rescale(mn, scale);
     st += st2 * fast_exp2((m2 - mn) * scale);
     if constexpr (DU) s1 += s12 * fast_exp2((m2 - mn) * kLog2e);
+  }
+  __device__ inline void merge_wave(float scale) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1)
+      merge(__shfl_xor(m, o), __shfl_xor(st, o), DU ? __shfl_xor(s1, o) : 0.f, scale);
   }
 };
 
@@ -148,7 +164,7 @@ __global__ __launch_bounds__(256) void kd_stream_kernel(const T* __restrict__ X,
   KdSums<DU> k;
   auto add1 = [&](float x) {
     k.rescale(fmaxf(k.m, x), scale);
-    k.add(x, scale);
+    k.template add<0>(x, scale);
   };
   if (tid < sp.head) add1(elem_to_f32(row[tid]));
   if (tid < c1 - c0 - sp.tail_start) add1(elem_to_f32(row[sp.tail_start + tid]));
@@ -161,12 +177,18 @@ __global__ __launch_bounds__(256) void kd_stream_kernel(const T* __restrict__ X,
       mx = fmaxf(mx, x[e]);
     }
     k.rescale(mx, scale);
+    auto all = [&](auto SQ) {
 #pragma unroll
-    for (int e = 0; e < RowSplit<T>::E; ++e) k.add(x[e], scale);
+      for (int e = 0; e < RowSplit<T>::E; ++e) k.template add<decltype(SQ)::value>(x[e], scale);
+    };
+    if (!DU || a.squares == 0)
+      all(std::integral_constant<int, 0>{});
+    else if (a.squares == 1)
+      all(std::integral_constant<int, 1>{});
+    else
+      all(std::integral_constant<int, 2>{});
   });
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1)
-    k.merge(__shfl_xor(k.m, o), __shfl_xor(k.st, o), DU ? __shfl_xor(k.s1, o) : 0.f, scale);
+  k.merge_wave(scale);
   if ((tid & 63) == 0) {
     red[tid >> 6][0] = k.m;
     red[tid >> 6][1] = k.st;
@@ -200,10 +222,11 @@ __global__ __launch_bounds__(256) void kd_loss_kernel(const T* __restrict__ X, l
   }
   const float scale = kLog2e * a.inv_t;
   KdSums<DU> k;
-  for (int s = 0; s < S; ++s) {
+  for (int s = tid & 63; s < S; s += 64) {
     const float4 p = part[n * S + s];
     k.merge(p.x, p.y, p.z, scale);
   }
+  k.merge_wave(scale);
   const float s1 = DU ? k.s1 : k.st;  // T == 1, or not used
   float q, lq;
   load_entries(a, n, V, e, col, q, lq);
@@ -320,6 +343,7 @@ int check_teacher(const cce_teacher* t, long N, const void* labels, int64_t igno
   a.kd = t->distill_weight * t->temperature * t->temperature;
   a.kdg = t->distill_weight * t->temperature;
   a.ce = t->ce_weight;
+  a.squares = t->temperature == 2.f ? 1 : t->temperature == 4.f ? 2 : 0;
   return CCE_OK;
 }
 
@@ -334,7 +358,7 @@ int softmaxes_of(const Teacher& a) {
 // Workgroups per row: enough for the card's CUs where there are few rows, with at
 // least 4096 columns each.
 int kd_splits(long N, long V) {
-  const long s = std::min(ceil_div(1024, std::max<long>(N, 1)), V / 4096);
+  const long s = std::min(ceil_div(4096, std::max<long>(N, 1)), V / 4096);
   return (int)std::max<long>(s, 1);
 }
 
