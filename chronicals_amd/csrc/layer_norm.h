@@ -384,9 +384,12 @@ constexpr long kNormGroups = 1024;
 // workgroup per row, 8192 x 4096: 69, 53, 51, and of 1024 threads, 2048 x 16384:
 // 60, 78, 78).
 constexpr long kNormParts = 768;
-long norm_parts(long N, int threads) {
+long most_norm_parts(long N, long D) {  // and no more than 128 MiB of them
+  return std::max<long>(1, std::min({N, kNormParts, (1L << 24) / D}));
+}
+long norm_parts(long N, long D, int threads) {
   const long parts = threads == 64 ? std::min(std::max(N / 32, 256L), kNormParts) : threads == 256 ? 512 : 256;
-  return std::max<long>(1, std::min(parts, threads == 64 ? ceil_div(N, 4) : N));
+  return std::max<long>(1, std::min({parts, threads == 64 ? ceil_div(N, 4) : N, most_norm_parts(N, D)}));
 }
 
 struct NormLayout {
@@ -397,7 +400,7 @@ struct NormLayout {
 NormLayout norm_layout(void* ws, long N, long D) {
   Carver c(ws);
   NormLayout L;
-  const size_t parts = (size_t)std::max<long>(1, std::min(N, kNormParts));
+  const size_t parts = (size_t)most_norm_parts(N, D);
   L.dw = c.take<float>(parts * D);
   L.db = c.take<float>(parts * D);
   L.bytes = align_up(c.off, 256);
@@ -436,7 +439,7 @@ bool norm_shape(long D, F&& f) {
 
 // The longest rows that stay in registers: 1024 threads with four chunks each, in
 // the backward with 16 elements each.  Past that it spills: 1024 x 20000 bf16 175
-// us, by the kernels for longer rows 134 (the forward 29, by those 100).
+// us, by the kernels for longer rows 134 to 152 (the forward 36, by those 100).
 template <typename T>
 constexpr int kNormFwdD = 1024 * 4 * 16 / (int)sizeof(T);
 constexpr int kNormBwdD = 1024 * 16;
@@ -469,10 +472,10 @@ int norm_backward(const void* dy, const void* x, int dtype, int64_t ldx, const v
     typedef decltype(t) T;
     typedef decltype(w) W;
     const bool params = dw || db;
-    long parts = norm_parts(N, 256);
+    long parts = norm_parts(N, D, 256);
     const bool in_registers = norm_shape<16 / sizeof(T), kNormBwdD>(D, [&](auto tr, auto c) {
       constexpr int TR = decltype(tr)::value;
-      parts = norm_parts(N, TR);
+      parts = norm_parts(N, D, TR);
       hipLaunchKernelGGL((layer_norm_bwd_rows_kernel<T, TR, decltype(c)::value>), dim3((unsigned)parts),
                          dim3(std::max(TR, 256)), 0, st, static_cast<const T*>(dy), static_cast<const T*>(x), (long)ldx,
                          weight, (int)(wdtype == CCE_DTYPE_F32), mean, rstd, (long)N, (int)D, static_cast<T*>(dx),

@@ -242,6 +242,9 @@ def test_c_workspaces(lib):
     kd = size(lib.cce_distill_backward_workspace_bytes, 4096, 896, 151936, 64, 8192, 1, 0, 1, 0)
     assert 4096 * 65 * 8 <= kd - ce <= 4096 * 65 * 8 + 1024
     assert size(lib.cce_layer_norm_backward_workspace_bytes, 0, 64) > 0
+    # parts of the parameters' gradients: little next to long rows, bounded for the longest
+    assert size(lib.cce_layer_norm_backward_workspace_bytes, 1 << 20, 1 << 20) <= (128 << 20) + 1024
+    assert size(lib.cce_layer_norm_backward_workspace_bytes, 1 << 20, 4096) == 768 * 4096 * 8
     # the splits' candidates where there are few rows, nothing else
     assert size(lib.cce_top_logits_workspace_bytes, 4096, 151936, 64) == 0
     assert 0 < size(lib.cce_top_logits_workspace_bytes, 3, 151936, 64) <= 3 * 2048 * 8

@@ -389,6 +389,50 @@ def test_captured_and_replayed(gpu):
         assert all(torch.equal(a, b) for a, b in zip(want, got)), turn
 
 
+def test_grad_modes(gpu):
+    d = entry_points()
+    g = torch.Generator().manual_seed(22)
+    x = torch.randn(6, 500, generator=g).to(gpu).requires_grad_(True)
+    h, w = (v.to(gpu).requires_grad_(True) for v in head(g, 6, 64, 500))
+    t, index = (v.to(gpu) for v in teacher(g, 6, 500, 5))
+    for f, leaf in ((lambda: d.distillation_loss(x, t, index), x),
+                    (lambda: d.linear_distillation_loss(h, w, t, index), h)):
+        want = f()
+        with torch.inference_mode():
+            assert torch.equal(f(), want)
+        with torch.no_grad():
+            assert not f().requires_grad
+        (g1,) = torch.autograd.grad(want, leaf, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g1.float().sum(), leaf)
+    # a teacher that requires grad gets none
+    tt = t.clone().requires_grad_(True)
+    d.distillation_loss(x, tt, index).backward()
+    assert tt.grad is None and x.grad is not None
+    # twice through one graph
+    loss = d.linear_distillation_loss(h, w, t, index)
+    a = torch.autograd.grad(loss, [h, w], retain_graph=True)
+    b = torch.autograd.grad(loss, [h, w])
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_one_row_without_a_batch(gpu):
+    d = entry_points()
+    g = torch.Generator().manual_seed(23)
+    x = torch.randn(1, 700, generator=g)
+    t, index = teacher(g, 1, 700, 6)
+    xd = x[0].to(gpu).requires_grad_(True)
+    loss = d.distillation_loss(xd, t[0].to(gpu), index[0].to(gpu), torch.tensor(3, device=gpu), reduction="none",
+                               ce_weight=0.5)
+    rows, grad, _, mag_rows, mag = reference(x, t, index, torch.tensor([3]), ce=0.5)
+    close(loss, rows[0], 2 * EXP_ERR * mag_rows[0])
+    (dx,) = torch.autograd.grad(loss, xd)
+    close(dx, grad[0], 2.0 ** -24 * grad[0].abs() + 2 * EXP_ERR * mag[0])
+    h, w = head(g, 1, 64, 700)
+    out = d.linear_distillation_loss(h[0].to(gpu), w.to(gpu), t[0].to(gpu), index[0].to(gpu), reduction="none")
+    assert out.shape == ()
+
+
 def test_distillation_step(gpu):
     """A step as it is trained: a teacher's logits kept as its top ones, the student's final norm, the head and both
     losses; gradients of the norm's input and parameters and of the head against 64-bit autograd."""

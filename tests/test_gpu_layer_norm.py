@@ -63,6 +63,13 @@ def test_sizes_and_types(gpu, N, D, dtype, wdtype):
     check(gpu, x, w, b)
 
 
+def test_long_rows(gpu):
+    """Longer than the registers hold, with fewer parts of the parameters' gradients."""
+    g = torch.Generator().manual_seed(40)
+    x = torch.randn(90, 300001, generator=g).bfloat16()
+    check(gpu, x, (1 + 0.3 * torch.randn(300001, generator=g)).bfloat16(), None)
+
+
 @pytest.mark.parametrize("D", [96, 1001, 4096])
 def test_without_parameters(gpu, D):
     g = torch.Generator().manual_seed(D)
@@ -172,6 +179,20 @@ def test_same_bits_streams_and_graphs(gpu):
         got = [v.clone() for v in out]
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(got, step())), turn
+
+
+def test_grad_modes(gpu):
+    from chronicals_amd.kernels.layer_norm import layer_norm
+    x = torch.randn(5, 64, generator=torch.Generator().manual_seed(8)).to(gpu).requires_grad_(True)
+    want = layer_norm(x)
+    with torch.inference_mode():
+        assert torch.equal(layer_norm(x), want)
+    with torch.no_grad():
+        assert not layer_norm(x).requires_grad
+    assert not layer_norm(x.detach()).requires_grad
+    (dx,) = torch.autograd.grad(want.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dx.sum(), x)
 
 
 def test_module_is_torchs(gpu):
