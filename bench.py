@@ -20,6 +20,11 @@ events between a step's kernels add about 0.5% to a C2 step.
 forward + backward producing dlogits); its kernels are HBM-bound and the
 roofline is algorithmic bytes (N*V*2 read forward; N*V*2 read + N*V*2
 written backward) over the HIP-event launch time.
+
+``--workload distill`` measures a distillation step at the configuration's shape:
+layer norm of the hidden states, then the fused head with the loss towards a
+teacher's top 64 logits (kept by ``top_logits``) at temperature 2 and the labels'
+cross-entropy, forward and backward to hidden, the norm's parameters and the head.
 """
 from __future__ import annotations
 
@@ -251,10 +256,11 @@ def main() -> int:
                          "CutCrossEntropyLoss")
     ap.add_argument("--blas-reference", action="store_true",
                     help="only time torch.matmul (hipBLASLt) on the path's GEMM shapes and exit")
-    ap.add_argument("--workload", choices=("fused", "logits", "logits-fused"), default="fused",
+    ap.add_argument("--workload", choices=("fused", "logits", "logits-fused", "distill"), default="fused",
                     help="fused: linear-CE from hidden + lm_head (default); logits: CE over existing logits, "
                          "forward + autograd backward; logits-fused: loss and gradient in one kernel "
-                         "(liger_cross_entropy_forward with compute_grads)")
+                         "(liger_cross_entropy_forward with compute_grads); distill: layer norm, the head and "
+                         "distillation from a teacher's top logits beside the labels' loss")
     args = ap.parse_args()
 
     if args.gpus != 1 or int(os.environ.get("WORLD_SIZE", "1")) != 1:
@@ -267,6 +273,8 @@ def main() -> int:
 
     if args.workload in ("logits", "logits-fused"):
         return bench_logits(args)
+    if args.workload == "distill":
+        return bench_distill(args)
     if args.blas_reference:
         from tests.cce_common import CONFIGS
         blas_reference(CONFIGS[args.config], args.chunk)
@@ -552,6 +560,68 @@ def bench_logits(args) -> int:
     if not args.skip_cpu:
         out["cpu_baseline"] = cpu_baseline_logits(cfg, args.cpu_rows or 8192)
     print(json.dumps(out), flush=True)
+    return 0
+
+
+def bench_distill(args) -> int:
+    """A distillation step over hidden states [N, d] and a head [V, d] of the configuration's shape."""
+    import torch
+
+    from chronicals_amd.kernels.distillation import LinearDistillationLoss, top_logits
+    from chronicals_amd.kernels.layer_norm import LayerNorm
+    from tests.cce_common import CONFIGS
+
+    cfg = CONFIGS[args.config]
+    N, d, V, K, T = args.rows or cfg.N, cfg.d, cfg.V, 64, 2.0
+    dev = torch.device("cuda:0")
+    torch.cuda.set_device(dev)
+    g = torch.Generator(device=dev).manual_seed(0)
+
+    def randn(*shape):
+        return torch.randn(*shape, generator=g, device=dev)
+
+    x = randn(N, d).to(torch.bfloat16).requires_grad_(True)
+    w = (randn(V, d) * 0.02).to(torch.bfloat16).requires_grad_(not args.frozen_weight)
+    norm = LayerNorm(d, device=dev, dtype=torch.bfloat16)
+    lab = torch.randint(0, V, (N,), generator=g, device=dev)
+    lab[torch.rand(N, generator=g, device=dev) < cfg.ignore_frac] = -100
+    # a teacher's logits, 2048 rows at a time, of which its answer is kept
+    answers = [top_logits((randn(min(2048, N - a), V) * 2).to(torch.bfloat16), K) for a in range(0, N, 2048)]
+    values, indices = (torch.cat(v) for v in zip(*answers))
+    loss_fn = LinearDistillationLoss(chunk_size=args.chunk, temperature=T, distill_weight=0.5, ce_weight=0.5)
+    leaves = [x, norm.weight, norm.bias] + ([] if args.frozen_weight else [w])
+
+    def step():
+        for v in leaves:
+            v.grad = None
+        loss = loss_fn(norm(x), w, values, indices, lab)
+        loss.backward()
+        return loss
+
+    for _ in range(args.warmup):
+        step()
+    ms, step_ms, loss = timed_steps(step, args.steps)
+    flops = (4.0 if args.frozen_weight else 6.0) * N * V * d
+    print(json.dumps({
+        "metric": f"distillation step tokens/s, {cfg.name} N={N} d={d} V={V}, teacher's top {K}",
+        "value": N / (ms * 1e-3),
+        "unit": "tokens/s",
+        "n_gpus": 1,
+        "steps": args.steps,
+        "warmup": args.warmup,
+        "ms_per_step": ms,
+        "step_ms": {"median": statistics.median(step_ms)},
+        "higher_is_better": True,
+        "scaling": "weak",
+        "vs_baseline": None,
+        "dtype": "bf16",
+        "data": f"synthetic (seeded N(0,1) hidden, uniform labels, {100 * cfg.ignore_frac:g}% ignore_index, a teacher "
+                f"of N(0,4) logits)",
+        "config": {"workload": f"layer norm + fused head with distillation (T={T:g}, weight 0.5) and cross-entropy "
+                               f"(0.5), fwd+bwd", "N": N, "d": d, "V": V, "K": K, "frozen_weight": args.frozen_weight},
+        "tflops_credited": flops / (ms * 1e-3) / 1e12,
+        "loss": float(loss.item()),
+    }), flush=True)
     return 0
 
 
