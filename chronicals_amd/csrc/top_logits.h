@@ -71,11 +71,46 @@ struct TopList {
   int* count;
 };
 
+// The first `need` of the m keys that equal tau, by position, into list.c[at..]
+// (at least so many are there).  Eight neighbouring keys per thread at a time.
+template <typename F>
+__device__ void take_equal(F&& key, int m, uint32_t tau, int need, int at, const TopList& list) {
+  __shared__ int wave_count[4];
+  const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
+  int done = 0;
+  for (int i0 = 0; i0 < m && done < need; i0 += 256 * 8) {
+    unsigned eq = 0;
+    for (int e = 0; e < 8; ++e) {
+      const int i = i0 + tid * 8 + e;
+      if (i < m && key(i) == tau) eq |= 1u << e;
+    }
+    int upto = __popc(eq);  // an inclusive scan over the wave
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(upto, o);
+      if (l >= o) upto += v;
+    }
+    __syncthreads();
+    if (l == 63) wave_count[w] = upto;
+    __syncthreads();
+    int p = done + upto - __popc(eq);
+    for (int v = 0; v < 4; ++v) {
+      if (v < w) p += wave_count[v];
+      done += wave_count[v];
+    }
+    for (int e = 0; e < 8; ++e)
+      if (eq >> e & 1) {
+        if (p < need) list.c[at + p] = candidate(tau, i0 + tid * 8 + e);
+        ++p;
+      }
+  }
+  __syncthreads();
+}
+
 // The k largest of m keys into `list`, in no order.
 template <int BITS, typename F>
 __device__ void top_exact(F&& key, int m, int k, uint32_t* hist, const TopList& list) {
-  __shared__ int wave_count[4];
-  const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
+  const int tid = threadIdx.x;
   uint32_t tau;
   const int equal = kth_key<BITS>(key, m, k, hist, tau);
   if (tid == 0) *list.count = 0;
@@ -84,23 +119,7 @@ __device__ void top_exact(F&& key, int m, int k, uint32_t* hist, const TopList& 
     const uint32_t v = key(i);
     if (v > tau) list.c[atomicAdd(list.count, 1)] = candidate(v, i);
   }
-  // those equal to tau in order of their positions, 256 at a time
-  int done = 0;
-  for (int i0 = 0; i0 < m && done < equal; i0 += 256) {
-    const int i = i0 + tid;
-    const bool eq = i < m && key(i) == tau;
-    const uint64_t mine = __ballot(eq);
-    __syncthreads();
-    if (l == 0) wave_count[w] = __popcll(mine);
-    __syncthreads();
-    int p = done + __popcll(mine & ((1ull << l) - 1));
-    for (int v = 0; v < 4; ++v) {
-      if (v < w) p += wave_count[v];
-      done += wave_count[v];
-    }
-    if (eq && p < equal) list.c[k - equal + p] = candidate(tau, i);
-  }
-  __syncthreads();
+  take_equal(key, m, tau, equal, k - equal, list);
   if (tid == 0) *list.count = k;
   __syncthreads();
 }
@@ -171,14 +190,17 @@ constexpr int kTopCandidates = 2048;
 // so at least k elements reach the k-th largest of these maxima, tau.  Pass 2
 // reads the groups that reach it again (about k of them, from the caches) and
 // collects their elements from tau on: for values in no particular order about
-// k more or less, 66 to 300 for k = 64 to 256.  A row with more than
-// kTopCandidates there (long ties), or with fewer chunks than k, goes by
-// top_exact, whose passes over the row are three to five.
+// k more or less, 66 to 300 for k = 64 to 256.  With more than kTopCandidates there
+// (a mask's value fills the row up to k), the elements above tau are collected
+// alone and the first ones that equal it added.  What overflows then too, or has
+// fewer chunks than k, goes by top_exact, whose passes over the row are three to
+// five.
 //
 // Bound by HBM: k = 64 of 2048 x 151936 bf16 takes 128 us, 4.9 TB/s (a large copy
 // reaches 4.9); by top_exact alone it took 1550 us.  Of that 144 -> 136 us came
 // from non-temporal loads in pass 1 and 136 -> 128 from eight workgroups per CU
-// instead of seven.
+// instead of seven.  With all but 20 columns of a row at a mask's value 390 us, and
+// by top_exact after the overflow 2510.
 template <typename T>
 __device__ void top_of_row(const T* row, int V, int k, uint32_t* hist, uint16_t* groups, const TopList& list) {
   constexpr int U = 4, NP = GroupMax<T>::kParts;
@@ -199,73 +221,93 @@ __device__ void top_of_row(const T* row, int V, int k, uint32_t* hist, uint16_t*
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (c + u * 256 < sp.chunks) g[u].add(body[c + u * 256]);
-    // tau: the largest integer that k groups reach, bit by bit from the top.  Of
-    // fp32's the lowest 12 bits stay 0: what lies in between is hardly ever a
-    // candidate more, and each bit costs a barrier
+    // tau: the largest integer that k groups reach, bit by bit from the top
     uint32_t tau = 0;
-    for (int bit = GroupMax<T>::kBits - 1; bit >= (GroupMax<T>::kBits == 32 ? 12 : 0); --bit) {
-      const uint32_t next = tau | 1u << bit;
-      int n = 0;
+    auto search = [&](int high, int low) {
+      for (int bit = high; bit >= low; --bit) {
+        const uint32_t next = tau | 1u << bit;
+        int n = 0;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int i = 0; i < NP; ++i) n += __popcll(__ballot(g[u].part(i) >= next));
-      int* const at = counts[bit & 1];
-      if (l == 0) at[w] = n;
+          for (int i = 0; i < NP; ++i) n += __popcll(__ballot(g[u].part(i) >= next));
+        int* const at = counts[bit & 1];
+        if (l == 0) at[w] = n;
+        __syncthreads();
+        if (at[0] + at[1] + at[2] + at[3] >= k) tau = next;
+      }
       __syncthreads();
-      if (at[0] + at[1] + at[2] + at[3] >= k) tau = next;
-    }
-    // the lowest integer of the same key: NaN are equal, and so are zeros
-    constexpr uint32_t kInf = GroupMax<T>::kInf + GroupMax<T>::kZero;
-    const uint32_t from = key_of(GroupMax<T>::value(tau));
-    tau = tau > kInf ? kInf + 1 : tau == GroupMax<T>::kZero ? tau - 1 : tau;
-    if (tid == 0) *list.count = ngroups = 0;
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      bool reach = false;
-#pragma unroll
-      for (int i = 0; i < NP; ++i) reach = reach || g[u].part(i) >= tau;
-      if (reach) groups[atomicAdd(&ngroups, 1)] = (uint16_t)(u * 256 + tid);
-    }
-    __syncthreads();
-    auto take = [&](T x, int at) {
-      const uint32_t key = key_of(x);
-      if (key < from) return;
-      const int p = atomicAdd(list.count, 1);
-      if (p < kTopCandidates) list.c[p] = candidate(key, at);
     };
-    const int rounds = (sp.chunks + U * 256 - 1) / (U * 256), items = ngroups * rounds;
-    for (int i0 = 0; i0 < items; i0 += U * 256) {
-      u32x4 raw[U];
-      int at[U];
+    const int rounds = (sp.chunks + U * 256 - 1) / (U * 256);
+    // The elements of keys from `from` on (above it: with `above`) into the list;
+    // whether they fit.
+    auto collect = [&](uint32_t from, bool above) {
+      // the lowest integer of the same key: NaN are equal, and so are zeros
+      constexpr uint32_t kInf = GroupMax<T>::kInf + GroupMax<T>::kZero;
+      const uint32_t reach = tau > kInf ? kInf + 1 : tau == GroupMax<T>::kZero ? tau - 1 : tau;
+      if (tid == 0) *list.count = ngroups = 0;
+      __syncthreads();
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int i = i0 + u * 256 + tid;
-        at[u] = -1;
-        if (i < items) {
-          // neighbouring threads take neighbouring groups of one round
-          const int chunk = (i / ngroups) * (U * 256) + groups[i % ngroups];
-          if (chunk < sp.chunks) {
-            at[u] = sp.head + chunk * RowSplit<T>::E;
-            raw[u] = body[chunk];
+        bool some = false;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) some = some || g[u].part(i) >= reach;
+        if (some) groups[atomicAdd(&ngroups, 1)] = (uint16_t)(u * 256 + tid);
+      }
+      __syncthreads();
+      auto take = [&](T x, int at) {
+        const uint32_t key = key_of(x);
+        if (key < from || (above && key == from)) return;
+        const int p = atomicAdd(list.count, 1);
+        if (p < kTopCandidates) list.c[p] = candidate(key, at);
+      };
+      const int items = ngroups * rounds;
+      for (int i0 = 0; i0 < items; i0 += U * 256) {
+        u32x4 raw[U];
+        int at[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int i = i0 + u * 256 + tid;
+          at[u] = -1;
+          if (i < items) {
+            // neighbouring threads take neighbouring groups of one round
+            const int chunk = (i / ngroups) * (U * 256) + groups[i % ngroups];
+            if (chunk < sp.chunks) {
+              at[u] = sp.head + chunk * RowSplit<T>::E;
+              raw[u] = body[chunk];
+            }
           }
         }
-      }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (at[u] < 0) continue;
-        const T* v = reinterpret_cast<const T*>(&raw[u]);
+        for (int u = 0; u < U; ++u) {
+          if (at[u] < 0) continue;
+          const T* v = reinterpret_cast<const T*>(&raw[u]);
 #pragma unroll
-        for (int e = 0; e < RowSplit<T>::E; ++e) take(v[e], at[u] + e);
+          for (int e = 0; e < RowSplit<T>::E; ++e) take(v[e], at[u] + e);
+        }
       }
+      if (tid < sp.head) take(row[tid], tid);
+      if (tid < V - sp.tail_start) take(row[sp.tail_start + tid], sp.tail_start + tid);
+      __syncthreads();
+      const int n = *list.count;
+      __syncthreads();
+      return n;
+    };
+    // Of fp32's bits the lowest 12 stay 0 at first: what lies in between is hardly
+    // ever a candidate more, and each bit costs a barrier
+    constexpr int kBits = GroupMax<T>::kBits, kFirst = kBits == 32 ? 12 : 0;
+    search(kBits - 1, kFirst);
+    if (collect(key_of(GroupMax<T>::value(tau)), false) <= kTopCandidates) return;
+    search(kFirst - 1, 0);
+    const uint32_t from = key_of(GroupMax<T>::value(tau));
+    const int above = collect(from, true);
+    if (above <= kTopCandidates) {
+      if (above >= k) return;
+      take_equal([&](int i) { return key_of(row[i]); }, V, from, k - above, above, list);
+      if (tid == 0) *list.count = k;
+      __syncthreads();
+      return;
     }
-    if (tid < sp.head) take(row[tid], tid);
-    if (tid < V - sp.tail_start) take(row[sp.tail_start + tid], sp.tail_start + tid);
-    __syncthreads();
-    const bool fits = *list.count <= kTopCandidates;
-    __syncthreads();
-    if (fits) return;
   }
   top_exact<kKeyBits<T>>([&](int i) { return key_of(row[i]); }, V, k, hist, list);
 }

@@ -75,6 +75,23 @@ def test_largest_in_one_place(gpu):
             check(gpu, x.to(dt), k)
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_masked_rows(gpu, dtype):
+    """Fewer values than k beside a mask's value, which fills the rest by the lowest columns; the mask's value may be
+    -inf, the type's lowest, zero of either sign or any other, and stand late in the row."""
+    dt = DTYPES[dtype]
+    g = torch.Generator().manual_seed(4)
+    V = 60013
+    for mask in (-math.inf, torch.finfo(dt).min, 0.0, -0.0, 1.25, -7.3, math.inf, math.nan):
+        x = torch.full((6, V), mask)
+        for n, kept in enumerate((1, 5, 40, 63, 300)):
+            at = torch.randperm(V, generator=g)[:kept]
+            x[n, at] = torch.randn(kept, generator=g) + (20 if n % 2 else 0)
+        x[5, :50000] = -2e4
+        for k in (1, 64, 256):
+            check(gpu, x.to(dt), k)
+
+
 def test_strided_rows_and_shapes(gpu):
     g = torch.Generator().manual_seed(2)
     big = torch.randn(6, 5007, generator=g).bfloat16()
