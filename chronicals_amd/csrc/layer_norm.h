@@ -437,19 +437,18 @@ bool norm_shape(long D, F&& f) {
   return true;
 }
 
-// The longest rows that stay in registers: 1024 threads with four chunks each, in
-// the backward with 16 elements each.  Past that it spills: 1024 x 20000 bf16 175
-// us, by the kernels for longer rows 134 to 152 (the forward 36, by those 100).
-template <typename T>
-constexpr int kNormFwdD = 1024 * 4 * 16 / (int)sizeof(T);
-constexpr int kNormBwdD = 1024 * 16;
+// The longest rows that stay in registers: 16 elements in each of 1024 threads.
+// Past that the kernels spill: with 18 registers in memory the forward of 1024 x
+// 20000 bf16 took 36 us, with 370 the backward 175, and by the kernels for longer
+// rows they take 100 and 134 to 152.
+constexpr int kNormRegD = 1024 * 16;
 
 int norm_forward(const void* x, int dtype, int64_t ldx, const void* weight, const void* bias, int wdtype, int64_t N,
                  int64_t D, float eps, void* y, float* mean, float* rstd, hipStream_t st) {
   return norm_types(dtype, wdtype, [&](auto t, auto w) {
     typedef decltype(t) T;
     typedef decltype(w) W;
-    const bool in_registers = norm_shape<16 / sizeof(T), kNormFwdD<T>>(D, [&](auto tr, auto c) {
+    const bool in_registers = norm_shape<16 / sizeof(T), kNormRegD>(D, [&](auto tr, auto c) {
       constexpr int TR = decltype(tr)::value, kRows = TR < 256 ? 256 / TR : 1;
       const unsigned grid = (unsigned)std::min<long>(ceil_div(N, kRows), kNormGroups);
       hipLaunchKernelGGL((layer_norm_fwd_rows_kernel<T, TR, decltype(c)::value>), dim3(grid), dim3(std::max(TR, 256)), 0,
@@ -473,7 +472,7 @@ int norm_backward(const void* dy, const void* x, int dtype, int64_t ldx, const v
     typedef decltype(w) W;
     const bool params = dw || db;
     long parts = norm_parts(N, D, 256);
-    const bool in_registers = norm_shape<16 / sizeof(T), kNormBwdD>(D, [&](auto tr, auto c) {
+    const bool in_registers = norm_shape<16 / sizeof(T), kNormRegD>(D, [&](auto tr, auto c) {
       constexpr int TR = decltype(tr)::value;
       parts = norm_parts(N, D, TR);
       hipLaunchKernelGGL((layer_norm_bwd_rows_kernel<T, TR, decltype(c)::value>), dim3((unsigned)parts),
