@@ -158,6 +158,7 @@ struct GroupMax {
       v = __builtin_elementwise_max(v, p);
     }
   }
+  __device__ inline void merge(const GroupMax& o) { v = __builtin_elementwise_max(v, o.v); }
   __device__ inline uint32_t part(int i) const { return v[i]; }
   static __device__ inline T value(uint32_t p) {
     const short b = (short)(p - kZero);
@@ -173,6 +174,7 @@ struct GroupMax<float> {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v = max(v, (raw[i] ^ (uint32_t)((int)raw[i] >> 31) >> 1) + kZero);
   }
+  __device__ inline void merge(const GroupMax& o) { v = max(v, o.v); }
   __device__ inline uint32_t part(int) const { return v; }
   static __device__ inline float value(uint32_t p) {
     const uint32_t b = p - kZero;
@@ -180,27 +182,29 @@ struct GroupMax<float> {
   }
 };
 
-constexpr int kTopCandidates = 2048;
+constexpr int kTopCandidates = 2048, kTopGroups = 1024;
 
 // The k largest of row[0, V) into `list` (at least those k, at most
 // kTopCandidates), by one pass over HBM and a second look at a few of its lines.
 //
-// Pass 1 keeps the largest of each of 1024 or 2048 groups: a thread's chunks at
-// each place of its four loads in flight.  Each group's largest is an element,
-// so at least k elements reach the k-th largest of these maxima, tau.  Pass 2
-// reads the groups that reach it again (about k of them, from the caches) and
-// collects their elements from tau on: for values in no particular order about
-// k more or less, 66 to 300 for k = 64 to 256.  With more than kTopCandidates there
+// Pass 1 keeps the largest of groups of chunks: a thread's chunks at each place of
+// its four loads in flight, by their round modulo four.  Four such groups together
+// (1024 or, of the 16-bit types, 2048 fours) have a largest element each, so at
+// least k elements reach the k-th largest of these, tau.  Pass 2 reads the groups
+// that reach tau again and collects their elements from it on: for values in no
+// particular order about k groups and k elements, 66 to 300 for k = 64 to 256.
+// A chunk of 16 bytes brings a line of 128 from the memory-side cache: with the
+// four groups as one that was 40% of the row again, and 128 us for 107.  With more than kTopCandidates there
 // (a mask's value fills the row up to k), the elements above tau are collected
 // alone and the first ones that equal it added.  What overflows then too, or has
 // fewer chunks than k, goes by top_exact, whose passes over the row are three to
 // five.
 //
-// Bound by HBM: k = 64 of 2048 x 151936 bf16 takes 128 us, 4.9 TB/s (a large copy
-// reaches 4.9); by top_exact alone it took 1550 us.  Of that 144 -> 136 us came
-// from non-temporal loads in pass 1 and 136 -> 128 from eight workgroups per CU
-// instead of seven.  With all but 20 columns of a row at a mask's value 390 us, and
-// by top_exact after the overflow 2510.
+// Bound by HBM: k = 64 of 2048 x 151936 bf16 takes 107 us, 5.8 TB/s of the rows (a
+// large copy reaches 4.9, half of it reads); by top_exact alone it took 1550 us.
+// 144 -> 136 us came from non-temporal loads in pass 1 and 136 -> 128 from eight
+// workgroups per CU instead of seven.  With all but 20 columns of a row at a mask's
+// value 390 us, and by top_exact after the overflow 2510.
 template <typename T>
 __device__ void top_of_row(const T* row, int V, int k, uint32_t* hist, uint16_t* groups, const TopList& list) {
   constexpr int U = 4, NP = GroupMax<T>::kParts;
@@ -209,18 +213,31 @@ __device__ void top_of_row(const T* row, int V, int k, uint32_t* hist, uint16_t*
   const RowSplit<T> sp(row, V);
   if (sp.chunks >= k) {
     const u32x4* const body = reinterpret_cast<const u32x4*>(row + sp.head);
-    GroupMax<T> g[U];
-    int c = tid;
-    for (; c + (U - 1) * 256 < sp.chunks; c += U * 256) {
-      u32x4 raw[U];
+    constexpr int R = 4;
+    GroupMax<T> part[R][U], g[U];
+    for (int c0 = tid; c0 < sp.chunks; c0 += R * U * 256) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) raw[u] = __builtin_nontemporal_load(body + c + u * 256);
+      for (int r = 0; r < R; ++r) {
+        const int c = c0 + r * U * 256;
+        if (c + (U - 1) * 256 < sp.chunks) {
+          u32x4 raw[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) g[u].add(raw[u]);
+          for (int u = 0; u < U; ++u) raw[u] = __builtin_nontemporal_load(body + c + u * 256);
+#pragma unroll
+          for (int u = 0; u < U; ++u) part[r][u].add(raw[u]);
+        } else {
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (c + u * 256 < sp.chunks) part[r][u].add(body[c + u * 256]);
+        }
+      }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (c + u * 256 < sp.chunks) g[u].add(body[c + u * 256]);
+    for (int u = 0; u < U; ++u) {
+      g[u] = part[0][u];
+#pragma unroll
+      for (int r = 1; r < R; ++r) g[u].merge(part[r][u]);
+    }
     // tau: the largest integer that k groups reach, bit by bit from the top
     uint32_t tau = 0;
     auto search = [&](int high, int low) {
@@ -238,7 +255,7 @@ __device__ void top_of_row(const T* row, int V, int k, uint32_t* hist, uint16_t*
       }
       __syncthreads();
     };
-    const int rounds = (sp.chunks + U * 256 - 1) / (U * 256);
+    const int rounds = (sp.chunks + R * U * 256 - 1) / (R * U * 256);  // of a group
     // The elements of keys from `from` on (above it: with `above`) into the list;
     // whether they fit.
     auto collect = [&](uint32_t from, bool above) {
@@ -248,12 +265,16 @@ __device__ void top_of_row(const T* row, int V, int k, uint32_t* hist, uint16_t*
       if (tid == 0) *list.count = ngroups = 0;
       __syncthreads();
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        bool some = false;
+      for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int i = 0; i < NP; ++i) some = some || g[u].part(i) >= reach;
-        if (some) groups[atomicAdd(&ngroups, 1)] = (uint16_t)(u * 256 + tid);
-      }
+        for (int u = 0; u < U; ++u) {
+          bool some = false;
+#pragma unroll
+          for (int i = 0; i < NP; ++i) some = some || part[r][u].part(i) >= reach;
+          if (!some) continue;
+          const int p = atomicAdd(&ngroups, 1);
+          if (p < kTopGroups) groups[p] = (uint16_t)((r * U + u) * 256 + tid);
+        }
       __syncthreads();
       auto take = [&](T x, int at) {
         const uint32_t key = key_of(x);
@@ -261,7 +282,9 @@ __device__ void top_of_row(const T* row, int V, int k, uint32_t* hist, uint16_t*
         const int p = atomicAdd(list.count, 1);
         if (p < kTopCandidates) list.c[p] = candidate(key, at);
       };
-      const int items = ngroups * rounds;
+      // with more groups than the list holds: every chunk
+      const bool listed = ngroups <= kTopGroups;
+      const int items = listed ? ngroups * rounds : sp.chunks;
       for (int i0 = 0; i0 < items; i0 += U * 256) {
         u32x4 raw[U];
         int at[U];
@@ -271,7 +294,7 @@ __device__ void top_of_row(const T* row, int V, int k, uint32_t* hist, uint16_t*
           at[u] = -1;
           if (i < items) {
             // neighbouring threads take neighbouring groups of one round
-            const int chunk = (i / ngroups) * (U * 256) + groups[i % ngroups];
+            const int chunk = listed ? (i / ngroups) * (R * U * 256) + groups[i % ngroups] : i;
             if (chunk < sp.chunks) {
               at[u] = sp.head + chunk * RowSplit<T>::E;
               raw[u] = body[chunk];
@@ -329,7 +352,7 @@ __global__ __launch_bounds__(256) void top_logits_kernel(const T* __restrict__ X
                                                          uint64_t* __restrict__ part) {
   __shared__ uint32_t hist[256];
   __shared__ uint64_t cands[kTopCandidates];
-  __shared__ uint16_t groups[1024];  // 16 bits: eight workgroups per CU fit with 20 KB each
+  __shared__ uint16_t groups[kTopGroups];  // 16 bits: eight workgroups per CU fit with 20 KB each
   __shared__ int count;
   const TopList list = {cands, &count};
   const long n = blockIdx.x / S;
