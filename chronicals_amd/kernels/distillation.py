@@ -21,7 +21,9 @@ so with ``ce_weight`` the labels' loss comes from the same passes.
   * An entry whose index is outside [0, V) (use -1 as padding) or whose logit is
     -inf takes no part, whatever else it holds; a row left without any has no
     distillation term.  Entries that share an index add up there.
-  * ``labels``: a row labelled ``ignore_index`` gives no loss and a zero gradient.
+  * ``labels``: a row labelled ``ignore_index`` gives no loss and a zero gradient,
+    whatever its logits hold; its hidden states have to be finite in the linear
+    form, whose products run over them with zero coefficients.
     A label outside [0, V) that is not ``ignore_index`` has no target logit.
     Without labels (``ce_weight`` is 0 then) a row counts if it has a usable entry.
   * 'mean' divides by the number of rows that count, at least 1; 'sum' adds them;

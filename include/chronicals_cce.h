@@ -305,7 +305,8 @@ int cce_distill_logits_backward(const float* grad_out, const void* logits, int l
                                 void* grad_logits, int64_t ld_grad, void* stream);
 
 /* Fused with the head's product, x = hidden . weight^T + bias, operands as
- * cce_forward's and cce_backward's.  The forward keeps for the backward
+ * cce_forward's and cce_backward's (the rows of hidden that do not count are
+ * finite: products run over them with zero coefficients).  The forward keeps for the backward
  * stats_out [N][2], entry_logits_out [N][entries + 1] and rows_out [N]; the
  * backward takes the same teacher, and no labels. */
 int cce_distill_forward_workspace_bytes(int64_t N, int64_t d, int64_t V, int reduction, size_t* bytes);
