@@ -2731,7 +2731,8 @@ struct SparseGrad {
   const void* args;
 };
 
-// G[m][col - v0] = val for the block's rows and the band's columns.
+// G[m][col - v0] = val for the block's rows and the band's columns: a launch of 5 us
+// per band (65 entries of 2048 or of 8192 rows), little more than its latency.
 __global__ __launch_bounds__(256) void sparse_grad_kernel(const int* __restrict__ col, const float* __restrict__ val,
                                                           int entries, int rows, const int* __restrict__ live,
                                                           int live_base, int v0, int vb, bf16_t* __restrict__ G,

