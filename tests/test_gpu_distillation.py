@@ -365,6 +365,67 @@ def test_another_stream(gpu):
     assert all(torch.equal(a, b) for a, b in zip(want, got))
 
 
+def test_two_streams_at_once(gpu):
+    """Calls that overlap on two streams share nothing."""
+    steps = [calls(gpu, s)[0] for s in (20, 21)]
+    want = [f() for f in steps]
+    streams = [torch.cuda.Stream() for _ in steps]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, (f, s) in enumerate(zip(steps, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(f())
+    torch.cuda.synchronize()
+    for w, runs in zip(want, got):
+        for r in runs:
+            assert all(torch.equal(a, b) for a, b in zip(w, r))
+
+
+def test_offsets_past_32_bits(gpu):
+    """Rows, and rows of the head's weight, that begin past 2^31 elements."""
+    d = entry_points()
+    g = torch.Generator().manual_seed(24)
+    N, V, K = 15000, 151936, 8
+    x = torch.zeros(N, V, dtype=torch.bfloat16, device=gpu)
+    last = torch.randn(2, V, generator=g).bfloat16()
+    x[-2:] = last.to(gpu)
+    t, index = teacher(g, 2, V, K)
+    tt, ii = torch.zeros(N, K), torch.full((N, K), -1)
+    tt[-2:], ii[-2:] = t, index
+    x.requires_grad_(True)
+    loss = d.distillation_loss(x, tt.to(gpu), ii.to(gpu), reduction="none")
+    rows, grad, _, mag_rows, mag = reference(last, t, index)
+    close(loss[-2:], rows, 2 * EXP_ERR * mag_rows)
+    (dx,) = torch.autograd.grad(loss.sum(), x)
+    close(dx[-2:], grad, 2.0 ** -8 * grad.abs() + 2 * EXP_ERR * mag)
+    assert not dx[:-2].any()
+    values, indices = d.top_logits(x.detach(), K)
+    top = torch.sort(last.float(), dim=1, descending=True, stable=True)
+    assert torch.equal(values[-2:].float().cpu(), top.values[:, :K]) and torch.equal(indices[-2:].cpu(), top.indices[:, :K])
+    del x, dx, loss, values, indices
+    N, dim, V = 3, 16384, 140000
+    h = (torch.randn(N, dim, generator=g) / 128).bfloat16().to(gpu).requires_grad_(True)
+    w = torch.empty(V, dim, dtype=torch.bfloat16, device=gpu).normal_(generator=torch.Generator(gpu).manual_seed(1))
+    t, index = teacher(g, N, V, K)
+    index[0, 0], index[1, 1] = V - 1, V - 2
+    loss = d.linear_distillation_loss(h, w, t.to(gpu), index.to(gpu), reduction="none")
+    (dh,) = torch.autograd.grad(loss.sum(), h)
+    logits = torch.cat([h.detach().double() @ w[a:a + 10000].double().t() for a in range(0, V, 10000)], 1).cpu()
+    rows, grad, _, mag_rows, mag = reference(logits, t, index)
+    # sixteen lanes, or the sixteen products of an MFMA step, share out the sum: 1024
+    # additions one after the other and a few more, each off by 2^-24 of the magnitudes
+    sums = [(h.detach().double().abs() @ w[a:a + 10000].double().abs().t()).max().item() for a in range(0, V, 10000)]
+    delta = 2.0 ** -24 * (16384 / 16 + 16) * max(sums)
+    close(loss, rows, 2 * EXP_ERR * mag_rows + 2 * delta)
+    want, scale = torch.zeros(N, dim).double(), torch.zeros(N, dim).double()
+    for a in range(0, V, 10000):
+        part = w[a:a + 10000].double().cpu()
+        want += grad[:, a:a + 10000] @ part
+        scale += mag[:, a:a + 10000] @ part.abs()
+    close(dh, want, 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2 * EXP_ERR + V * 2.0 ** -24) * scale)
+
+
 def test_captured_and_replayed(gpu):
     step, inputs = calls(gpu)
     other = calls(gpu, 21)[1]

@@ -181,6 +181,21 @@ def test_same_bits_streams_and_graphs(gpu):
         assert all(torch.equal(p, q) for p, q in zip(got, step())), turn
 
 
+def test_offsets_past_32_bits(gpu):
+    from chronicals_amd.kernels.layer_norm import layer_norm
+    N, D = 2_200_000, 1024
+    x = torch.zeros(N, D, dtype=torch.bfloat16, device=gpu)
+    x[-3:] = torch.randn(3, D, generator=torch.Generator().manual_seed(9)).bfloat16().to(gpu)
+    few = x[-3:].clone().requires_grad_(True)
+    y = layer_norm(few)
+    (want,) = torch.autograd.grad(y, few, few.detach())
+    x.requires_grad_(True)
+    z = layer_norm(x)
+    assert torch.equal(z[-3:], y) and not z[:-3].any()
+    (dx,) = torch.autograd.grad(z, x, x.detach())
+    assert torch.equal(dx[-3:], want)
+
+
 def test_grad_modes(gpu):
     from chronicals_amd.kernels.layer_norm import layer_norm
     x = torch.randn(5, 64, generator=torch.Generator().manual_seed(8)).to(gpu).requires_grad_(True)
