@@ -6,7 +6,9 @@
 // and the K + 1 columns written over it before the band's products read it.
 
 // rows[n]: -1 where row n does not count, else its label, or V without a target.
-// One wave per row.
+// One wave per row.  Only the order of the rows needs this ahead of the loss:
+// without one (a single row tile) kd_linear_loss_kernel does it, a launch less (64
+// rows, d 896, V 32000, forward and backward 119 -> 117 us).
 __global__ __launch_bounds__(256) void kd_rows_kernel(Teacher a, int N, int V, int* __restrict__ rows) {
   const int l = threadIdx.x & 63;
   const long n = blockIdx.x * 4L + (threadIdx.x >> 6);
@@ -35,14 +37,20 @@ template <bool DU>
 __global__ __launch_bounds__(256) void kd_linear_loss_kernel(
     const float* __restrict__ pm, const float* __restrict__ ps, const float* __restrict__ ps1, int splits, long ldp,
     const bf16_t* __restrict__ H, const bf16_t* __restrict__ W, const float* __restrict__ bias, int d, int V, Teacher a,
-    const int* __restrict__ rows, const int* __restrict__ idx, const int* __restrict__ live,
+    int* __restrict__ rows, int rows_known, const int* __restrict__ idx, const int* __restrict__ live,
     float2* __restrict__ stats, float* __restrict__ xk, float* __restrict__ rowloss, float* __restrict__ bsum,
     int* __restrict__ bcnt) {
   __shared__ Entries e;
   __shared__ float ex[kMaxEntries + 1];
   const int tid = threadIdx.x, l = tid & 63;
   const long i = blockIdx.x, n = idx ? idx[i] : i;
-  const int r = rows[n];
+  int r;
+  if (rows_known) {
+    r = rows[n];
+  } else {
+    r = row_counts(a, n, V, r) ? (r < 0 ? V : r) : -1;
+    if (tid == 0) rows[n] = r;
+  }
   if (r < 0) {
     if (tid == 0) {
       stats[n] = make_float2(0.f, 0.f);
@@ -193,10 +201,10 @@ int distill_forward_run(const bf16_t* H, const bf16_t* W, const float* bias, lon
                         const DistillLayout& L, hipStream_t st) {
   const FwdLayout& F = L.f;
   const bool dual = two_softmaxes(a);
-  hipLaunchKernelGGL(kd_rows_kernel, dim3((unsigned)ceil_div(N, 4)), dim3(256), 0, st, a, (int)N, (int)V, rows);
-  HIP_TRY(hipGetLastError());
   const int slots = (int)forward_slots(N, V, F.idx != nullptr);
   if (F.idx) {
+    hipLaunchKernelGGL(kd_rows_kernel, dim3((unsigned)ceil_div(N, 4)), dim3(256), 0, st, a, (int)N, (int)V, rows);
+    HIP_TRY(hipGetLastError());
     hipLaunchKernelGGL(compact_rows_kernel, dim3(1), dim3(1024), 0, st, rows, 0, (int)N, -1L, F.idx, F.live, slots,
                        (int)ceil_div(V, kBN), device_cus());
     HIP_TRY(hipGetLastError());
@@ -238,7 +246,7 @@ int distill_forward_run(const bf16_t* H, const bf16_t* W, const float* bias, lon
   float* const rowloss = reduction == CCE_REDUCTION_NONE ? loss_out : F.rowloss;
   auto* const loss = dual ? kd_linear_loss_kernel<true> : kd_linear_loss_kernel<false>;
   hipLaunchKernelGGL(loss, dim3((unsigned)N), dim3(256), 0, st, F.pm, F.ps, L.ps1, ep.splits, (long)N, H, W, bias,
-                     (int)d, (int)V, a, rows, F.idx, F.live, stats, xk, rowloss, L.bsum, L.bcnt);
+                     (int)d, (int)V, a, rows, F.idx != nullptr, F.idx, F.live, stats, xk, rowloss, L.bsum, L.bcnt);
   HIP_TRY(hipGetLastError());
   hipLaunchKernelGGL(fwd_finalize_kernel, dim3(1), dim3(1024), 0, st, L.bsum, L.bcnt, (int)N, reduction, loss_out,
                      n_valid);
