@@ -76,8 +76,8 @@ extern "C" {
 /* Library ABI version (CCE_ABI_VERSION).  No reference counterpart. */
 int cce_abi_version(void);
 
-/* Hex SHA-256 of the sources the library was compiled from (the kernel file
-   and this header; "unknown" for a build that did not pass it).  No reference
+/* Hex SHA-256 of the sources the library was compiled from (the kernel file with
+   its parts and this header; "unknown" for a build that did not pass it).  No reference
    counterpart: the Python loader compares it with the source tree and
    refuses a library built from other sources. */
 const char* cce_source_hash(void);

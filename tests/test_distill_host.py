@@ -226,6 +226,19 @@ def test_c_operands(lib):
     assert back(None, P, 0, 64, P, 0, P, P, 4, 64, P, P, P, P, 1 << 30, None) == bad
 
 
+def test_source_hash_follows_the_parts(tmp_path, monkeypatch):
+    from chronicals_amd import build
+    text = open(build.SRC).read()
+    for part in build.PARTS:
+        assert f'#include "{part.rsplit("/", 1)[1]}"' in text
+    base, torch_base = build.source_hash(), build.source_hash((build.TORCH_SRC, build.HEADER))
+    edited = tmp_path / "distill.h"
+    edited.write_text(open(build.PARTS[0]).read() + "// edit\n")
+    monkeypatch.setattr(build, "PARTS", (str(edited), *build.PARTS[1:]))
+    assert build.source_hash() != base
+    assert build.source_hash((build.TORCH_SRC, build.HEADER)) == torch_base
+
+
 def test_c_workspaces(lib):
     def size(fn, *args):
         out = ctypes.c_size_t(0)
