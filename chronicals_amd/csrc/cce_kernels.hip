@@ -411,9 +411,12 @@ __host__ __device__ inline float split_cost(int gl, int tn, int s, int ncu) {
 //
 // SM, the softmaxes that an epilogue computes: one of the logits, one at a
 // temperature (the launch's scale; as a parameter of the first kind too, it cost
-// the cross-entropy of 16384 x 896 x 151936 0.8%), or both.  With both the running maximum is kept in logits and starts at
-// kLogitFloor, whose products with either scale stay in range.
-constexpr int kOneSoftmax = 0, kAtTemperature = 1, kTwoSoftmaxes = 2;
+// the cross-entropy of 16384 x 896 x 151936 0.8%), or both.  With both the
+// running maximum is kept in logits and starts at kLogitFloor, whose products
+// with either scale stay in range.  A backward of kCrossEntropy has one softmax
+// and the label's one-hot term, and its G has no unit; the others have no such
+// term and a unit (BwdLayout's).
+constexpr int kOneSoftmax = 0, kAtTemperature = 1, kTwoSoftmaxes = 2, kCrossEntropy = 3;
 constexpr float kLogitFloor = -1e30f;
 
 template <int BN, bool HB, int SM = kOneSoftmax>
@@ -594,7 +597,7 @@ struct GradParams {
   long ldg;
   int v0;                // first vocabulary row of the band
   int tiles_n;           // column tiles in the band
-  float scale;           // log2(e) over a temperature (not with kOneSoftmax)
+  float scale;           // log2(e) over a temperature (not with one softmax)
 };
 
 // Backward recompute: G[n][c] = dLoss/dS for one vocabulary band, stored bf16.
@@ -608,7 +611,7 @@ struct GradParams {
 // row so the 16 lanes of a write phase hit distinct banks), reads it back
 // row-major and stores whole 128-byte row segments, 8 rows per instruction.
 // A wave's LDS operations execute in order, so no barrier is needed.
-template <int BN, bool HB, int SM = kOneSoftmax>
+template <int BN, bool HB, int SM = kCrossEntropy>
 struct EpiGradT {
   static constexpr bool DU = SM == kTwoSoftmaxes;
   typedef GradParams Params;
@@ -649,7 +652,7 @@ struct EpiGradT {
     constexpr int kArea = 32 * (BN / 2);  // 32 rows x the wave's columns, in 32 x 64 blocks
     bf16_t* const ws = scratch + (wm * 2 + wn) * 2 * kArea;
     const int col0 = tn * BN + wn * (BN / 2);
-    const float scale = SM == kOneSoftmax ? kLog2e : p.scale;
+    const float scale = SM == kOneSoftmax || SM == kCrossEntropy ? kLog2e : p.scale;
     auto stage = [&](int i, float4 rp, auto INTERIOR) __attribute__((always_inline)) {
       int lp = l;
       asm volatile("" : "+v"(lp));  // the columns' masks are not kept from row block to row block
@@ -749,7 +752,7 @@ struct EpiGradT {
         stage(i, rp, std::true_type{});
       else
         stage(i, rp, std::false_type{});
-      if constexpr (SM == kOneSoftmax) one_hot(i, rp, lab);
+      if constexpr (SM == kCrossEntropy) one_hot(i, rp, lab);
       if (i > 0) store(i - 1);
       rp = rp1;
       lab = lab1;
@@ -760,19 +763,6 @@ struct EpiGradT {
                                        int) {}
 };
 
-template <int BN>
-using EpiGrad = EpiGradT<BN, false>;
-template <int BN>
-using EpiGradBias = EpiGradT<BN, true>;
-template <int BN>
-using EpiGradTemp = EpiGradT<BN, false, kAtTemperature>;
-template <int BN>
-using EpiGradBiasTemp = EpiGradT<BN, true, kAtTemperature>;
-template <int BN>
-using EpiGradTwo = EpiGradT<BN, false, kTwoSoftmaxes>;
-template <int BN>
-using EpiGradBiasTwo = EpiGradT<BN, true, kTwoSoftmaxes>;
-
 struct AccParams {
   float* acc32;
   long ldacc;
@@ -781,14 +771,17 @@ struct AccParams {
   int out_f32;  // 0: bf16 output, 1: fp32 output
   int mode;
   const int* rowmap = nullptr;  // out row of GEMM row m (acc32 keeps GEMM rows); null: m
+  const float* unit = nullptr;  // EpiAccT's, with UNIT
 };
 
 // Plain GEMM output with optional fp32 accumulation buffer.
 //   mode 0: out = C            1: acc32 = C
 //   mode 2: acc32 += C          3: out = acc32 + C
 //   mode 4: out += C (fp32 output only: the output is its own accumulator)
-template <int BN>
-struct EpiAcc {
+// UNIT: C is the product times *unit, else the product (as a parameter of the
+// launch, the unit cost the cross-entropy of 2048 x 896 x 151936 0.5%).
+template <int BN, bool UNIT>
+struct EpiAccT {
   typedef AccParams Params;
   static constexpr bool kOneTile = true;
   static constexpr bool kDynSplits = false;
@@ -884,12 +877,17 @@ struct EpiAcc {
     pin_epilogue(l, tm, tn);
     float* const ws = reinterpret_cast<float*>(scratch) + (wm * 2 + wn) * 32 * kPitch;
     const int n0 = tn * BN + wn * kC;
+    const float unit = UNIT ? *p.unit : 1.f;
 #pragma unroll 1
     for (int i = 0; i < FM; ++i) {
       const int m0 = tm * kBM + acc_row(wm, i, 0);
       if (m0 >= g.M) break;
       f32x16 x[BN / 64];
       acc.take_row(i, x);
+      if constexpr (UNIT) {
+#pragma unroll
+        for (int j = 0; j < BN / 64; ++j) x[j] *= unit;
+      }
       if (m0 + 32 <= g.M && n0 + kC <= g.N)
         rows32<true>(p, x, g, m0, n0, l, ws);
       else
@@ -1197,7 +1195,7 @@ struct BandLaunch {
 };
 
 // One workgroup of the dH population (see BandLaunch).
-template <int BN>
+template <int BN, template <int> class Epi>
 __device__ __forceinline__ void dh_body(const GemmShape& g0, const AccParams& e0, int ks, int kc, long stride, int b,
                                      int nb, bf16_t* smem) {
   const int k = b % ks, k0 = k * kc;
@@ -1207,13 +1205,23 @@ __device__ __forceinline__ void dh_body(const GemmShape& g0, const AccParams& e0
   g.B += k0 * g.ldb;
   g.K = min(kc, g0.K - k0);
   e.acc32 += k * stride;
-  gemm_body<BN, true, false, EpiAcc>(g, e, b / ks, nb / ks, smem);
+  gemm_body<BN, true, false, Epi>(g, e, b / ks, nb / ks, smem);
 }
+
+// The epilogues of a band launch, by EpiGradT's SM and HB.
+template <int SM, bool HB>
+struct BandEpi {
+  template <int BN>
+  using Grad = EpiGradT<BN, HB, SM>;
+  template <int BN>
+  using Acc = EpiAccT<BN, SM != kCrossEntropy>;
+};
 
 // HB: with a bias.  AROW: the recompute reads H's rows through the row order.
 // KTAIL: d is no multiple of 64 (the recompute's K).  SM: EpiGradT's.
-template <bool HB, bool AROW, bool KTAIL, int SM = kOneSoftmax>
+template <bool HB, bool AROW, bool KTAIL, int SM>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))) void band_kernel(BandLaunch p) {
+  typedef BandEpi<SM, HB> Epi;
   __shared__ __attribute__((aligned(16))) bf16_t smem[kLdsElems];
   // the populations in the launch's order, then the reduction
   int b = blockIdx.x, pop = kPopReduce;
@@ -1228,33 +1236,23 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
   }
   if (pop == kPopDW) {
     if (b < p.nb_dw) {
-      gemm_body<kBN, false, true, EpiAcc>(p.dw, p.e_dw, b, p.nb_dw, smem);
+      gemm_body<kBN, false, true, Epi::template Acc>(p.dw, p.e_dw, b, p.nb_dw, smem);
       return;
     }
-    gemm_body<kTailBN, false, true, EpiAcc>(p.dw2, p.e_dw2, b - p.nb_dw, p.nb_dw2, smem);
+    gemm_body<kTailBN, false, true, Epi::template Acc>(p.dw2, p.e_dw2, b - p.nb_dw, p.nb_dw2, smem);
     return;
   }
   if (pop == kPopDH) {
     if (b < p.nb_dh) {
-      dh_body<kBN>(p.dh, p.e_dh, p.dh_ks, p.dh_kc, p.dh_part_stride, b, p.nb_dh, smem);
+      dh_body<kBN, Epi::template Acc>(p.dh, p.e_dh, p.dh_ks, p.dh_kc, p.dh_part_stride, b, p.nb_dh, smem);
       return;
     }
-    dh_body<kTailBN>(p.dh2, p.e_dh2, p.dh_ks, p.dh_kc, p.dh_part_stride, b - p.nb_dh, p.nb_dh2, smem);
+    dh_body<kTailBN, Epi::template Acc>(p.dh2, p.e_dh2, p.dh_ks, p.dh_kc, p.dh_part_stride, b - p.nb_dh, p.nb_dh2,
+                                        smem);
     return;
   }
   if (pop == kPopGrad) {
-    if constexpr (SM == kOneSoftmax && HB)
-      gemm_body<kBN, true, true, EpiGradBias, AROW, KTAIL>(p.gr, p.e_gr, b, p.nb_gr, smem);
-    else if constexpr (SM == kOneSoftmax)
-      gemm_body<kBN, true, true, EpiGrad, AROW, KTAIL>(p.gr, p.e_gr, b, p.nb_gr, smem);
-    else if constexpr (SM == kAtTemperature && HB)
-      gemm_body<kBN, true, true, EpiGradBiasTemp, AROW, KTAIL>(p.gr, p.e_gr, b, p.nb_gr, smem);
-    else if constexpr (SM == kAtTemperature)
-      gemm_body<kBN, true, true, EpiGradTemp, AROW, KTAIL>(p.gr, p.e_gr, b, p.nb_gr, smem);
-    else if constexpr (HB)
-      gemm_body<kBN, true, true, EpiGradBiasTwo, AROW, KTAIL>(p.gr, p.e_gr, b, p.nb_gr, smem);
-    else
-      gemm_body<kBN, true, true, EpiGradTwo, AROW, KTAIL>(p.gr, p.e_gr, b, p.nb_gr, smem);
+    gemm_body<kBN, true, true, Epi::template Grad, AROW, KTAIL>(p.gr, p.e_gr, b, p.nb_gr, smem);
     return;
   }
   dh_reduce_body(p.red, b * (long)kThreads + threadIdx.x, (long)p.nb_red * kThreads);
@@ -1975,12 +1973,12 @@ __global__ __launch_bounds__(256) void transpose_kernel(const bf16_t* __restrict
   }
 }
 
-// dB[c] = sum_m G[m][c] for c < C (fixed order: deterministic).  Block = 64
-// columns.  With `live`, M = min(M, live rows of the block at live_base);
+// dB[c] = sum_m G[m][c] for c < C (fixed order: deterministic), times *unit
+// where there is one.  Block = 64 columns.  With `live`, M = min(M, live rows of the block at live_base);
 // with `accumulate`, out[c] += the sum (row blocks after the first).
 __global__ __launch_bounds__(256) void colsum_kernel(const bf16_t* __restrict__ G, long ldg, int M, int C,
                                                      const int* __restrict__ live, int live_base, int accumulate,
-                                                     float* __restrict__ out) {
+                                                     const float* __restrict__ unit, float* __restrict__ out) {
   // blockIdx.y = row split: rows [y*M/gridDim.y, (y+1)*M/gridDim.y) into out[y][C]
   __shared__ float part[32][65];
   if (live) M = min(M, live_rows(live, live_base));
@@ -2020,6 +2018,7 @@ __global__ __launch_bounds__(256) void colsum_kernel(const bf16_t* __restrict__ 
   if (tid < 64) {
     float s = 0.f;
     for (int r = 0; r < 32; ++r) s += part[r][tid];
+    if (unit) s *= *unit;
     const int c = blockIdx.x * 64 + tid;
     if (c < C) out[c] = accumulate ? out[c] + s : s;
   }
@@ -2305,9 +2304,10 @@ struct BwdLayout {
   // null when unsplit
   float* dhpart;
   int dh_ks;
-  // SparseGrad's columns and values
+  // SparseGrad's columns and values, and the unit of G
   int* col;
   float* val;
+  float* unit;
   size_t bytes;
 };
 
@@ -2375,6 +2375,7 @@ BwdLayout bwd_layout(void* ws, long N, long d, long V, long Vb, bool need_dh, bo
                          : nullptr;
   L.col = entries ? c.take<int>((size_t)N * entries) : nullptr;
   L.val = entries ? c.take<float>((size_t)N * entries) : nullptr;
+  L.unit = entries ? c.take<float>(1) : nullptr;
   L.bytes = align_up(c.off, 256);
   return L;
 }
@@ -2543,7 +2544,7 @@ auto* pick_band(bool has_bias, bool arow, bool ktail) {
 }
 
 int launch_band(const BandLaunch& p, bool has_bias, hipStream_t st, int kind = CCE_KERNEL_BWD_BAND,
-                int softmaxes = kOneSoftmax) {
+                int softmaxes = kCrossEntropy) {
   const int nb = p.nb_dw + p.nb_dw2 + p.nb_dh + p.nb_dh2 + p.nb_gr + p.nb_red;
   if (nb <= 0) return CCE_OK;
   int rc = CCE_OK;
@@ -2557,7 +2558,8 @@ int launch_band(const BandLaunch& p, bool has_bias, hipStream_t st, int kind = C
   hipEvent_t t0 = nullptr, t1 = nullptr;
   const bool timed = timing_begin(st, &t0, &t1);
   const bool arow = p.gr.arow != nullptr;
-  auto* const kernel = softmaxes == kOneSoftmax      ? pick_band<kOneSoftmax>(has_bias, arow, ktail)
+  auto* const kernel = softmaxes == kCrossEntropy    ? pick_band<kCrossEntropy>(has_bias, arow, ktail)
+                       : softmaxes == kOneSoftmax    ? pick_band<kOneSoftmax>(has_bias, arow, ktail)
                        : softmaxes == kAtTemperature ? pick_band<kAtTemperature>(has_bias, arow, ktail)
                                                      : pick_band<kTwoSoftmaxes>(has_bias, arow, ktail);
   hipLaunchKernelGGL(kernel, dim3(nb), dim3(kThreads), 0, st, p);
@@ -2697,7 +2699,7 @@ int forward_run(const void* hidden, const void* weight, const void* labels, int 
   const bool uniform = smoothing_form == CCE_SMOOTH_UNIFORM && label_smoothing > 0.f;
   if (uniform) {
     hipLaunchKernelGGL(colsum_kernel, dim3((unsigned)ceil_div(d, 64), (unsigned)L.wsplits), dim3(256), 0, st,
-                       static_cast<const bf16_t*>(weight), (long)d, (int)V, (int)d, nullptr, 0, 0, L.wpart);
+                       static_cast<const bf16_t*>(weight), (long)d, (int)V, (int)d, nullptr, 0, 0, nullptr, L.wpart);
     HIP_TRY(hipGetLastError());
     hipLaunchKernelGGL(sum_parts_kernel, dim3((unsigned)ceil_div(d, 256)), dim3(256), 0, st, L.wpart, L.wsplits,
                        (int)d, bias, (int)V, L.wsum);
@@ -2725,9 +2727,10 @@ struct SparseGrad {
   int softmaxes;  // EpiGradT
   int entries;  // columns per row
   // rowp and rowlab of the N rows in the GEMM's order (idx; null: as they are),
-  // their columns ([N][entries], -1: none) and the values of G there
+  // their columns ([N][entries], -1: none) and the values of G there, all in
+  // units of *unit, which multiplies the products with G
   int (*prep)(const SparseGrad& s, const int* idx, long N, float4* rowp, int* rowlab, int* col, float* val,
-              hipStream_t st);
+              float* unit, hipStream_t st);
   const void* args;
 };
 
@@ -2804,7 +2807,7 @@ int backward_run(const float* grad_out, const void* hidden, const void* weight, 
     }
   }
   if (sparse) {
-    rc = sparse->prep(*sparse, L.idx, N, L.rowp, L.rowlab, L.col, L.val, st);
+    rc = sparse->prep(*sparse, L.idx, N, L.rowp, L.rowlab, L.col, L.val, L.unit, st);
     if (rc) return rc;
   } else {
     hipLaunchKernelGGL(bwd_prep_kernel, dim3((unsigned)ceil_div(N, 256)), dim3(256), 0, st, grad_out, lse, n_valid,
@@ -2863,6 +2866,7 @@ int backward_run(const float* grad_out, const void* hidden, const void* weight, 
     g.M = (int)rows; g.N = (int)nc; g.K = (int)vb;
     g.live = L.live; g.dyn = L.live ? kDynM : kDynNone; g.live_base = (int)m0;
     e.rowmap = L.idx ? L.idx + m0 : nullptr;
+    e.unit = L.unit;
     e.acc32 = L.dHacc ? L.dHacc + m0 * d + c0 : nullptr; e.ldacc = d;
     // with a row map the output rows are global (the map holds them);
     // without one (no compaction) the block's rows start at m0
@@ -2884,6 +2888,7 @@ int backward_run(const float* grad_out, const void* hidden, const void* weight, 
     g.M = (int)vb; g.N = (int)nc; g.K = (int)rows;
     g.live = L.live; g.dyn = L.live ? kDynK : kDynNone; g.live_base = (int)m0;
     e.rowmap = nullptr;
+    e.unit = L.unit;
     e.acc32 = L.dWacc ? L.dWacc + c0 : nullptr; e.ldacc = d;
     const long o = v0 * d + c0;
     e.out = dw_f32 ? static_cast<void*>(static_cast<float*>(grad_weight) + o)
@@ -2898,7 +2903,7 @@ int backward_run(const float* grad_out, const void* hidden, const void* weight, 
     band_cols(b, v0, vb);
     block_span(r, m0, rows);
     hipLaunchKernelGGL(colsum_kernel, dim3((unsigned)ceil_div(vb, 64)), dim3(256), 0, st, G, (long)Vb, (int)rows,
-                       (int)vb, L.live, (int)m0, r > 0 ? 1 : 0, grad_bias + v0);
+                       (int)vb, L.live, (int)m0, r > 0 ? 1 : 0, L.unit, grad_bias + v0);
     HIP_TRY(hipGetLastError());
     return CCE_OK;
   };
@@ -2921,7 +2926,7 @@ int backward_run(const float* grad_out, const void* hidden, const void* weight, 
     HIP_TRY(hipGetLastError());
     return CCE_OK;
   };
-  const int softmaxes = sparse ? sparse->softmaxes : kOneSoftmax;
+  const int softmaxes = sparse ? sparse->softmaxes : kCrossEntropy;
 
   // launch u: dW and dH of unit u from G[u & 1] and the recompute of unit
   // u+1 into G[(u+1) & 1]; unit 0's recompute runs alone first.

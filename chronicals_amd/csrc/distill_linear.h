@@ -125,17 +125,50 @@ struct DistillGrad {
   Teacher a;
 };
 
+// The unit of G.  G is held in bf16, and at a row's label it is nearly the same
+// number in every row, -ce g (or without labels -kd T g, where one entry has all
+// the weight): rounded the same way in every row, half a step of it, up to 2^-8 of
+// the label's share, would stay in the sums over the rows.  So G is held over the
+// mantissa of that number, in [1, 2), and the products' fp32 sums are multiplied by
+// it: the number itself becomes a power of two, no range is lost, and what is
+// rounded differs from row to row.
+__device__ inline float mantissa(float x) { return __uint_as_float((__float_as_uint(x) & 0x007fffffu) | 0x3f800000u); }
+__device__ inline float unit_of(const Teacher& a, float g) { return mantissa(g * (a.ce != 0.f ? a.ce : a.kdg)); }
+
+// *unit where every row has a factor of its own: the largest finite one's, which
+// all have where a mean or a masked mean of the rows follows.
+__global__ __launch_bounds__(1024) void kd_unit_kernel(Teacher a, const float* __restrict__ grad_out, int N,
+                                                       float* __restrict__ unit) {
+  __shared__ float red[16];
+  float g = 0.f;
+  for (int n = threadIdx.x; n < N; n += 1024) {
+    const float v = fabsf(grad_out[n]);
+    if (v < INFINITY) g = fmaxf(g, v);
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) g = fmaxf(g, __shfl_xor(g, o));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = g;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int w = 1; w < 16; ++w) g = fmaxf(g, red[w]);
+  *unit = unit_of(a, g);
+}
+
 // One workgroup per GEMM row i of source row idx[i] (idx null: i): its
-// coefficients, and the gradient at its K + 1 columns.
+// coefficients, and the gradient at its K + 1 columns, in units of *unit.
 template <bool DU>
 __global__ __launch_bounds__(256) void kd_linear_prep_kernel(DistillGrad p, const int* __restrict__ idx,
                                                              float4* __restrict__ rowp, int* __restrict__ rowlab,
-                                                             int* __restrict__ cols, float* __restrict__ vals) {
+                                                             int* __restrict__ cols, float* __restrict__ vals,
+                                                             float* __restrict__ unit) {
   __shared__ Entries e;
   const int tid = threadIdx.x, K = p.a.K;
   const long i = blockIdx.x, n = idx ? idx[i] : i;
   const int r = p.rows[n];
+  const float g = grad_factor(p.grad_out, p.n_valid, p.reduction, n);
+  const float u = p.reduction == CCE_REDUCTION_NONE ? *unit : unit_of(p.a, g);
   if (tid == 0) rowlab[i] = -1;
+  if (i == 0 && tid == 0 && p.reduction != CCE_REDUCTION_NONE) *unit = u;
   if (r < 0) {
     if (tid == 0) rowp[i] = make_float4(FLT_MAX, 0.f, 0.f, DU ? FLT_MAX : 0.f);
     for (int j = tid; j <= K; j += 256) cols[i * (K + 1) + j] = -1;
@@ -144,9 +177,8 @@ __global__ __launch_bounds__(256) void kd_linear_prep_kernel(DistillGrad p, cons
   int col;
   float q, lq;
   const bool any = load_entries(p.a, n, p.V, e, col, q, lq);
-  const float g = grad_factor(p.grad_out, p.n_valid, p.reduction, n);
   const float2 st = p.stats[n];
-  const float scale = kLog2e * p.a.inv_t, ce = g * p.a.ce, kdg = any ? g * p.a.kdg : 0.f;
+  const float scale = kLog2e * p.a.inv_t, ce = g * p.a.ce / u, kdg = any ? g * p.a.kdg / u : 0.f;
   const float cp = DU ? kdg : kdg + ce;
   const int label = r < p.V && p.a.ce != 0.f ? r : -1;
   if (tid == 0) rowp[i] = make_float4(st.x, cp, DU ? ce : 0.f, DU ? st.y : 0.f);
@@ -165,13 +197,14 @@ __global__ __launch_bounds__(256) void kd_linear_prep_kernel(DistillGrad p, cons
 }
 
 int distill_prep(const SparseGrad& s, const int* idx, long N, float4* rowp, int* rowlab, int* col, float* val,
-                 hipStream_t st) {
+                 float* unit, hipStream_t st) {
   const DistillGrad& p = *static_cast<const DistillGrad*>(s.args);
-  if (s.softmaxes == kTwoSoftmaxes)
-    hipLaunchKernelGGL(kd_linear_prep_kernel<true>, dim3((unsigned)N), dim3(256), 0, st, p, idx, rowp, rowlab, col, val);
-  else
-    hipLaunchKernelGGL(kd_linear_prep_kernel<false>, dim3((unsigned)N), dim3(256), 0, st, p, idx, rowp, rowlab, col,
-                       val);
+  if (p.reduction == CCE_REDUCTION_NONE) {
+    hipLaunchKernelGGL(kd_unit_kernel, dim3(1), dim3(1024), 0, st, p.a, p.grad_out, (int)N, unit);
+    HIP_TRY(hipGetLastError());
+  }
+  auto* const prep = s.softmaxes == kTwoSoftmaxes ? kd_linear_prep_kernel<true> : kd_linear_prep_kernel<false>;
+  hipLaunchKernelGGL(prep, dim3((unsigned)N), dim3(256), 0, st, p, idx, rowp, rowlab, col, val, unit);
   HIP_TRY(hipGetLastError());
   return CCE_OK;
 }

@@ -34,8 +34,8 @@ so with ``ce_weight`` the labels' loss comes from the same passes.
     tensors get no gradient, and gradients cannot be differentiated again.
   * ``linear_distillation_loss`` computes in bf16 with fp32 accumulation (fp16 and
     fp32 operands are rounded to bf16 at the boundary) and rounds the gradient of
-    the logits to bf16 once, as ``cut_cross_entropy`` does; gradients come back in
-    the input dtypes.
+    the logits to bf16 once, as ``cut_cross_entropy`` does, in units that hold the
+    label's share of it exactly; gradients come back in the input dtypes.
 
 The reference has no distillation; the argument order follows its losses.
 """
