@@ -332,7 +332,8 @@ int check_teacher(const cce_teacher* t, long N, const void* labels, int64_t igno
     return fail(CCE_ERR_INVALID_ARG, "temperature must be in [0.01, 1000] (got %g)", (double)t->temperature);
   if (!(fabsf(t->distill_weight) < INFINITY) || !(fabsf(t->ce_weight) < INFINITY))
     return fail(CCE_ERR_INVALID_ARG, "distill_weight and ce_weight must be finite");
-  if (t->ce_weight != 0.f && !labels) return fail(CCE_ERR_INVALID_ARG, "ce_weight needs labels");
+  // without rows, labels that were given may well be at a null address
+  if (N > 0 && t->ce_weight != 0.f && !labels) return fail(CCE_ERR_INVALID_ARG, "ce_weight needs labels");
   if (N > 0 && (!t->logits || !t->indices))
     return fail(CCE_ERR_INVALID_ARG, "the teacher's logits and indices must not be null");
   a.t = t->logits;
