@@ -564,6 +564,11 @@ Tensor as_rows(const Tensor& t) {
 optional<Tensor> given(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : std::nullopt; }
 optional<Tensor> contiguous(const optional<Tensor>& t) { return t.has_value() ? optional<Tensor>(t->contiguous()) : t; }
 
+// The one element of a fresh tensor.  Autograd forbids its user to change a result
+// of a function in place that is a view made inside the function; this one, as
+// _unsafe_view elsewhere, counts as none, and nothing else holds its storage.
+Tensor scalar(const Tensor& t) { return at::_unsafe_view(t, at::IntArrayRef()); }
+
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const optional<Tensor>& weight,
                         const optional<Tensor>& bias, double eps) {
@@ -576,7 +581,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const optional<Tensor>& p = weight.has_value() ? weight : bias;
     ctx->saved_data["param_f32"] = p.has_value() && p->scalar_type() == at::kFloat;
     ctx->saved_data["bias"] = bias.has_value();
-    return y.view_symint(x.sym_sizes());
+    return x.dim() == 2 ? y : at::_unsafe_view_symint(y, x.sym_sizes());
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     static const auto bwd =
@@ -617,7 +622,7 @@ struct DistillLogits : torch::autograd::Function<DistillLogits> {
     ctx->saved_data["reduction"] = reduction;
     ctx->saved_data["dim"] = logits.dim();
     if (logits.dim() != 2) ctx->saved_data["shape"] = logits.sym_sizes();
-    return reduction == CCE_REDUCTION_NONE ? loss : loss.reshape(at::IntArrayRef());
+    return reduction == CCE_REDUCTION_NONE ? loss : scalar(loss);
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     static const auto bwd =
@@ -662,7 +667,7 @@ struct DistillLinear : torch::autograd::Function<DistillLinear> {
     ctx->saved_data["hidden"] = (int64_t)hidden.scalar_type();
     ctx->saved_data["weight"] = (int64_t)weight.scalar_type();
     if (bias.has_value()) ctx->saved_data["bias"] = (int64_t)bias->scalar_type();
-    return reduction == CCE_REDUCTION_NONE ? loss : loss.reshape(at::IntArrayRef());
+    return reduction == CCE_REDUCTION_NONE ? loss : scalar(loss);
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     static const auto bwd = find<std::tuple<Tensor, Tensor, Tensor>(
