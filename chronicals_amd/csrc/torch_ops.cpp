@@ -26,6 +26,8 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -542,7 +544,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor& grad_y, const Te
 // ---------------------------------------------------------------------------
 // Differentiable operators: autograd functions over the ones above, which they
 // call through the dispatcher, so that a trace sees those.  The gradients are
-// kernels' results and have none of their own.
+// kernels' results and have none of their own (gradients()).
 // ---------------------------------------------------------------------------
 using c10::SymInt;
 using torch::autograd::AutogradContext;
@@ -569,6 +571,33 @@ optional<Tensor> contiguous(const optional<Tensor>& t) { return t.has_value() ? 
 // _unsafe_view elsewhere, counts as none, and nothing else holds its storage.
 Tensor scalar(const Tensor& t) { return at::_unsafe_view(t, at::IntArrayRef()); }
 
+// The body of a backward: the gradients are computed without a graph of their own.
+// Where one is asked for (create_graph), they lead to what the function's inputs
+// and its incoming gradient came from, through a node that raises.  Without it
+// they would be constants where the operands saved are copies (of another type,
+// of strided rows), and a penalty on them would be left out without a word.
+template <typename F>
+variable_list gradients(const Tensor& grad, F&& compute) {
+  const bool twice = at::GradMode::is_enabled();
+  variable_list out;
+  {
+    at::AutoGradMode off(false);
+    out = compute();
+  }
+  if (!twice) return out;
+  torch::autograd::edge_list edges;
+  if (const auto node = torch::autograd::get_current_node()) edges = node->next_edges();
+  if (grad.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(grad));
+  const auto error = std::make_shared<torch::autograd::Error>(
+      "the gradients of chronicals_hip operators cannot be differentiated again", std::move(edges));
+  for (Tensor& t : out) {
+    if (!t.defined()) continue;
+    t = t.tensor_data();  // no view: it gets a graph
+    torch::autograd::set_history(t, error);
+  }
+  return out;
+}
+
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const optional<Tensor>& weight,
                         const optional<Tensor>& bias, double eps) {
@@ -593,11 +622,13 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
                need_dw = has_w && ctx->needs_input_grad(1),
                need_db = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(has_w ? 2 : 1);
     if (!need_dx && !need_dw && !need_db) return variable_list(4);
-    const Tensor g = grads[0].reshape_symint(saved[0].sym_sizes()).contiguous();
-    const auto [dx, dw, db] = bwd.call(g, saved[0], given(saved[1]), saved[2], saved[3],
-                                       ctx->saved_data["param_f32"].toBool(), need_dx, need_dw, need_db);
-    return {need_dx ? dx.view_symint(grads[0].sym_sizes()) : Tensor(), need_dw ? dw : Tensor(), need_db ? db : Tensor(),
-            Tensor()};
+    return gradients(grads[0], [&]() -> variable_list {
+      const Tensor g = grads[0].reshape_symint(saved[0].sym_sizes()).contiguous();
+      const auto [dx, dw, db] = bwd.call(g, saved[0], given(saved[1]), saved[2], saved[3],
+                                         ctx->saved_data["param_f32"].toBool(), need_dx, need_dw, need_db);
+      return {need_dx ? dx.view_symint(grads[0].sym_sizes()) : Tensor(), need_dw ? dw : Tensor(),
+              need_db ? db : Tensor(), Tensor()};
+    });
   }
 };
 
@@ -628,14 +659,16 @@ struct DistillLogits : torch::autograd::Function<DistillLogits> {
     static const auto bwd =
         find<Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const optional<Tensor>&, const Tensor&,
                     const Tensor&, double, double, double, SymInt, SymInt)>("chronicals_hip::distill_logits_bwd");
-    variable_list out(9);
-    if (!ctx->needs_input_grad(0)) return out;
-    const auto s = ctx->get_saved_variables();
-    const auto how = ctx->saved_data["how"].toDoubleVector();
-    out[0] = bwd.call(grads[0], s[0], s[1], s[2], given(s[3]), s[4], s[5], how[0], how[1], how[2],
-                      ctx->saved_data["ignore_index"].toInt(), ctx->saved_data["reduction"].toInt());
-    if (ctx->saved_data["dim"].toInt() != 2) out[0] = out[0].view_symint(ctx->saved_data["shape"].toSymIntVector());
-    return out;
+    if (!ctx->needs_input_grad(0)) return variable_list(9);
+    return gradients(grads[0], [&] {
+      variable_list out(9);
+      const auto s = ctx->get_saved_variables();
+      const auto how = ctx->saved_data["how"].toDoubleVector();
+      out[0] = bwd.call(grads[0], s[0], s[1], s[2], given(s[3]), s[4], s[5], how[0], how[1], how[2],
+                        ctx->saved_data["ignore_index"].toInt(), ctx->saved_data["reduction"].toInt());
+      if (ctx->saved_data["dim"].toInt() != 2) out[0] = out[0].view_symint(ctx->saved_data["shape"].toSymIntVector());
+      return out;
+    });
   }
 };
 
@@ -674,23 +707,25 @@ struct DistillLinear : torch::autograd::Function<DistillLinear> {
         const Tensor&, const Tensor&, const Tensor&, const optional<Tensor>&, const Tensor&, const Tensor&, const Tensor&,
         const Tensor&, const Tensor&, const Tensor&, double, double, double, SymInt, SymInt, bool, bool, bool, bool,
         bool)>("chronicals_hip::distill_bwd");
-    variable_list out(12);
     const auto s = ctx->get_saved_variables();
     const bool need_dh = ctx->needs_input_grad(0), need_dw = ctx->needs_input_grad(1),
                need_db = s[2].defined() && ctx->needs_input_grad(2);
-    if (!need_dh && !need_dw && !need_db) return out;
-    auto& kept = ctx->saved_data;
-    const auto how = kept["how"].toDoubleVector();
-    const auto htype = (at::ScalarType)kept["hidden"].toInt(), wtype = (at::ScalarType)kept["weight"].toInt();
-    // bf16 inputs get bf16 gradients, fp16 and fp32 inputs get them from fp32
-    const auto [dh, dw, db] =
-        bwd.call(grads[0], s[0], s[1], given(s[2]), s[3], s[4], s[5], s[6], s[7], s[8], how[0], how[1], how[2],
-                 kept["reduction"].toInt(), kept["chunk_size"].toInt(), need_dh, need_dw, need_db,
-                 htype != at::kBFloat16, wtype != at::kBFloat16);
-    if (need_dh) out[0] = dh.view_symint(kept["shape"].toSymIntVector()).to(htype);
-    if (need_dw) out[1] = dw.to(wtype);
-    if (need_db) out[2] = db.to((at::ScalarType)kept["bias"].toInt());
-    return out;
+    if (!need_dh && !need_dw && !need_db) return variable_list(12);
+    return gradients(grads[0], [&] {
+      variable_list out(12);
+      auto& kept = ctx->saved_data;
+      const auto how = kept["how"].toDoubleVector();
+      const auto htype = (at::ScalarType)kept["hidden"].toInt(), wtype = (at::ScalarType)kept["weight"].toInt();
+      // bf16 inputs get bf16 gradients, fp16 and fp32 inputs get them from fp32
+      const auto [dh, dw, db] =
+          bwd.call(grads[0], s[0], s[1], given(s[2]), s[3], s[4], s[5], s[6], s[7], s[8], how[0], how[1], how[2],
+                   kept["reduction"].toInt(), kept["chunk_size"].toInt(), need_dh, need_dw, need_db,
+                   htype != at::kBFloat16, wtype != at::kBFloat16);
+      if (need_dh) out[0] = dh.view_symint(kept["shape"].toSymIntVector()).to(htype);
+      if (need_dw) out[1] = dw.to(wtype);
+      if (need_db) out[2] = db.to((at::ScalarType)kept["bias"].toInt());
+      return out;
+    });
   }
 };
 

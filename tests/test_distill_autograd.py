@@ -44,3 +44,48 @@ def test_results_may_be_changed_in_place(make):
     y /= 4
     y += 1
     y.sum().backward()
+
+
+def strided(*shape):
+    """A leaf whose transpose has rows that are not contiguous: the operators work on a copy."""
+    return leaf(*reversed(shape)), lambda v: v.t()
+
+
+TWICE = {
+    "norm": lambda: (x := leaf(12, 16), norm(x)),
+    "norm of a copy": lambda: ((p := strided(12, 16))[0], norm(p[1](p[0]))),
+    "norm, the weight": lambda: (w := leaf(16), ops.layer_norm(meta(12, 16), w, None, 1e-5)),
+    "logits": lambda: (x := leaf(12, 50), from_logits(x)),
+    "logits of a copy": lambda: ((p := strided(12, 50))[0], from_logits(p[1](p[0]), 0)),
+}
+for _dt in (torch.bfloat16, torch.float16, torch.float32):
+    TWICE[f"hidden, {_dt}"] = lambda dt=_dt: (h := leaf(12, 16, dtype=dt), from_head(h, meta(50, 16, dtype=dt)))
+    TWICE[f"weight, {_dt}"] = lambda dt=_dt: (w := leaf(50, 16, dtype=dt), from_head(meta(12, 16, dtype=dt), w))
+
+
+@pytest.mark.parametrize("name", list(TWICE))
+def test_gradients_are_not_differentiated_again(name):
+    """A gradient taken with create_graph leads back to the input and raises there, alone or within another loss: it is
+    never taken for a constant."""
+    x, y = TWICE[name]()
+    (g,) = torch.autograd.grad(y.sum(), x, create_graph=True)
+    assert g.requires_grad and g.shape == x.shape and g.dtype == x.dtype
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        torch.autograd.grad(g.float().square().sum(), x, retain_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        (y.sum() + g.float().square().sum()).backward()
+
+
+def test_gradients_depend_on_the_incoming_gradient():
+    x, up = leaf(12, 16), leaf(12, 16)
+    (g,) = torch.autograd.grad(norm(x), x, up, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        torch.autograd.grad(g.sum(), up)
+
+
+def test_first_gradients_have_no_graph():
+    x = leaf(12, 16)
+    (g,) = torch.autograd.grad(norm(x).sum(), x)
+    assert not g.requires_grad
+    norm(x).sum().backward()
+    assert not x.grad.requires_grad

@@ -54,3 +54,27 @@ def test_layer_norm_changed_in_place(gpu, shape):
     assert torch.equal(y, torch.relu(plain + r)) and y.shape == shape
     (y * r).sum().backward()
     assert all(torch.equal(p.grad, q) for p, q in zip(leaves, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_gradients_are_not_differentiated_again(gpu, dtype):
+    """Taken with create_graph they have the same bits, and a penalty on them raises, also where the operands that were
+    saved are copies."""
+    from chronicals_amd.kernels.distillation import distillation_loss, linear_distillation_loss
+    from chronicals_amd.kernels.layer_norm import layer_norm
+    v = inputs(gpu, dtype)
+    h, w, x = (v[k].requires_grad_(True) for k in ("h", "w", "x"))
+    wide = v["x"].detach().permute(2, 1, 0).contiguous().permute(2, 1, 0).requires_grad_(True)
+    assert wide.stride(-1) != 1
+    cases = [(lambda: linear_distillation_loss(h, w, v["t"], v["index"], v["lab"], **HOW), [h, w]),
+             (lambda: distillation_loss(x, v["t"], v["index"], v["lab"], **HOW), [x]),
+             (lambda: distillation_loss(wide, v["t"], v["index"], v["lab"], **HOW), [wide]),
+             (lambda: layer_norm(wide).square().mean(), [wide])]
+    for f, leaves in cases:
+        plain = torch.autograd.grad(f(), leaves)
+        loss = f()
+        grads = torch.autograd.grad(loss, leaves, create_graph=True)
+        for leaf, p, g in zip(leaves, plain, grads):
+            assert g.requires_grad and not p.requires_grad and torch.equal(g, p) and g.stride() == p.stride()
+            with pytest.raises(RuntimeError, match="differentiated again"):
+                torch.autograd.grad(loss + g.float().square().sum(), leaf, retain_graph=True)
