@@ -11,7 +11,7 @@ import threading
 from . import build as _build
 
 # constants mirrored from include/chronicals_cce.h
-CCE_ABI_VERSION = 8
+CCE_ABI_VERSION = 9
 CCE_OK = 0
 CCE_ERR_INVALID_ARG = 1
 CCE_ERR_WORKSPACE = 2
@@ -150,6 +150,7 @@ SIGNATURES = {
         _i64, _i64, _f32, _vp, _vp, _vp, _vp,  # N, D, eps, y_out, mean_out, rstd_out, stream
     ]),
     "cce_layer_norm_backward_workspace_bytes": (_i32, [_i64, _i64, _size_out]),
+    "cce_layer_norm_backward_workspace_bytes_for": (_i32, [_i64, _i64, _i32, _i32, _size_out]),
     "cce_layer_norm_backward": (_i32, [
         _vp, _vp, _i32, _i64, _vp, _i32,     # grad_y, x, dtype, ldx, weight, param_dtype
         _vp, _vp, _i64, _i64,                # mean, rstd, N, D

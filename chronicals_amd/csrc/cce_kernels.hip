@@ -3558,7 +3558,16 @@ int cce_layer_norm_backward_workspace_bytes(int64_t N, int64_t D, size_t* bytes)
   if (!bytes) return fail(CCE_ERR_INVALID_ARG, "bytes must not be null");
   const int rc = check_norm(N, D, CCE_DTYPE_F32, D, CCE_DTYPE_F32);
   if (rc) return rc;
-  *bytes = norm_layout(nullptr, N, D).bytes;
+  *bytes = norm_layout(nullptr, most_norm_parts(N, D), D).bytes;
+  return CCE_OK;
+}
+
+int cce_layer_norm_backward_workspace_bytes_for(int64_t N, int64_t D, int dtype, int need_params, size_t* bytes) {
+  g_err[0] = 0;
+  if (!bytes) return fail(CCE_ERR_INVALID_ARG, "bytes must not be null");
+  const int rc = check_norm(N, D, dtype, D, CCE_DTYPE_F32);
+  if (rc) return rc;
+  *bytes = norm_bytes(dtype, N, D, need_params != 0);
   return CCE_OK;
 }
 
@@ -3572,11 +3581,11 @@ int cce_layer_norm_backward(const void* grad_y, const void* x, int dtype, int64_
   if (N > 0 && (!grad_y || !x || !mean || !rstd))
     return fail(CCE_ERR_INVALID_ARG, "grad_y, x, mean and rstd must not be null");
   if (misaligned(workspace)) return fail(CCE_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
-  const NormLayout need = norm_layout(nullptr, N, D);
-  if (workspace_bytes < need.bytes || !workspace)
-    return fail(CCE_ERR_WORKSPACE, "workspace too small: need %zu bytes, got %zu", need.bytes, workspace_bytes);
+  const size_t need = norm_bytes(dtype, N, D, grad_weight || grad_bias);
+  if (workspace_bytes < need || (need && !workspace))
+    return fail(CCE_ERR_WORKSPACE, "workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
   return norm_backward(grad_y, x, dtype, ldx, weight, param_dtype, mean, rstd, N, D, grad_x, grad_weight, grad_bias,
-                       norm_layout(workspace, N, D), reinterpret_cast<hipStream_t>(stream));
+                       workspace, reinterpret_cast<hipStream_t>(stream));
 }
 
 int cce_kernel_timing_enable(int enable) {

@@ -401,12 +401,11 @@ struct NormLayout {
   size_t bytes;
 };
 
-NormLayout norm_layout(void* ws, long N, long D) {
+NormLayout norm_layout(void* ws, long parts, long D) {
   Carver c(ws);
   NormLayout L;
-  const size_t parts = (size_t)most_norm_parts(N, D);
-  L.dw = c.take<float>(parts * D);
-  L.db = c.take<float>(parts * D);
+  L.dw = c.take<float>((size_t)(parts * D));
+  L.db = c.take<float>((size_t)(parts * D));
   L.bytes = align_up(c.off, 256);
   return L;
 }
@@ -447,6 +446,23 @@ bool norm_shape(long D, F&& f) {
 // rows they take 100 and 134 to 152.
 constexpr int kNormRegD = 1024 * 16;
 
+// Threads of a row of D elements in registers; 256 for longer ones, whose parts
+// are as many.
+int norm_threads(int dtype, long D) {
+  int threads = 256;
+  auto shape = [&](auto tr, auto) { threads = decltype(tr)::value; };
+  if (dtype == CCE_DTYPE_F32)
+    norm_shape<4, kNormRegD>(D, shape);
+  else
+    norm_shape<8, kNormRegD>(D, shape);
+  return threads;
+}
+
+// What one backward uses: nothing where neither dw nor db is wanted.
+size_t norm_bytes(int dtype, long N, long D, bool params) {
+  return params ? norm_layout(nullptr, norm_parts(N, D, norm_threads(dtype, D)), D).bytes : 0;
+}
+
 int norm_forward(const void* x, int dtype, int64_t ldx, const void* weight, const void* bias, int wdtype, int64_t N,
                  int64_t D, float eps, void* y, float* mean, float* rstd, hipStream_t st) {
   return norm_types(dtype, wdtype, [&](auto t, auto w) {
@@ -470,19 +486,20 @@ int norm_forward(const void* x, int dtype, int64_t ldx, const void* weight, cons
 
 int norm_backward(const void* dy, const void* x, int dtype, int64_t ldx, const void* weight, int wdtype,
                   const float* mean, const float* rstd, int64_t N, int64_t D, void* dx, void* dw, void* db,
-                  const NormLayout& L, hipStream_t st) {
+                  void* workspace, hipStream_t st) {
   return norm_types(dtype, wdtype, [&](auto t, auto w) {
     typedef decltype(t) T;
     typedef decltype(w) W;
     const bool params = dw || db;
-    long parts = norm_parts(N, D, 256);
+    if (!dx && !params) return CCE_OK;
+    const long parts = norm_parts(N, D, norm_threads(dtype, D));
+    const NormLayout L = norm_layout(params ? workspace : nullptr, parts, D);
     const bool in_registers = norm_shape<16 / sizeof(T), kNormRegD>(D, [&](auto tr, auto c) {
       constexpr int TR = decltype(tr)::value;
-      parts = norm_parts(N, D, TR);
       hipLaunchKernelGGL((layer_norm_bwd_rows_kernel<T, TR, decltype(c)::value>), dim3((unsigned)parts),
                          dim3(std::max(TR, 256)), 0, st, static_cast<const T*>(dy), static_cast<const T*>(x), (long)ldx,
                          weight, (int)(wdtype == CCE_DTYPE_F32), mean, rstd, (long)N, (int)D, static_cast<T*>(dx),
-                         params ? L.dw : nullptr, L.db);
+                         L.dw, L.db);
     });
     HIP_TRY(hipGetLastError());
     if (!in_registers && dx && N > 0) {

@@ -60,7 +60,7 @@ struct Api {
   decltype(&cce_top_logits_workspace_bytes) top_logits_workspace_bytes;
   decltype(&cce_top_logits) top_logits;
   decltype(&cce_layer_norm_forward) layer_norm_forward;
-  decltype(&cce_layer_norm_backward_workspace_bytes) layer_norm_backward_workspace_bytes;
+  decltype(&cce_layer_norm_backward_workspace_bytes_for) layer_norm_backward_workspace_bytes_for;
   decltype(&cce_layer_norm_backward) layer_norm_backward;
 };
 
@@ -532,7 +532,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor& grad_y, const Te
   Tensor dx = at::empty(need_dx ? x.sizes() : at::IntArrayRef{0}, x.options());
   Tensor dw = at::empty({need_dw ? D : 0}, popt), db = at::empty({need_db ? D : 0}, popt);
   size_t bytes = 0;
-  check(a, a.layer_norm_backward_workspace_bytes(N, D, &bytes));
+  check(a, a.layer_norm_backward_workspace_bytes_for(N, D, logits_dtype(x), need_dw || need_db, &bytes));
   const Tensor ws = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
   check(a, a.layer_norm_backward(grad_y.data_ptr(), x.data_ptr(), logits_dtype(x), row_stride(x), label_ptr(weight),
                                  pdt, f32(mean), f32(rstd), N, D, need_dx ? dx.data_ptr() : nullptr,
@@ -766,7 +766,7 @@ int chronicals_torch_bind(void* handle) {
   get(a.top_logits_workspace_bytes, "cce_top_logits_workspace_bytes");
   get(a.top_logits, "cce_top_logits");
   get(a.layer_norm_forward, "cce_layer_norm_forward");
-  get(a.layer_norm_backward_workspace_bytes, "cce_layer_norm_backward_workspace_bytes");
+  get(a.layer_norm_backward_workspace_bytes_for, "cce_layer_norm_backward_workspace_bytes_for");
   get(a.layer_norm_backward, "cce_layer_norm_backward");
   if (!ok) return 1;
   if (!g_bound.load(std::memory_order_acquire)) {

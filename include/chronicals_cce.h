@@ -43,7 +43,7 @@
 extern "C" {
 #endif
 
-#define CCE_ABI_VERSION 8
+#define CCE_ABI_VERSION 9
 
 #define CCE_OK 0
 #define CCE_ERR_INVALID_ARG 1
@@ -340,13 +340,16 @@ int cce_top_logits(const void* logits, int logits_dtype, int64_t ld, int64_t N, 
  * with fp32 statistics (mean_out, rstd_out [N]).  x has the row stride ldx, y_out
  * and the gradients are contiguous, of x's dtype; weight and bias (either may be
  * NULL) and their gradients are of param_dtype, which is x's or fp32.  The
- * backward leaves out the gradients whose pointer is NULL.  No reference
- * counterpart.
+ * backward leaves out the gradients whose pointer is NULL.  Its workspace is what
+ * the second query gives for its dtype and for whether grad_weight or grad_bias is
+ * wanted (0 bytes, which may be NULL, where neither is); what the first one gives
+ * is enough for every call of N and D.  No reference counterpart.
  */
 int cce_layer_norm_forward(const void* x, int dtype, int64_t ldx, const void* weight, const void* bias,
                            int param_dtype, int64_t N, int64_t D, float eps, void* y_out, float* mean_out,
                            float* rstd_out, void* stream);
 int cce_layer_norm_backward_workspace_bytes(int64_t N, int64_t D, size_t* bytes);
+int cce_layer_norm_backward_workspace_bytes_for(int64_t N, int64_t D, int dtype, int need_params, size_t* bytes);
 int cce_layer_norm_backward(const void* grad_y, const void* x, int dtype, int64_t ldx, const void* weight,
                             int param_dtype, const float* mean, const float* rstd, int64_t N, int64_t D, void* grad_x,
                             void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
