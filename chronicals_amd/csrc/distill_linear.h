@@ -29,7 +29,7 @@ __global__ __launch_bounds__(256) void kd_rows_kernel(Teacher a, int N, int V, i
 }
 
 // One workgroup per row: joins the vocabulary splits, takes the logits at the
-// row's columns (xk[n][j], j = K: the label) and forms its loss.  Bound by the
+// row's columns (xk[n][j], j = K: the label; 0 where there is none) and forms its loss.  Bound by the
 // weight's rows that the columns name: K = 64, 2048 x 896 43 us (5.4 TB/s, most of
 // it from the memory-side cache), 8192 x 4096 689 us (6.2 TB/s).
 // stats[n] = {log2-sum-exp2 at the temperature, at 1}.
@@ -57,6 +57,7 @@ __global__ __launch_bounds__(256) void kd_linear_loss_kernel(
       rowloss[n] = bsum[n] = 0.f;
       bcnt[n] = 0;
     }
+    for (int j = tid; j <= a.K; j += 256) xk[n * (a.K + 1) + j] = 0.f;
     return;
   }
   if (live) {  // as in fwd_combine_kernel
@@ -83,7 +84,10 @@ __global__ __launch_bounds__(256) void kd_linear_loss_kernel(
   const bf16_t* const h = H + n * (long)d;
   for (int j = tid >> 4; j <= a.K; j += 16) {
     const int c = j < a.K ? e.col[j] : label;
-    if (c < 0) continue;
+    if (c < 0) {
+      if ((tid & 15) == 0) xk[n * (a.K + 1) + j] = 0.f;
+      continue;
+    }
     const bf16_t* const wr = W + (long)c * d;
     float dot = 0.f;
     for (int k = (tid & 15) * 8; k < d; k += 128) {

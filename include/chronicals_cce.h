@@ -307,8 +307,9 @@ int cce_distill_logits_backward(const float* grad_out, const void* logits, int l
 /* Fused with the head's product, x = hidden . weight^T + bias, operands as
  * cce_forward's and cce_backward's (the rows of hidden that do not count are
  * finite: products run over them with zero coefficients).  The forward keeps for the backward
- * stats_out [N][2], entry_logits_out [N][entries + 1] and rows_out [N]; the
- * backward takes the same teacher, and no labels. */
+ * stats_out [N][2], entry_logits_out [N][entries + 1] (the logits at the entries'
+ * columns and, with ce_weight, at the label; 0 where there is none) and rows_out
+ * [N]; the backward takes the same teacher, and no labels. */
 int cce_distill_forward_workspace_bytes(int64_t N, int64_t d, int64_t V, int reduction, size_t* bytes);
 int cce_distill_forward(const void* hidden, const void* weight, const float* bias, const cce_teacher* teacher,
                         const void* labels, int labels_int64, int64_t N, int64_t d, int64_t V, int64_t ignore_index,
