@@ -3107,7 +3107,7 @@ const char* cce_last_error(void) { return g_err; }
 
 int cce_abi_version(void) { return CCE_ABI_VERSION; }
 
-// The build passes the SHA-256 of this file and the header as bare hex digits.
+// The build passes the SHA-256 of this file, its parts and the header as bare hex digits.
 #ifndef CCE_SOURCE_HASH
 #define CCE_SOURCE_HASH unknown
 #endif

@@ -459,10 +459,11 @@ bool norm_shape(long D, F&& f) {
   return true;
 }
 
-// The longest rows that stay in registers: 16 elements in each of 1024 threads.
-// Past that the kernels spill: with 18 registers in memory the forward of 1024 x
-// 20000 bf16 took 36 us, with 370 the backward 175, and by the kernels for longer
-// rows they take 100 and 134 to 152.
+// The longest rows that stay in registers, forward and backward: 16 elements in
+// each of 1024 threads, past which both spill.  It is the backward's limit: 1024 x
+// 20000 bf16 took 175 us with 370 registers in memory, and takes 134 to 152 by the
+// kernels for longer rows.  The forward has no limit of its own: with 18 registers
+// in memory it took 36 us there, and takes 98 by those kernels.
 constexpr int kNormRegD = 1024 * 16;
 
 // Threads of a row of D elements in registers; 256 for longer ones, whose parts

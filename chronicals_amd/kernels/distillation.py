@@ -31,7 +31,9 @@ so with ``ce_weight`` the labels' loss comes from the same passes.
   * K is at most 256, the temperature in [0.01, 1000].
   * Losses are fp32.  Sums are added in a fixed order: the same bits on every run.
   * Tensors must live on a HIP device; there is no CPU path.  The teacher's
-    tensors get no gradient, and gradients cannot be differentiated again.
+    tensors get no gradient.  Losses may be changed in place.  Differentiating a
+    gradient again raises an error, and so do function transforms
+    (``torch.func``, forward mode).
   * ``linear_distillation_loss`` computes in bf16 with fp32 accumulation (fp16 and
     fp32 operands are rounded to bf16 at the boundary) and rounds the gradient of
     the logits to bf16 once, as ``cut_cross_entropy`` does, in units that hold the

@@ -11,7 +11,8 @@ the parameters'.
   * x is bf16, fp16 or fp32 of any shape; rows may be strided (a last dimension
     that is not contiguous is copied).  weight and bias are [D], either or both,
     of x's dtype or fp32, both alike.
-  * Its gradients are kernels' results and cannot be differentiated again.
+  * The output may be changed in place.  Its gradients are kernels' results:
+    differentiating them again raises an error.
 
 The reference has no layer norm of its own; the models that it fine-tunes bring
 torch's.
