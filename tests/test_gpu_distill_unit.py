@@ -79,3 +79,24 @@ def test_factors_that_differ(gpu):
     off = (dh - up[:, None] * one).abs()
     assert (off[finite] <= (tol * up[:, None])[finite] * 1.01).all()
     assert not dh[3].any() and not dh[11].isfinite().any()
+
+
+@pytest.mark.parametrize("temperature", [1.0, 2.0, 3.0])
+@pytest.mark.parametrize("bias", [False, True])
+def test_rows_read_in_place(gpu, monkeypatch, temperature, bias):
+    """The recompute that reads the hidden rows through their order, in several bands and row blocks, with each form of
+    the epilogues."""
+    from tests.distill_common import labels, teacher
+    from tests.test_gpu_distillation import check_linear, head
+    g = torch.Generator().manual_seed(70)
+    N, d, V = 600, 64, 1200
+    h, w = head(g, N, d, V)
+    t, index = teacher(g, N, V, 16, 0.3)
+    lab = labels(g, N, V, 0.3)
+    monkeypatch.setenv("CHRONICALS_CCE_ROW_GATHER", "1")
+    monkeypatch.setenv("CHRONICALS_CCE_G_BUDGET_MB", "1")
+    b = torch.randn(V, generator=g) if bias else None
+    for ce in (0.0, 0.3):
+        for reduction in ("mean", "none"):
+            check_linear(gpu, h, w, t, index, lab, b, reduction, chunk_size=512, temperature=temperature,
+                         distill_weight=0.7, ce_weight=ce)
