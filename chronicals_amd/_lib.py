@@ -11,7 +11,7 @@ import threading
 from . import build as _build
 
 # constants mirrored from include/chronicals_cce.h
-CCE_ABI_VERSION = 9
+CCE_ABI_VERSION = 10
 CCE_OK = 0
 CCE_ERR_INVALID_ARG = 1
 CCE_ERR_WORKSPACE = 2
@@ -22,6 +22,8 @@ CCE_REDUCTION_SUM = 2
 CCE_DTYPE_BF16 = 0
 CCE_DTYPE_F32 = 1
 CCE_DTYPE_F16 = 2
+CCE_DTYPE_E4M3 = 3
+CCE_DTYPE_INT8 = 4
 CCE_SMOOTH_LOGV = 0
 CCE_SMOOTH_UNIFORM = 1
 CCE_LSE_ALL_ROWS = 0
@@ -155,6 +157,49 @@ SIGNATURES = {
         _vp, _vp, _i32, _i64, _vp, _i32,     # grad_y, x, dtype, ldx, weight, param_dtype
         _vp, _vp, _i64, _i64,                # mean, rstd, N, D
         _vp, _vp, _vp, _vp, _sz, _vp,        # grad_x, grad_weight, grad_bias, workspace, workspace_bytes, stream
+    ]),
+    "cce_token_logprobs_workspace_bytes": (_i32, [_i64, _i64, _i64, _size_out]),
+    "cce_token_logprobs_forward": (_i32, [
+        _vp, _i32, _i64, _vp, _i32,          # logits, dtype, ld, tokens, tokens_int64
+        _i64, _i64, _i64, _f32, _i64,        # N, V, ignore_index, temperature, top_k
+        _vp, _vp, _vp, _vp, _vp,             # logprobs_out, entropy_out, stats_out, top_logprobs_out, top_indices_out
+        _vp, _sz, _vp,                       # workspace, workspace_bytes, stream
+    ]),
+    "cce_token_logprobs_backward": (_i32, [
+        _vp, _vp, _vp, _i32, _i64, _vp, _i32,  # grad_logprobs, grad_entropy, logits, dtype, ld, tokens, tokens_int64
+        _vp, _i64, _i64, _i64, _f32,         # stats, N, V, ignore_index, temperature
+        _vp, _i64, _vp,                      # grad_logits, ld_grad, stream
+    ]),
+    "cce_linear_token_logprobs_workspace_bytes": (_i32, [_i64, _i64, _i64, _i64, _size_out]),
+    "cce_linear_token_logprobs_forward": (_i32, [
+        _vp, _vp, _vp, _vp, _i32,            # hidden, weight, bias, tokens, tokens_int64
+        _i64, _i64, _i64, _i64, _f32, _i64,  # N, d, V, ignore_index, temperature, top_k
+        _vp, _vp, _vp, _vp, _vp,             # logprobs_out, entropy_out, stats_out, top_logprobs_out, top_indices_out
+        _vp, _sz, _vp,                       # workspace, workspace_bytes, stream
+    ]),
+    "cce_linear_token_logprobs_backward_workspace_bytes": (_i32, [_i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32,
+                                                                  _size_out]),
+    "cce_linear_token_logprobs_backward": (_i32, [
+        _vp, _vp, _vp, _vp, _vp, _vp, _i32,  # grad_logprobs, grad_entropy, hidden, weight, bias, tokens, tokens_int64
+        _vp, _i64, _i64, _i64, _i64, _f32, _i64,  # stats, N, d, V, ignore_index, temperature, chunk_size
+        _vp, _i32, _vp, _i32, _vp,           # grad_hidden, dtype, grad_weight, dtype, grad_bias
+        _vp, _sz, _vp,                       # workspace, workspace_bytes, stream
+    ]),
+    "cce_rms_norm_forward": (_i32, [
+        _vp, _i32, _i64, _vp, _i32, _i64,    # x, dtype, ldx, residual, residual_dtype, ldr
+        _vp, _i32, _i64, _i64, _f32,         # weight, param_dtype, N, D, eps
+        _vp, _vp, _vp, _vp,                  # y_out, sum_out, rstd_out, stream
+    ]),
+    "cce_rms_norm_quantized": (_i32, [
+        _vp, _i32, _i64, _vp, _i32, _i64,    # x, dtype, ldx, residual, residual_dtype, ldr
+        _vp, _i32, _i64, _i64, _f32,         # weight, param_dtype, N, D, eps
+        _i32, _i64, _vp, _vp, _vp, _vp,      # q_dtype, group, q_out, scales_out, sum_out, stream
+    ]),
+    "cce_rms_norm_backward_workspace_bytes": (_i32, [_i64, _i64, _i32, _i32, _size_out]),
+    "cce_rms_norm_backward": (_i32, [
+        _vp, _vp, _vp, _i32, _i32, _i64,     # grad_y, grad_sum, sum, dtype, sum_dtype, ld_sum
+        _vp, _i32, _vp, _i64, _i64,          # weight, param_dtype, rstd, N, D
+        _vp, _vp, _vp, _vp, _sz, _vp,        # grad_x, grad_residual, grad_weight, workspace, workspace_bytes, stream
     ]),
     "cce_kernel_timing_enable": (_i32, [_i32]),
     "cce_kernel_timing_read": (_i32, [_i32, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(_i64),

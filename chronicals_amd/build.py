@@ -26,7 +26,8 @@ SRC = os.path.join(PKG_DIR, "csrc", "cce_kernels.hip")
 HEADER = os.path.join(REPO_DIR, "include", "chronicals_cce.h")
 # what SRC includes beside the header
 PARTS = tuple(os.path.join(PKG_DIR, "csrc", name)
-              for name in ("distill.h", "distill_linear.h", "layer_norm.h", "top_logits.h"))
+              for name in ("distill.h", "distill_linear.h", "layer_norm.h", "rms_norm.h", "token_logprobs.h",
+                           "token_logprobs_linear.h", "top_logits.h"))
 TORCH_SRC = os.path.join(PKG_DIR, "csrc", "torch_ops.cpp")
 LIB_DIR = os.path.join(PKG_DIR, "lib")
 LIB_NAME = "libchronicals_cce.so"

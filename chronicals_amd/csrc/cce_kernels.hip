@@ -388,7 +388,7 @@ struct LseParams {
   float* ps;          // [splits][ldp] sum of 2^(x - max)
   long ldp;           // row stride of pm / ps
   float scale;        // log2(e) over a temperature (not with kOneSoftmax)
-  float* ps1;         // kTwoSoftmaxes: the same sums in units of log2(e)
+  float* ps1;         // kTwoSoftmaxes: the same sums in units of log2(e); kEntropy: those of 2^(x - max) (x - max)
   int splits;
   int tiles_n;
 };
@@ -416,18 +416,26 @@ __host__ __device__ inline float split_cost(int gl, int tn, int s, int ncu) {
 // with either scale stay in range.  A backward of kCrossEntropy has one softmax
 // and the label's one-hot term, and its G has no unit; the others have no such
 // term and a unit (BwdLayout's).
-constexpr int kOneSoftmax = 0, kAtTemperature = 1, kTwoSoftmaxes = 2, kCrossEntropy = 3;
+//
+// kEntropy: one softmax at a temperature with the sum of 2^(x - m) (x - m) beside,
+// one more multiply-add per element, which gives the entropy (token_logprobs.h); its
+// backward has the one-hot term and a unit.  Its maximum starts at kLogitFloor, so
+// that differences of maxima stay finite.
+constexpr int kOneSoftmax = 0, kAtTemperature = 1, kTwoSoftmaxes = 2, kCrossEntropy = 3, kEntropy = 4;
 constexpr float kLogitFloor = -1e30f;
+// Below this exponent a power of two is 0 in fp32; products with it stay finite where
+// the exponent itself is -inf (masked columns).
+constexpr float kLeastExponent = -1000.f;
 
 template <int BN, bool HB, int SM = kOneSoftmax>
 struct EpiLseT {
-  static constexpr bool DU = SM == kTwoSoftmaxes;
+  static constexpr bool DU = SM == kTwoSoftmaxes, EN = SM == kEntropy;
   typedef LseParams Params;
   static constexpr bool kOneTile = false;
   static constexpr bool kDynSplits = true;
   static constexpr int FM = kFM;
   struct State {
-    float m[FM], s[FM], s1[DU ? FM : 1];
+    float m[FM], s[FM], s1[DU || EN ? FM : 1];
   };
   static __device__ inline void assign(const GemmShape& g, const Params& p, int bid, int nb, int& tm,
                                        int& t0, int& t1, int& split) {
@@ -446,9 +454,9 @@ struct EpiLseT {
   static __device__ inline void init(const Params&, State& st, const GemmShape&, int, int, int) {
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
-      st.m[i] = DU ? kLogitFloor : kNegBig;
+      st.m[i] = DU || EN ? kLogitFloor : kNegBig;
       st.s[i] = 0.f;
-      if constexpr (DU) st.s1[i] = 0.f;
+      if constexpr (DU || EN) st.s1[i] = 0.f;
     }
   }
   static __device__ __forceinline__ void tile(const Params& p, State& st, WaveAcc<BN>& acc, const GemmShape& g, int tm,
@@ -459,7 +467,8 @@ struct EpiLseT {
     const float scale = SM == kOneSoftmax ? kLog2e : p.scale;
     // max over raw logits (the scale > 0 commutes with max), then one fused
     // exp2(x*scale - m) per element and sum
-    auto update = [&](int i, const f32x16 (&x)[FN]) {
+    // MASKED: some elements may be -inf
+    auto update = [&](int i, const f32x16 (&x)[FN], auto MASKED) {
       float mx = kNegBig;
 #pragma unroll
       for (int j = 0; j < FN; ++j)
@@ -482,6 +491,20 @@ struct EpiLseT {
         return;
       }
       const float mn = fmaxf(st.m[i], mx * scale);
+      if constexpr (EN) {
+        float sum = 0.f, sum1 = 0.f;
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float u = __builtin_fmaf(x[j][r], scale, -mn), e = fast_exp2(u);
+            sum += e;
+            sum1 = __builtin_fmaf(e, decltype(MASKED)::value ? fmaxf(u, kLeastExponent) : u, sum1);
+          }
+        merge_entropy(st.m[i], st.s[i], st.s1[i], mn, sum, sum1);
+        __builtin_amdgcn_sched_barrier(0);
+        return;
+      }
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < FN; ++j)
@@ -497,7 +520,7 @@ struct EpiLseT {
         f32x16 x[FN];
 #pragma unroll
         for (int j = 0; j < FN; ++j) x[j] = acc.take(i, j);
-        update(i, x);
+        update(i, x, std::false_type{});
       }
       return;
     }
@@ -523,8 +546,16 @@ struct EpiLseT {
         asm volatile("" ::: "memory");  // one block's bias loads at a time
         __builtin_amdgcn_sched_barrier(0);
       }
-      update(i, x);
+      update(i, x, std::true_type{});
     }
+  }
+  // (m, s, w) with another partial (maxima in base 2 and from kLogitFloor up): where a
+  // maximum goes up to mn, w becomes r (w + (m - mn) s), r = 2^(m - mn)
+  static __device__ inline void merge_entropy(float& m, float& s, float& w, float m2, float s2, float w2) {
+    const float mn = fmaxf(m, m2), a = m - mn, b = m2 - mn, ra = fast_exp2(a), rb = fast_exp2(b);
+    w = ra * __builtin_fmaf(a, s, w) + rb * __builtin_fmaf(b, s2, w2);
+    s = s * ra + s2 * rb;
+    m = mn;
   }
   static __device__ inline void merge(float& m, float& s, float m2, float s2) {
     const float mn = fmaxf(m, m2);
@@ -538,6 +569,8 @@ struct EpiLseT {
       st.s[i] = st.s[i] * fast_exp2(a * p.scale) + s2 * fast_exp2(b * p.scale);
       st.s1[i] = st.s1[i] * fast_exp2(a * kLog2e) + s12 * fast_exp2(b * kLog2e);
       st.m[i] = mn;
+    } else if constexpr (EN) {
+      merge_entropy(st.m[i], st.s[i], st.s1[i], m2, s2, s12);
     } else {
       merge(st.m[i], st.s[i], m2, s2);
     }
@@ -547,7 +580,7 @@ struct EpiLseT {
     // lanes l and l+32 hold the same rows
 #pragma unroll
     for (int i = 0; i < FM; ++i)
-      merge_row(p, st, i, __shfl_xor(st.m[i], 32), __shfl_xor(st.s[i], 32), DU ? __shfl_xor(st.s1[DU ? i : 0], 32) : 0.f);
+      merge_row(p, st, i, __shfl_xor(st.m[i], 32), __shfl_xor(st.s[i], 32), DU || EN ? __shfl_xor(st.s1[DU || EN ? i : 0], 32) : 0.f);
     float* red = reinterpret_cast<float*>(smem);
     if (wn == 1 && l < 32) {
 #pragma unroll
@@ -555,7 +588,7 @@ struct EpiLseT {
         const int row = acc_row(wm, i, l);
         red[row] = st.m[i];
         red[kBM + row] = st.s[i];
-        if constexpr (DU) red[2 * kBM + row] = st.s1[i];
+        if constexpr (DU || EN) red[2 * kBM + row] = st.s1[i];
       }
     }
     __syncthreads();
@@ -563,13 +596,13 @@ struct EpiLseT {
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
         const int row = acc_row(wm, i, l);
-        merge_row(p, st, i, red[row], red[kBM + row], DU ? red[2 * kBM + row] : 0.f);
+        merge_row(p, st, i, red[row], red[kBM + row], DU || EN ? red[2 * kBM + row] : 0.f);
         const int grow = tm * kBM + row;
         if (grow < g.M) {
           const long ldp = g.dyn == kDynM ? (long)(g.M + kBM - 1) / kBM * kBM : p.ldp;
           p.pm[(long)split * ldp + grow] = st.m[i];
           p.ps[(long)split * ldp + grow] = st.s[i];
-          if constexpr (DU) p.ps1[(long)split * ldp + grow] = st.s1[i];
+          if constexpr (DU || EN) p.ps1[(long)split * ldp + grow] = st.s1[i];
         }
       }
     }
@@ -588,6 +621,10 @@ template <int BN>
 using EpiLseTwo = EpiLseT<BN, false, kTwoSoftmaxes>;
 template <int BN>
 using EpiLseBiasTwo = EpiLseT<BN, true, kTwoSoftmaxes>;
+template <int BN>
+using EpiLseEntropy = EpiLseT<BN, false, kEntropy>;
+template <int BN>
+using EpiLseBiasEntropy = EpiLseT<BN, true, kEntropy>;
 
 struct GradParams {
   const float* bias;     // [V] or null (full vocabulary, indexed by v0 + c)
@@ -604,6 +641,8 @@ struct GradParams {
 // rowp[n] = {lse2, cP, cT, cU}: g = cP*2^(x*scale - lse2) - cU - cT*[c == label].
 // kTwoSoftmaxes (no label then): rowp[n] = {lse2, cP, cA, lse2_1}:
 // g = cP*2^(x*scale - lse2) + cA*2^(x*log2e - lse2_1).
+// kEntropy: rowp[n] = {lse2, c, cT, b}: g = 2^y*(c + b*y) - cT*[c == label],
+// y = x*scale - lse2.
 //
 // Stores go through LDS: in the MFMA layout a lane holds one row, so a direct
 // store instruction would touch 32 rows with 16 bytes each.  Each wave writes
@@ -613,7 +652,7 @@ struct GradParams {
 // A wave's LDS operations execute in order, so no barrier is needed.
 template <int BN, bool HB, int SM = kCrossEntropy>
 struct EpiGradT {
-  static constexpr bool DU = SM == kTwoSoftmaxes;
+  static constexpr bool DU = SM == kTwoSoftmaxes, EN = SM == kEntropy;
   typedef GradParams Params;
   static constexpr bool kOneTile = true;  // splits == tiles_n: a workgroup takes one column tile
   static constexpr bool kDynSplits = false;
@@ -627,6 +666,10 @@ struct EpiGradT {
     const int gm = (g.M + kBM - 1) / kBM;
     grouped_map(bid, nb, gm, p.tiles_n, tm, t0);
     split = 0;
+  }
+  // without a bias no logit is -inf
+  static __device__ inline float entropy_grad(const float4& rp, float y) {
+    return fast_exp2(y) * __builtin_fmaf(rp.w, HB ? fmaxf(y, kLeastExponent) : y, rp.y);
   }
   static __device__ inline void row_params(const Params& p, const GemmShape& g, int m, float4& rp, int& lab) {
     const int mc = m < g.M ? m : 0;
@@ -672,7 +715,11 @@ struct EpiGradT {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float xe = HB ? x[j][4 * q + e] + bv[e] : x[j][4 * q + e];
-            float gg = __builtin_fmaf(rp.y, fast_exp2(__builtin_fmaf(xe, scale, -rp.x)), DU ? 0.f : -rp.w);
+            float gg;
+            if constexpr (EN)
+              gg = entropy_grad(rp, __builtin_fmaf(xe, scale, -rp.x));
+            else
+              gg = __builtin_fmaf(rp.y, fast_exp2(__builtin_fmaf(xe, scale, -rp.x)), DU ? 0.f : -rp.w);
             if constexpr (DU) gg = __builtin_fmaf(rp.z, fast_exp2(__builtin_fmaf(xe, kLog2e, -rp.w)), gg);
             gv[e] = decltype(INTERIOR)::value || cb + e < g.N ? gg : 0.f;
           }
@@ -714,7 +761,8 @@ struct EpiGradT {
         for (int k = 0; k < n; ++k) v[k] = at & bit ? v[2 * k + 1] : v[2 * k];
       if (mine) {
         const float xe = HB ? v[0] + p.bias[p.v0 + lab] : v[0];
-        const float gg = __builtin_fmaf(rp.y, fast_exp2(__builtin_fmaf(xe, scale, -rp.x)), -rp.w) - rp.z;
+        const float y = __builtin_fmaf(xe, scale, -rp.x);
+        const float gg = (EN ? entropy_grad(rp, y) : __builtin_fmaf(rp.y, fast_exp2(y), -rp.w)) - rp.z;
         bf16_t* const t = ws + (i & 1) * kArea + r * 64 + (lc >> 6) * 2048 +
                           ((((int)(lc & 63) >> 2) ^ (r & 15)) << 2) + (lc & 3);
         *t = __builtin_bit_cast(bf16_t, (__bf16)gg);
@@ -752,7 +800,7 @@ struct EpiGradT {
         stage(i, rp, std::true_type{});
       else
         stage(i, rp, std::false_type{});
-      if constexpr (SM == kCrossEntropy) one_hot(i, rp, lab);
+      if constexpr (SM == kCrossEntropy || EN) one_hot(i, rp, lab);
       if (i > 0) store(i - 1);
       rp = rp1;
       lab = lab1;
@@ -1117,6 +1165,64 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
 // 2 acc += s, 3 out = acc + s, 4 out += s (fp32 out); out rows go through the
 // row map.  The rows are a block starting at row live_base of the compacted
 // order (P, acc and rowmap point at the block).
+// A block of logits in fp32: out = C, with HB plus the columns' bias.  The output's
+// rows hold whole fours of columns (ldo a multiple of 4, N or more); those past N get
+// numbers of no meaning.  Stored in whole rows of a wave's columns, as EpiAccT's.
+struct OutParams {
+  float* out;
+  long ldo;
+  const float* bias;  // [N]
+};
+template <int BN, bool HB>
+struct EpiOutT : EpiAccT<BN, false> {
+  typedef EpiAccT<BN, false> Base;
+  typedef OutParams Params;
+  using Base::FM, Base::kC, Base::kL, Base::kPitch;
+  typedef typename Base::State State;
+  static __device__ inline void assign(const GemmShape& g, const Params&, int bid, int nb, int& tm, int& t0, int& t1,
+                                       int& split) {
+    Base::assign(g, AccParams(), bid, nb, tm, t0, t1, split);
+  }
+  static __device__ inline void init(const Params&, State&, const GemmShape&, int, int, int) {}
+  static __device__ __forceinline__ void tile(const Params& p, State&, WaveAcc<BN>& acc, const GemmShape& g, int tm,
+                                              int tn, int wm, int wn, int l, bf16_t* scratch) {
+    pin_epilogue(l, tm, tn);
+    constexpr int kR = 64 / kL, kT = 32 / kR;  // rows per instruction, instructions
+    float* const ws = reinterpret_cast<float*>(scratch) + (wm * 2 + wn) * 32 * kPitch;
+    const int n0 = tn * BN + wn * kC, rr = l / kL, c = (l % kL) * 4;
+    f32x4 b = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (HB) b = load4(make_rsrc(p.bias + n0, max(g.N - n0, 0) * 4L), c * 4);
+#pragma unroll 1
+    for (int i = 0; i < FM; ++i) {
+      const int m0 = tm * kBM + acc_row(wm, i, 0);
+      if (m0 >= g.M) break;
+      f32x16 x[BN / 64];
+      acc.take_row(i, x);
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int j = 0; j < BN / 64; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<f32x4*>(ws + (l & 31) * kPitch + j * 32 + q * 8 + (l >> 5) * 4) =
+              f32x4{x[j][4 * q], x[j][4 * q + 1], x[j][4 * q + 2], x[j][4 * q + 3]};
+      asm volatile("" ::: "memory");
+      float* const out = p.out + (long)(m0 + rr) * p.ldo + n0 + c;
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+        f32x4 v = *reinterpret_cast<const f32x4*>(ws + (t * kR + rr) * kPitch + c);
+        if constexpr (HB) v += b;
+        if (n0 + c < g.N && m0 + t * kR + rr < g.M) *reinterpret_cast<f32x4*>(out + (long)t * kR * p.ldo) = v;
+      }
+      asm volatile("" ::: "memory");
+    }
+  }
+  static __device__ inline void finish(const Params&, State&, const GemmShape&, int, int, bf16_t*, int, int, int) {}
+};
+template <int BN>
+using EpiOut = EpiOutT<BN, false>;
+template <int BN>
+using EpiOutBias = EpiOutT<BN, true>;
+
 struct DhReduce {
   const float* P;
   long stride;
@@ -2304,7 +2410,7 @@ struct BwdLayout {
   // null when unsplit
   float* dhpart;
   int dh_ks;
-  // SparseGrad's columns and values, and the unit of G
+  // SparseGrad's columns and values, and the unit of G (without a SparseGrad: none)
   int* col;
   float* val;
   float* unit;
@@ -2341,7 +2447,7 @@ int dh_splits(long N, long d, long Vb) {
 long ht_cols(long N) { return (long)align_up((size_t)N, kBK); }
 
 BwdLayout bwd_layout(void* ws, long N, long d, long V, long Vb, bool need_dh, bool need_dw, bool dh_f32,
-                     bool dw_f32, int entries = 0) {
+                     bool dw_f32, int entries = -1) {  // a SparseGrad's; -1: none
   Carver c(ws);
   BwdLayout L;
   L.N = N;
@@ -2373,9 +2479,9 @@ BwdLayout bwd_layout(void* ws, long N, long d, long V, long Vb, bool need_dh, bo
   // band launch writes the one buffer again
   L.dhpart = L.dh_ks > 1 ? c.take<float>((size_t)(dh_fold(L.dh_ks) && units > 1 ? 2 : 1) * L.dh_ks * L.Nb * d)
                          : nullptr;
-  L.col = entries ? c.take<int>((size_t)N * entries) : nullptr;
-  L.val = entries ? c.take<float>((size_t)N * entries) : nullptr;
-  L.unit = entries ? c.take<float>(1) : nullptr;
+  L.col = entries > 0 ? c.take<int>((size_t)N * entries) : nullptr;
+  L.val = entries > 0 ? c.take<float>((size_t)N * entries) : nullptr;
+  L.unit = entries >= 0 ? c.take<float>(1) : nullptr;
   L.bytes = align_up(c.off, 256);
   return L;
 }
@@ -2561,6 +2667,7 @@ int launch_band(const BandLaunch& p, bool has_bias, hipStream_t st, int kind = C
   auto* const kernel = softmaxes == kCrossEntropy    ? pick_band<kCrossEntropy>(has_bias, arow, ktail)
                        : softmaxes == kOneSoftmax    ? pick_band<kOneSoftmax>(has_bias, arow, ktail)
                        : softmaxes == kAtTemperature ? pick_band<kAtTemperature>(has_bias, arow, ktail)
+                       : softmaxes == kEntropy       ? pick_band<kEntropy>(has_bias, arow, ktail)
                                                      : pick_band<kTwoSoftmaxes>(has_bias, arow, ktail);
   hipLaunchKernelGGL(kernel, dim3(nb), dim3(kThreads), 0, st, p);
   HIP_TRY(hipGetLastError());
@@ -2621,6 +2728,40 @@ int launch_lse(const GemmShape& g, const LseParams& ep, int slots, hipStream_t s
   return launch_gemm<kBN, Epi>(g, ep, slots, st, kKind, true);
 }
 
+// The row order of a compacted forward (the labels' rows first, the vocabulary split
+// over `slots` workgroups), and H in that order where it is copied.
+int order_rows(const void* labels, int labels_int64, long ignore_index, const bf16_t* H, long N, long d, long V,
+               int slots, const FwdLayout& L, hipStream_t st) {
+  if (!L.idx) return CCE_OK;
+  hipLaunchKernelGGL(compact_rows_kernel, dim3(1), dim3(1024), 0, st, labels, labels_int64, (int)N, ignore_index, L.idx,
+                     L.live, slots, (int)ceil_div(V, kBN), device_cus());
+  HIP_TRY(hipGetLastError());
+  if (!L.Hc) return CCE_OK;
+  hipLaunchKernelGGL(gather_rows_kernel, dim3((unsigned)std::min<long>(ceil_div(N * (d / 8), 256), 8192)), dim3(256), 0,
+                     st, H, (int)d, L.idx, (int)N, L.Hc);
+  HIP_TRY(hipGetLastError());
+  return CCE_OK;
+}
+
+// The forward's product over the rows of that order, or over all as they are.
+GemmShape forward_shape(const bf16_t* H, const bf16_t* W, long N, long d, long V, const FwdLayout& L) {
+  GemmShape g;
+  g.A = L.Hc ? L.Hc : H;
+  if (L.idx && !L.Hc) {
+    g.arow = L.idx;
+    g.arows = N;
+  }
+  g.lda = d;
+  g.B = W;
+  g.ldb = d;
+  g.M = (int)N;
+  g.N = (int)V;
+  g.K = (int)d;
+  g.live = L.live;
+  g.dyn = L.live ? kDynM : kDynNone;
+  return g;
+}
+
 int forward_run(const void* hidden, const void* weight, const void* labels, int labels_int64, const float* bias,
                 int64_t N, int64_t d, int64_t V, int64_t ignore_index, float label_smoothing, float z_loss_weight,
                 int smoothing_form, int reduction, int lse_rows, float* loss_out, float* lse_out, float* target_out,
@@ -2658,32 +2799,10 @@ int forward_run(const void* hidden, const void* weight, const void* labels, int 
 
   // CCE_LSE_LABELLED_ROWS: the labelled rows go first and the GEMM runs only
   // over the row tiles that hold them (the partials then follow that order)
-  if (L.idx) {
-    hipLaunchKernelGGL(compact_rows_kernel, dim3(1), dim3(1024), 0, st, labels, labels_int64, (int)N,
-                       (long)ignore_index, L.idx, L.live, slots, (int)ceil_div(V, kBN), device_cus());
-    HIP_TRY(hipGetLastError());
-    if (L.Hc) {
-      const long chunks = (long)N * (d / 8);
-      hipLaunchKernelGGL(gather_rows_kernel, dim3((unsigned)std::min<long>(ceil_div(chunks, 256), 8192)), dim3(256),
-                         0, st, static_cast<const bf16_t*>(hidden), (int)d, L.idx, (int)N, L.Hc);
-      HIP_TRY(hipGetLastError());
-    }
-  }
-
-  GemmShape g;
-  g.A = L.Hc ? L.Hc : static_cast<const bf16_t*>(hidden);
-  if (L.idx && !L.Hc) {
-    g.arow = L.idx;
-    g.arows = N;
-  }
-  g.lda = d;
-  g.B = static_cast<const bf16_t*>(weight);
-  g.ldb = d;
-  g.M = (int)N;
-  g.N = (int)V;
-  g.K = (int)d;
-  g.live = L.live;
-  g.dyn = L.live ? kDynM : kDynNone;
+  const bf16_t* const H = static_cast<const bf16_t*>(hidden);
+  rc = order_rows(labels, labels_int64, (long)ignore_index, H, N, d, V, slots, L, st);
+  if (rc) return rc;
+  const GemmShape g = forward_shape(H, static_cast<const bf16_t*>(weight), N, d, V, L);
   LseParams ep;
   ep.bias = bias;
   ep.pm = L.pm;
@@ -2721,11 +2840,11 @@ int forward_run(const void* hidden, const void* weight, const void* labels, int 
 }
 
 // Row coefficients and sparse columns of a gradient that is not the
-// cross-entropy's (distillation), in place of bwd_prep_kernel.
+// cross-entropy's (distillation, token log-probabilities), in place of bwd_prep_kernel.
 struct SparseGrad {
   float scale;  // GradParams
   int softmaxes;  // EpiGradT
-  int entries;  // columns per row
+  int entries;  // columns per row; 0: none, the epilogue's one-hot term has them
   // rowp and rowlab of the N rows in the GEMM's order (idx; null: as they are),
   // their columns ([N][entries], -1: none) and the values of G there, all in
   // units of *unit, which multiplies the products with G
@@ -2773,7 +2892,7 @@ int backward_run(const float* grad_out, const void* hidden, const void* weight, 
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const bool dh_f32 = grad_hidden_dtype == CCE_DTYPE_F32, dw_f32 = grad_weight_dtype == CCE_DTYPE_F32;
   const long Vb = band_width(V, chunk_size, N);
-  const int entries = sparse ? sparse->entries : 0;
+  const int entries = sparse ? sparse->entries : -1;
   const BwdLayout need = bwd_layout(nullptr, N, d, V, Vb, need_dh, need_dw, dh_f32, dw_f32, entries);
   if (workspace_bytes < need.bytes || (need.bytes && !workspace))
     return fail(CCE_ERR_WORKSPACE, "workspace too small: need %zu bytes, got %zu", need.bytes, workspace_bytes);
@@ -2916,7 +3035,7 @@ int backward_run(const float* grad_out, const void* hidden, const void* weight, 
 
   // the sparse columns of unit u over its dense gradient
   auto sparse_unit = [&](long u) -> int {
-    if (!sparse) return CCE_OK;
+    if (entries <= 0) return CCE_OK;
     long v0, vb, m0, rows;
     band_cols(u / R, v0, vb);
     block_span(u % R, m0, rows);
@@ -3094,6 +3213,9 @@ int noalloc_scratch(void** out) {
 #include "top_logits.h"
 #include "distill.h"
 #include "distill_linear.h"
+#include "token_logprobs.h"
+#include "token_logprobs_linear.h"
+#include "rms_norm.h"
 
 }  // namespace
 
@@ -3586,6 +3708,208 @@ int cce_layer_norm_backward(const void* grad_y, const void* x, int dtype, int64_
     return fail(CCE_ERR_WORKSPACE, "workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
   return norm_backward(grad_y, x, dtype, ldx, weight, param_dtype, mean, rstd, N, D, grad_x, grad_weight, grad_bias,
                        workspace, reinterpret_cast<hipStream_t>(stream));
+}
+
+int cce_token_logprobs_workspace_bytes(int64_t N, int64_t V, int64_t top_k, size_t* bytes) {
+  g_err[0] = 0;
+  if (!bytes) return fail(CCE_ERR_INVALID_ARG, "bytes must not be null");
+  int rc = check_logits_args(N, V, CCE_DTYPE_F32, V, CCE_REDUCTION_NONE, 0.f, CCE_SMOOTH_LOGV);
+  if (!rc) rc = check_alternatives(top_k, V, 0, nullptr, nullptr);
+  if (rc) return rc;
+  *bytes = lp_layout(nullptr, N, V, top_k).bytes;
+  return CCE_OK;
+}
+
+int cce_token_logprobs_forward(const void* logits, int logits_dtype, int64_t ld, const void* tokens, int tokens_int64,
+                               int64_t N, int64_t V, int64_t ignore_index, float temperature, int64_t top_k,
+                               float* logprobs_out, float* entropy_out, float* stats_out, float* top_logprobs_out,
+                               int64_t* top_indices_out, void* workspace, size_t workspace_bytes, void* stream) {
+  g_err[0] = 0;
+  int rc = check_logits_args(N, V, logits_dtype, ld, CCE_REDUCTION_NONE, 0.f, CCE_SMOOTH_LOGV);
+  Tokens a;
+  if (!rc) rc = check_tokens(tokens, tokens_int64, N, ignore_index, temperature, a);
+  if (!rc) rc = check_alternatives(top_k, V, N, top_logprobs_out, top_indices_out);
+  if (rc) return rc;
+  if (N == 0) return CCE_OK;
+  if (!logits || !logprobs_out || !entropy_out || !stats_out)
+    return fail(CCE_ERR_INVALID_ARG, "logits, logprobs_out, entropy_out and stats_out must not be null");
+  if (misaligned(stats_out) || misaligned(workspace))
+    return fail(CCE_ERR_INVALID_ARG, "stats_out and workspace must be 16-byte aligned");
+  const size_t need = lp_layout(nullptr, N, V, top_k).bytes;
+  if (workspace_bytes < need || (need && !workspace))
+    return fail(CCE_ERR_WORKSPACE, "workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+  const LpOut out = {logprobs_out,    entropy_out, reinterpret_cast<float4*>(stats_out), 1.f, top_logprobs_out,
+                     top_indices_out};
+  return logits_type(logits_dtype, [&](auto t) {
+    return lp_forward_run(static_cast<const decltype(t)*>(logits), (long)ld, (long)N, (long)V, (long)top_k, a, nullptr,
+                          out, lp_layout(workspace, N, V, top_k), reinterpret_cast<hipStream_t>(stream));
+  });
+}
+
+int cce_token_logprobs_backward(const float* grad_logprobs, const float* grad_entropy, const void* logits,
+                                int logits_dtype, int64_t ld, const void* tokens, int tokens_int64, const float* stats,
+                                int64_t N, int64_t V, int64_t ignore_index, float temperature, void* grad_logits,
+                                int64_t ld_grad, void* stream) {
+  g_err[0] = 0;
+  int rc = check_logits_args(N, V, logits_dtype, ld, CCE_REDUCTION_NONE, 0.f, CCE_SMOOTH_LOGV);
+  Tokens a;
+  if (!rc) rc = check_tokens(tokens, tokens_int64, N, ignore_index, temperature, a);
+  if (rc) return rc;
+  if (ld_grad < V)
+    return fail(CCE_ERR_INVALID_ARG, "gradient row stride %ld is smaller than V = %ld", (long)ld_grad, (long)V);
+  if (N == 0) return CCE_OK;
+  if (!logits || !stats || !grad_logits)
+    return fail(CCE_ERR_INVALID_ARG, "logits, stats and grad_logits must not be null");
+  if (grad_logits == logits) return fail(CCE_ERR_INVALID_ARG, "grad_logits must not be the logits");
+  if (misaligned(stats)) return fail(CCE_ERR_INVALID_ARG, "stats must be 16-byte aligned");
+  const LpGrad p = {grad_logprobs, grad_entropy, a.inv_t};
+  const int S = kd_splits(N, V);
+  return logits_type(logits_dtype, [&](auto t) {
+    typedef decltype(t) T;
+    hipLaunchKernelGGL(lp_grad_kernel<T>, dim3((unsigned)(N * S)), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), p,
+                       static_cast<const T*>(logits), (long)ld, (int)V, S, a, reinterpret_cast<const float4*>(stats),
+                       static_cast<T*>(grad_logits), (long)ld_grad);
+    HIP_TRY(hipGetLastError());
+    return CCE_OK;
+  });
+}
+
+int cce_linear_token_logprobs_workspace_bytes(int64_t N, int64_t d, int64_t V, int64_t top_k, size_t* bytes) {
+  g_err[0] = 0;
+  if (!bytes) return fail(CCE_ERR_INVALID_ARG, "bytes must not be null");
+  int rc = check_dims(N, d, V);
+  if (!rc) rc = check_alternatives(top_k, V, 0, nullptr, nullptr);
+  if (rc) return rc;
+  *bytes = lp_linear_layout(nullptr, N, d, V, top_k).bytes;
+  return CCE_OK;
+}
+
+int cce_linear_token_logprobs_forward(const void* hidden, const void* weight, const float* bias, const void* tokens,
+                                      int tokens_int64, int64_t N, int64_t d, int64_t V, int64_t ignore_index,
+                                      float temperature, int64_t top_k, float* logprobs_out, float* entropy_out,
+                                      float* stats_out, float* top_logprobs_out, int64_t* top_indices_out,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
+  g_err[0] = 0;
+  int rc = check_dims(N, d, V);
+  Tokens a;
+  if (!rc) rc = check_tokens(tokens, tokens_int64, N, ignore_index, temperature, a);
+  if (!rc) rc = check_alternatives(top_k, V, N, top_logprobs_out, top_indices_out);
+  if (rc) return rc;
+  if (N == 0) return CCE_OK;
+  if (!hidden || !weight || !logprobs_out || !entropy_out || !stats_out)
+    return fail(CCE_ERR_INVALID_ARG, "hidden, weight, logprobs_out, entropy_out and stats_out must not be null");
+  if (misaligned(hidden) || misaligned(weight) || misaligned(stats_out) || misaligned(workspace))
+    return fail(CCE_ERR_INVALID_ARG, "hidden, weight, stats_out and workspace must be 16-byte aligned");
+  const size_t need = lp_linear_layout(nullptr, N, d, V, top_k).bytes;
+  if (workspace_bytes < need || !workspace)
+    return fail(CCE_ERR_WORKSPACE, "workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+  const LpOut out = {logprobs_out,    entropy_out, reinterpret_cast<float4*>(stats_out), 1.f, top_logprobs_out,
+                     top_indices_out};
+  return lp_linear_forward_run(static_cast<const bf16_t*>(hidden), static_cast<const bf16_t*>(weight), bias, (long)N,
+                               (long)d, (long)V, (long)top_k, a, out, lp_linear_layout(workspace, N, d, V, top_k),
+                               reinterpret_cast<hipStream_t>(stream));
+}
+
+int cce_linear_token_logprobs_backward_workspace_bytes(int64_t N, int64_t d, int64_t V, int64_t chunk_size,
+                                                       int need_grad_hidden, int grad_hidden_dtype,
+                                                       int need_grad_weight, int grad_weight_dtype, size_t* bytes) {
+  const int rc = cce_backward_workspace_bytes(N, d, V, chunk_size, need_grad_hidden, grad_hidden_dtype,
+                                              need_grad_weight, grad_weight_dtype, bytes);
+  if (rc) return rc;
+  *bytes = bwd_layout(nullptr, N, d, V, band_width(V, chunk_size, N), need_grad_hidden != 0, need_grad_weight != 0,
+                      grad_hidden_dtype == CCE_DTYPE_F32, grad_weight_dtype == CCE_DTYPE_F32, 0).bytes;
+  return CCE_OK;
+}
+
+int cce_linear_token_logprobs_backward(const float* grad_logprobs, const float* grad_entropy, const void* hidden,
+                                       const void* weight, const float* bias, const void* tokens, int tokens_int64,
+                                       const float* stats, int64_t N, int64_t d, int64_t V, int64_t ignore_index,
+                                       float temperature, int64_t chunk_size, void* grad_hidden, int grad_hidden_dtype,
+                                       void* grad_weight, int grad_weight_dtype, float* grad_bias, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+  g_err[0] = 0;
+  LpLinearGrad q;
+  const int rc = check_tokens(tokens, tokens_int64, N, ignore_index, temperature, q.a);
+  if (rc) return rc;
+  if (N > 0 && !stats) return fail(CCE_ERR_INVALID_ARG, "stats must not be null");
+  if (misaligned(stats)) return fail(CCE_ERR_INVALID_ARG, "stats must be 16-byte aligned");
+  if (V > INT_MAX) return check_dims(N, d, V);
+  q.p = {grad_logprobs, grad_entropy, q.a.inv_t};
+  q.stats = reinterpret_cast<const float4*>(stats);
+  q.V = (int)V;
+  SparseGrad s;
+  s.scale = q.a.scale;
+  s.softmaxes = kEntropy;
+  s.entries = 0;
+  s.prep = lp_prep;
+  s.args = &q;
+  // stats stands for the cross-entropy's gradient, lse and count, which the prep above replaces
+  return backward_run(stats, hidden, weight, tokens, tokens_int64, bias, stats, reinterpret_cast<const int32_t*>(stats),
+                      N, d, V, ignore_index, 0.f, 0.f, CCE_REDUCTION_NONE, chunk_size, grad_hidden, grad_hidden_dtype,
+                      grad_weight, grad_weight_dtype, grad_bias, workspace, workspace_bytes, stream, &s);
+}
+
+int cce_rms_norm_forward(const void* x, int dtype, int64_t ldx, const void* residual, int residual_dtype, int64_t ldr,
+                         const void* weight, int param_dtype, int64_t N, int64_t D, float eps, void* y_out, void* sum_out,
+                         float* rstd_out, void* stream) {
+  g_err[0] = 0;
+  const int rc = check_rms(N, D, dtype, ldx, residual_dtype, ldr, param_dtype, eps);
+  if (rc) return rc;
+  if (N == 0) return CCE_OK;
+  if (!x || !y_out || !rstd_out || (residual && !sum_out))
+    return fail(CCE_ERR_INVALID_ARG, "x, y_out, rstd_out and (with a residual) sum_out must not be null");
+  return rms_forward<false>(x, dtype, ldx, residual, residual_dtype, ldr, weight, param_dtype, N, D, eps, y_out, sum_out,
+                            rstd_out, RmsQuant(), reinterpret_cast<hipStream_t>(stream));
+}
+
+int cce_rms_norm_quantized(const void* x, int dtype, int64_t ldx, const void* residual, int residual_dtype, int64_t ldr,
+                           const void* weight, int param_dtype, int64_t N, int64_t D, float eps, int q_dtype,
+                           int64_t group, void* q_out, float* scales_out, void* sum_out, void* stream) {
+  g_err[0] = 0;
+  const int rc = check_rms(N, D, dtype, ldx, residual_dtype, ldr, param_dtype, eps);
+  if (rc) return rc;
+  if (q_dtype != CCE_DTYPE_E4M3 && q_dtype != CCE_DTYPE_INT8)
+    return fail(CCE_ERR_INVALID_ARG, "q_dtype must be CCE_DTYPE_E4M3 or CCE_DTYPE_INT8, got %d", q_dtype);
+  if (group != 0 && group != 32 && group != 64 && group != 128 && group != 256)
+    return fail(CCE_ERR_INVALID_ARG, "group must be 0 (a row), 32, 64, 128 or 256, got %ld", (long)group);
+  if (N == 0) return CCE_OK;
+  if (!x || !q_out || !scales_out || (residual && !sum_out))
+    return fail(CCE_ERR_INVALID_ARG, "x, q_out, scales_out and (with a residual) sum_out must not be null");
+  RmsQuant o;
+  o.q = static_cast<uint8_t*>(q_out);
+  o.scales = scales_out;
+  o.group = (int)group;
+  o.shift = group ? __builtin_ctz((unsigned)group) : 0;
+  o.groups = group ? (int)ceil_div(D, group) : 1;
+  o.int8 = q_dtype == CCE_DTYPE_INT8;
+  return rms_forward<true>(x, dtype, ldx, residual, residual_dtype, ldr, weight, param_dtype, N, D, eps, nullptr, sum_out,
+                           nullptr, o, reinterpret_cast<hipStream_t>(stream));
+}
+
+int cce_rms_norm_backward_workspace_bytes(int64_t N, int64_t D, int dtype, int need_grad_weight, size_t* bytes) {
+  g_err[0] = 0;
+  if (!bytes) return fail(CCE_ERR_INVALID_ARG, "bytes must not be null");
+  const int rc = check_norm(N, D, dtype, D, CCE_DTYPE_F32);
+  if (rc) return rc;
+  *bytes = rms_bytes(dtype, N, D, need_grad_weight != 0);
+  return CCE_OK;
+}
+
+int cce_rms_norm_backward(const void* grad_y, const void* grad_sum, const void* sum, int dtype, int sum_dtype,
+                          int64_t ld_sum, const void* weight, int param_dtype, const float* rstd, int64_t N, int64_t D,
+                          void* grad_x, void* grad_residual, void* grad_weight, void* workspace, size_t workspace_bytes,
+                          void* stream) {
+  g_err[0] = 0;
+  const int rc = check_rms(N, D, dtype, D, sum_dtype, ld_sum, param_dtype, 0.f);
+  if (rc) return rc;
+  if (N > 0 && (!grad_y || !sum || !rstd))
+    return fail(CCE_ERR_INVALID_ARG, "grad_y, sum and rstd must not be null");
+  if (misaligned(workspace)) return fail(CCE_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
+  const size_t need = rms_bytes(dtype, N, D, grad_weight != nullptr);
+  if (workspace_bytes < need || (need && !workspace))
+    return fail(CCE_ERR_WORKSPACE, "workspace too small: need %zu bytes, got %zu", need, workspace_bytes);
+  return rms_backward(grad_y, grad_sum, sum, dtype, sum_dtype, ld_sum, weight, param_dtype, rstd, N, D, grad_x,
+                      grad_residual, grad_weight, static_cast<float*>(workspace), reinterpret_cast<hipStream_t>(stream));
 }
 
 int cce_kernel_timing_enable(int enable) {

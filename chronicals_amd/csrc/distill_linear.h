@@ -139,24 +139,29 @@ struct DistillGrad {
 __device__ inline float mantissa(float x) { return __uint_as_float((__float_as_uint(x) & 0x007fffffu) | 0x3f800000u); }
 __device__ inline float unit_of(const Teacher& a, float g) { return mantissa(g * (a.ce != 0.f ? a.ce : a.kdg)); }
 
-// *unit where every row has a factor of its own: the largest finite one's, which
-// all have where a mean or a masked mean of the rows follows.  One workgroup, bound
-// by latency: 5 us for 2048 rows, 10 for 16384.
-__global__ __launch_bounds__(1024) void kd_unit_kernel(Teacher a, const float* __restrict__ grad_out, int N,
-                                                       float* __restrict__ unit) {
+// The largest finite magnitude of v[0, N), by a workgroup of 1024; thread 0 gets it.
+__device__ inline float largest_finite(const float* __restrict__ v, int N) {
   __shared__ float red[16];
   float g = 0.f;
   for (int n = threadIdx.x; n < N; n += 1024) {
-    const float v = fabsf(grad_out[n]);
-    if (v < INFINITY) g = fmaxf(g, v);
+    const float x = fabsf(v[n]);
+    if (x < INFINITY) g = fmaxf(g, x);
   }
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) g = fmaxf(g, __shfl_xor(g, o));
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = g;
   __syncthreads();
-  if (threadIdx.x != 0) return;
-  for (int w = 1; w < 16; ++w) g = fmaxf(g, red[w]);
-  *unit = unit_of(a, g);
+  for (int w = 0; w < 16; ++w) g = fmaxf(g, red[w]);
+  return g;
+}
+
+// *unit where every row has a factor of its own: the largest finite one's, which
+// all have where a mean or a masked mean of the rows follows.  One workgroup, bound
+// by latency: 5 us for 2048 rows, 10 for 16384.
+__global__ __launch_bounds__(1024) void kd_unit_kernel(Teacher a, const float* __restrict__ grad_out, int N,
+                                                       float* __restrict__ unit) {
+  const float g = largest_finite(grad_out, N);
+  if (threadIdx.x == 0) *unit = unit_of(a, g);
 }
 
 // One workgroup per GEMM row i of source row idx[i] (idx null: i): its
@@ -243,29 +248,10 @@ int distill_forward_run(const bf16_t* H, const bf16_t* W, const float* bias, lon
   if (F.idx) {
     hipLaunchKernelGGL(kd_rows_kernel, dim3((unsigned)ceil_div(N, 4)), dim3(256), 0, st, a, (int)N, (int)V, rows);
     HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL(compact_rows_kernel, dim3(1), dim3(1024), 0, st, rows, 0, (int)N, -1L, F.idx, F.live, slots,
-                       (int)ceil_div(V, kBN), device_cus());
-    HIP_TRY(hipGetLastError());
-    if (F.Hc) {
-      hipLaunchKernelGGL(gather_rows_kernel, dim3((unsigned)std::min<long>(ceil_div(N * (d / 8), 256), 8192)),
-                         dim3(256), 0, st, H, (int)d, F.idx, (int)N, F.Hc);
-      HIP_TRY(hipGetLastError());
-    }
+    const int rc = order_rows(rows, 0, -1L, H, N, d, V, slots, F, st);
+    if (rc) return rc;
   }
-  GemmShape g;
-  g.A = F.Hc ? F.Hc : H;
-  if (F.idx && !F.Hc) {
-    g.arow = F.idx;
-    g.arows = N;
-  }
-  g.lda = d;
-  g.B = W;
-  g.ldb = d;
-  g.M = (int)N;
-  g.N = (int)V;
-  g.K = (int)d;
-  g.live = F.live;
-  g.dyn = F.live ? kDynM : kDynNone;
+  const GemmShape g = forward_shape(H, W, N, d, V, F);
   LseParams ep;
   ep.bias = bias;
   ep.pm = F.pm;

@@ -1,0 +1,212 @@
+// Token log-probabilities (token_logprobs.h) fused with the head's product: the logits
+// H . W^T + b are not kept.  The forward's GEMM gives each row's maximum and two sums,
+// the token's logit is a dot product of its own.  The backward is the
+// cross-entropy's, band by band, with another form of the epilogue's coefficients.
+// With alternatives the logits of a block of rows go through memory in fp32, and the
+// row kernels take them from there.
+
+// One wave per row: joins the vocabulary splits and takes the token's logit.
+// stats[n] = {maximum in base 2, log2 of the sum, entropy, 0}.
+__global__ __launch_bounds__(256) void lp_linear_join_kernel(const float* __restrict__ pm, const float* __restrict__ ps,
+                                                             const float* __restrict__ pw, int splits, long ldp,
+                                                             const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
+                                                             const float* __restrict__ bias, int N, int d, int V,
+                                                             Tokens a, const int* __restrict__ idx,
+                                                             const int* __restrict__ live, LpOut out) {
+  const int l = threadIdx.x & 63;
+  const long i = blockIdx.x * 4L + (threadIdx.x >> 6);
+  if (i >= N) return;
+  const long n = idx ? idx[i] : i;
+  int col;
+  if (!token_of(a, n, V, col)) {
+    if (l == 0) {
+      out.logprobs[n] = out.entropy[n] = 0.f;
+      out.stats[n] = make_float4(0.f, FLT_MAX, 0.f, 0.f);
+    }
+    return;
+  }
+  if (live) {  // as in fwd_combine_kernel
+    splits = live[1];
+    ldp = (long)((live[0] + kBM - 1) / kBM) * kBM;
+  }
+  typedef EpiLseEntropy<kBN> Epi;
+  float m = kLogitFloor, s = 0.f, w = 0.f;
+  for (int k = l; k < splits; k += 64) Epi::merge_entropy(m, s, w, pm[k * ldp + i], ps[k * ldp + i], pw[k * ldp + i]);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) Epi::merge_entropy(m, s, w, __shfl_xor(m, o), __shfl_xor(s, o), __shfl_xor(w, o));
+  float x = 0.f;
+  if (col >= 0) {
+    const bf16_t *const h = H + n * (long)d, *const wr = W + (long)col * d;
+    for (int k = l * 8; k < d; k += 512) {
+      const u32x4 hv = *reinterpret_cast<const u32x4*>(h + k), wv = *reinterpret_cast<const u32x4*>(wr + k);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        x += bf16_to_f32(hv[q] & 0xffffu) * bf16_to_f32(wv[q] & 0xffffu);
+        x += bf16_to_f32(hv[q] >> 16) * bf16_to_f32(wv[q] >> 16);
+      }
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o);
+    if (bias) x += bias[col];
+  }
+  if (l != 0) return;
+  const bool none = s == 0.f;
+  // the maximum's logit and the token's are sums in different orders: where they are
+  // one, their difference may come out above 0
+  float lp = none ? -INFINITY : kLn2 * (__builtin_fmaf(x, a.scale, -m) - log2f(s));
+  if (lp > 0.f) lp = 0.f;
+  const float h = none ? 0.f : kLn2 * (log2f(s) - w / s);
+  out.logprobs[n] = col >= 0 ? lp : 0.f;
+  out.entropy[n] = h;
+  out.stats[n] = make_float4(m, none ? FLT_MAX : log2f(s), h, 0.f);
+}
+
+struct LpLinearGrad {
+  LpGrad p;
+  Tokens a;
+  const float4* stats;
+  int V;
+};
+
+// The unit of G (distill_linear.h): at a row's token G is nearly -g / T, so the
+// mantissa of the largest one, which all rows have where the gradient is a mean's.
+__global__ __launch_bounds__(1024) void lp_unit_kernel(LpGrad p, int N, float* __restrict__ unit) {
+  const float g = p.g ? largest_finite(p.g, N) : 0.f;
+  if (threadIdx.x == 0) *unit = mantissa(g * p.inv_t);
+}
+
+// Coefficients of GEMM row i, of source row idx[i] (null: i), in units of *unit.
+__global__ __launch_bounds__(256) void lp_linear_prep_kernel(LpLinearGrad q, const int* __restrict__ idx, int N,
+                                                             float4* __restrict__ rowp, int* __restrict__ rowlab,
+                                                             const float* __restrict__ unit) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= N) return;
+  const long n = idx ? idx[i] : i;
+  int col;
+  const bool counts = token_of(q.a, n, q.V, col);
+  const float4 st = q.stats[n];
+  float4 rp = make_float4(FLT_MAX, 0.f, 0.f, 0.f);
+  if (counts && st.y != FLT_MAX) {
+    float c, b, at;
+    q.p.row(n, col, st.z, c, b, at);
+    const float u = *unit;
+    rp = make_float4(st.x + st.y, c / u, -at / u, b / u);
+  } else {
+    col = -1;
+  }
+  rowp[i] = rp;
+  rowlab[i] = col;
+}
+
+int lp_prep(const SparseGrad& s, const int* idx, long N, float4* rowp, int* rowlab, int*, float*, float* unit,
+            hipStream_t st) {
+  const LpLinearGrad& q = *static_cast<const LpLinearGrad*>(s.args);
+  hipLaunchKernelGGL(lp_unit_kernel, dim3(1), dim3(1024), 0, st, q.p, (int)N, unit);
+  HIP_TRY(hipGetLastError());
+  hipLaunchKernelGGL(lp_linear_prep_kernel, dim3((unsigned)ceil_div(N, 256)), dim3(256), 0, st, q, idx, (int)N, rowp,
+                     rowlab, unit);
+  HIP_TRY(hipGetLastError());
+  return CCE_OK;
+}
+
+// Rows of a block whose logits go through memory, with k alternatives: fp32 logits of
+// 512 MiB, whole row tiles.
+constexpr long kLogitsBudget = 512L << 20;
+long logits_ld(long V) { return (long)align_up((size_t)V, 64); }
+long logits_block(long N, long V) {
+  return std::min<long>(std::max<long>(kLogitsBudget / (4 * logits_ld(V)) / kBM * kBM, kBM), std::max<long>(N, 1));
+}
+
+struct LpLinearLayout {
+  FwdLayout f;
+  float* pw;
+  float* logits;
+  void* rows;  // workspace of a block's row kernels
+  size_t bytes;
+};
+
+LpLinearLayout lp_linear_layout(void* ws, long N, long d, long V, long k) {
+  LpLinearLayout L;
+  L.f = fwd_layout(ws, N, d, V, CCE_REDUCTION_NONE, CCE_LSE_LABELLED_ROWS);
+  Carver c(ws);
+  c.off = L.f.bytes;
+  if (k > 0) {
+    const long R = logits_block(N, V);
+    L.pw = nullptr;
+    L.logits = c.take<float>((size_t)(R * logits_ld(V)));
+    // the last block has fewer rows, which may be split over more workgroups
+    const long last = N > 0 ? (N - 1) % R + 1 : 0;
+    L.rows = c.take<char>(std::max(lp_layout(nullptr, R, V, k).bytes, lp_layout(nullptr, last, V, k).bytes));
+    L.bytes = align_up(c.off, 256);
+    return L;
+  }
+  L.pw = c.take<float>((size_t)forward_slots(N, V, fwd_compacts(N, d, CCE_LSE_LABELLED_ROWS)) * kBM);
+  L.logits = nullptr;
+  L.rows = nullptr;
+  L.bytes = align_up(c.off, 256);
+  return L;
+}
+
+template <template <int> class Epi>
+int launch_out(const GemmShape& g, const OutParams& e, hipStream_t st) {
+  const int nb = (int)(ceil_div(g.M, kBM) * ceil_div(g.N, kBN));
+  constexpr int kKind = CCE_KERNEL_FWD_LSE;
+  if (!whole_slabs(g.K)) return launch_gemm<kBN, Epi, false, true>(g, e, nb, st, kKind, true);
+  if (g.arow) return launch_gemm<kBN, Epi, true>(g, e, nb, st, kKind, true);
+  return launch_gemm<kBN, Epi>(g, e, nb, st, kKind, true);
+}
+
+int lp_linear_forward_run(const bf16_t* H, const bf16_t* W, const float* bias, long N, long d, long V, long k,
+                          const Tokens& a, LpOut out, const LpLinearLayout& L, hipStream_t st) {
+  const FwdLayout& F = L.f;
+  const int slots = (int)forward_slots(N, V, F.idx != nullptr);
+  int rc = order_rows(a.ids, a.ids64, a.ignore_index, H, N, d, V, slots, F, st);
+  if (rc) return rc;
+  GemmShape g = forward_shape(H, W, N, d, V, F);
+  if (k > 0) {
+    const long R = logits_block(N, V), ld = logits_ld(V);
+    out.stat_scale = a.scale;
+    const OutParams e = {L.logits, ld, bias};
+    for (long m0 = 0; m0 < N; m0 += R) {
+      const long rows = std::min(R, N - m0);
+      if (F.idx && !F.Hc)
+        g.arow = F.idx + m0;
+      else
+        g.A = (F.Hc ? F.Hc : H) + m0 * d;
+      g.M = (int)rows;
+      g.live_base = (int)m0;
+      rc = bias ? launch_out<EpiOutBias>(g, e, st) : launch_out<EpiOut>(g, e, st);
+      if (rc) return rc;
+      // without a row order the rows' tokens and outputs start at m0
+      Tokens b = a;
+      LpOut o = out;
+      if (!F.idx && m0 > 0) {
+        b.ids = static_cast<const char*>(a.ids) + m0 * (a.ids64 ? 8 : 4);
+        o.logprobs += m0;
+        o.entropy += m0;
+        o.stats += m0;
+        o.top_logprobs += m0 * k;
+        o.top_indices += m0 * k;
+      }
+      rc = lp_forward_run(L.logits, ld, rows, V, k, b, F.idx ? F.idx + m0 : nullptr, o,
+                          lp_layout(L.rows, rows, V, k), st);
+      if (rc) return rc;
+    }
+    return CCE_OK;
+  }
+  LseParams ep;
+  ep.bias = bias;
+  ep.pm = F.pm;
+  ep.ps = F.ps;
+  ep.ps1 = L.pw;
+  ep.ldp = N;
+  ep.splits = forward_splits(N, V);
+  ep.tiles_n = (int)ceil_div(V, kBN);
+  ep.scale = a.scale;
+  rc = bias ? launch_lse<EpiLseBiasEntropy>(g, ep, slots, st) : launch_lse<EpiLseEntropy>(g, ep, slots, st);
+  if (rc) return rc;
+  hipLaunchKernelGGL(lp_linear_join_kernel, dim3((unsigned)ceil_div(N, 4)), dim3(256), 0, st, F.pm, F.ps, L.pw, ep.splits,
+                     (long)N, H, W, bias, (int)N, (int)d, (int)V, a, F.idx, F.live, out);
+  HIP_TRY(hipGetLastError());
+  return CCE_OK;
+}

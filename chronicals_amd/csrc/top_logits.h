@@ -206,8 +206,12 @@ constexpr int kTopCandidates = 2048, kTopGroups = 1024;
 // 144 -> 136 us came from non-temporal loads in pass 1 and 136 -> 128 from eight
 // workgroups per CU instead of seven.  With all but 20 columns of a row at a mask's
 // value 390 us, and by top_exact after the overflow 2510.
-template <typename T>
-__device__ void top_of_row(const T* row, int V, int k, uint32_t* hist, uint16_t* groups, const TopList& list) {
+//
+// Pass 1 hands every chunk to each(chunk); without a pass 1 (fewer chunks than k)
+// nothing is handed out.
+template <typename T, typename Each>
+__device__ void top_of_row(const T* row, int V, int k, uint32_t* hist, uint16_t* groups, const TopList& list,
+                           Each&& each) {
   constexpr int U = 4, NP = GroupMax<T>::kParts;
   __shared__ int counts[2][4], ngroups;
   const int tid = threadIdx.x, l = tid & 63, w = tid >> 6;
@@ -225,11 +229,18 @@ __device__ void top_of_row(const T* row, int V, int k, uint32_t* hist, uint16_t*
 #pragma unroll
           for (int u = 0; u < U; ++u) raw[u] = __builtin_nontemporal_load(body + c + u * 256);
 #pragma unroll
-          for (int u = 0; u < U; ++u) part[r][u].add(raw[u]);
+          for (int u = 0; u < U; ++u) {
+            part[r][u].add(raw[u]);
+            each(raw[u]);
+          }
         } else {
 #pragma unroll
           for (int u = 0; u < U; ++u)
-            if (c + u * 256 < sp.chunks) part[r][u].add(body[c + u * 256]);
+            if (c + u * 256 < sp.chunks) {
+              const u32x4 raw = body[c + u * 256];
+              part[r][u].add(raw);
+              each(raw);
+            }
         }
       }
     }
@@ -361,7 +372,7 @@ __global__ __launch_bounds__(256) void top_logits_kernel(const T* __restrict__ X
   split_span(V, S, blockIdx.x % S, c0, c1);
   const T* const row = X + n * ld + c0;
   const int m = min(k, c1 - c0);
-  if (m > 0) top_of_row(row, c1 - c0, m, hist, groups, list);
+  if (m > 0) top_of_row(row, c1 - c0, m, hist, groups, list, [](const u32x4&) {});
   if (S == 1) {
     top_ranked(list, k, [&](int rank, uint64_t c) {
       values[n * k + rank] = row[column(c)];
@@ -374,19 +385,16 @@ __global__ __launch_bounds__(256) void top_logits_kernel(const T* __restrict__ X
   for (int i = m + threadIdx.x; i < k; i += 256) out[i] = 0;
 }
 
-// The k largest of a row from those of its S splits.  S * ceil(k / S) candidates
-// reach the smallest of the splits' ceil(k / S)-th ones, so no other counts.
-template <typename T>
-__global__ __launch_bounds__(256) void top_join_kernel(const T* __restrict__ X, long ld, int S, int k,
-                                                       const uint64_t* __restrict__ part, T* __restrict__ values,
-                                                       int64_t* __restrict__ indices) {
+// Calls f(rank, candidate) for the k largest of a row from those of its S splits, at
+// p.  S * ceil(k / S) candidates reach the smallest of the splits' ceil(k / S)-th
+// ones, so no other counts.
+template <typename F>
+__device__ void top_join(const uint64_t* __restrict__ p, int S, int k, F&& f) {
   constexpr int kE = kTopCandidates / 256;
   __shared__ uint64_t cands[kTopCandidates], low[4];
   __shared__ int count;
   const TopList list = {cands, &count};
-  const long n = blockIdx.x;
   const int tid = threadIdx.x;
-  const uint64_t* const p = part + n * S * k;
   uint64_t c[kE], tau = ~0ull;
   for (int s = tid; s < S; s += 256) tau = min(tau, p[s * k + (k + S - 1) / S - 1]);
 #pragma unroll
@@ -401,7 +409,15 @@ __global__ __launch_bounds__(256) void top_join_kernel(const T* __restrict__ X, 
   for (int e = 0; e < kE; ++e)
     if (c[e] >= tau && c[e] != 0) cands[atomicAdd(&count, 1)] = c[e];
   __syncthreads();
-  top_ranked(list, k, [&](int rank, uint64_t v) {
+  top_ranked(list, k, f);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void top_join_kernel(const T* __restrict__ X, long ld, int S, int k,
+                                                       const uint64_t* __restrict__ part, T* __restrict__ values,
+                                                       int64_t* __restrict__ indices) {
+  const long n = blockIdx.x;
+  top_join(part + n * S * k, S, k, [&](int rank, uint64_t v) {
     values[n * k + rank] = X[n * ld + column(v)];
     indices[n * k + rank] = column(v);
   });

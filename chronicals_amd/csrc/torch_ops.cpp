@@ -62,6 +62,17 @@ struct Api {
   decltype(&cce_layer_norm_forward) layer_norm_forward;
   decltype(&cce_layer_norm_backward_workspace_bytes_for) layer_norm_backward_workspace_bytes_for;
   decltype(&cce_layer_norm_backward) layer_norm_backward;
+  decltype(&cce_token_logprobs_workspace_bytes) token_logprobs_workspace_bytes;
+  decltype(&cce_token_logprobs_forward) token_logprobs_forward;
+  decltype(&cce_token_logprobs_backward) token_logprobs_backward;
+  decltype(&cce_linear_token_logprobs_workspace_bytes) linear_token_logprobs_workspace_bytes;
+  decltype(&cce_linear_token_logprobs_forward) linear_token_logprobs_forward;
+  decltype(&cce_linear_token_logprobs_backward_workspace_bytes) linear_token_logprobs_backward_workspace_bytes;
+  decltype(&cce_linear_token_logprobs_backward) linear_token_logprobs_backward;
+  decltype(&cce_rms_norm_forward) rms_norm_forward;
+  decltype(&cce_rms_norm_quantized) rms_norm_quantized;
+  decltype(&cce_rms_norm_backward_workspace_bytes) rms_norm_backward_workspace_bytes;
+  decltype(&cce_rms_norm_backward) rms_norm_backward;
 };
 
 Api g_api;
@@ -480,12 +491,15 @@ std::tuple<Tensor, Tensor> top_logits(const Tensor& logits, int64_t k) {
   return {values, indices};
 }
 
+void check_norm_rows(const Tensor& x, const char* what) {
+  TORCH_CHECK(is_logits(x), what, " dtype ", x.scalar_type(), " not supported (bf16, fp16, fp32)");
+  TORCH_CHECK(x.dim() == 2 && (x.size(0) == 0 || x.size(1) <= 1 || x.stride(1) == 1), what,
+              " ops take [N, D] rows with a contiguous last dimension, got shape ", x.sizes(), " strides ", x.strides());
+}
+
 // The parameters' type: that of the weight or, without one, of the bias.
 int check_norm(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias) {
-  TORCH_CHECK(is_logits(x), "layer_norm dtype ", x.scalar_type(), " not supported (bf16, fp16, fp32)");
-  TORCH_CHECK(x.dim() == 2 && (x.size(1) <= 1 || x.stride(1) == 1),
-              "layer_norm ops take [N, D] rows with a contiguous last dimension, got shape ", x.sizes(), " strides ",
-              x.strides());
+  check_norm_rows(x, "layer_norm");
   at::ScalarType type = x.scalar_type();
   for (const optional<Tensor>* p : {&bias, &weight}) {
     if (!p->has_value()) continue;
@@ -542,6 +556,223 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor& grad_y, const Te
 }
 
 // ---------------------------------------------------------------------------
+// Token log-probabilities, RMS norm
+// ---------------------------------------------------------------------------
+
+void check_tokens(const Tensor& tokens, const Tensor& x) {
+  TORCH_CHECK(tokens.dim() == 1 && tokens.size(0) == x.size(0) && is_label(tokens) && tokens.is_contiguous(),
+              "token_logprobs ops take contiguous int64/int32 tokens [N = ", x.size(0), "], got ", tokens.scalar_type(),
+              " ", tokens.sizes());
+  TORCH_CHECK(tokens.device() == x.device(), "tokens must be on the device of the logits or hidden states");
+}
+
+struct LogprobsOut {
+  Tensor logprobs, entropy, stats, top_logprobs, top_indices;
+  LogprobsOut(const Tensor& x, int64_t top_k, int64_t V) {
+    TORCH_CHECK(top_k >= 0 && top_k <= std::min<int64_t>(V, CCE_MAX_TEACHER_ENTRIES), "top_k must be in [0, min(",
+                CCE_MAX_TEACHER_ENTRIES, ", V = ", V, ")], got ", top_k);
+    const int64_t N = x.size(0);
+    const auto opt = x.options().dtype(at::kFloat);
+    logprobs = at::empty({N}, opt);
+    entropy = at::empty({N}, opt);
+    stats = at::empty({N, 4}, opt);
+    top_logprobs = at::empty({N, top_k}, opt);
+    top_indices = at::empty({N, top_k}, x.options().dtype(at::kLong));
+  }
+  std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> all() const {
+    return {logprobs, entropy, stats, top_logprobs, top_indices};
+  }
+  int64_t* indices() const { return static_cast<int64_t*>(top_indices.data_ptr()); }
+};
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs_fwd(const Tensor& logits, const Tensor& tokens,
+                                                                      double temperature, int64_t top_k,
+                                                                      int64_t ignore_index) {
+  check_student_logits(logits);
+  check_tokens(tokens, logits);
+  const Api& a = api();
+  const c10::DeviceGuard guard(logits.device());
+  const int64_t N = logits.size(0), V = logits.size(1);
+  const LogprobsOut o(logits, top_k, V);
+  size_t bytes = 0;
+  check(a, a.token_logprobs_workspace_bytes(N, V, top_k, &bytes));
+  const Tensor ws = at::empty({(int64_t)bytes}, logits.options().dtype(at::kByte));
+  check(a, a.token_logprobs_forward(logits.data_ptr(), logits_dtype(logits), row_stride(logits), tokens.data_ptr(),
+                                    tokens.scalar_type() == at::kLong, N, V, ignore_index, (float)temperature, top_k,
+                                    f32(o.logprobs), f32(o.entropy), f32(o.stats), f32(o.top_logprobs), o.indices(),
+                                    ws.data_ptr(), bytes, stream(logits.device())));
+  return o.all();
+}
+
+// A gradient per row that may be absent, as contiguous fp32.
+struct RowGrad {
+  Tensor t;
+  RowGrad(const optional<Tensor>& g, const char* name, const Tensor& x) {
+    if (!g.has_value()) return;
+    t = grad_rows(*g);
+    check_kept(t, name, at::kFloat, x.size(0), x);
+  }
+  const float* ptr() const { return t.defined() ? f32(t) : nullptr; }
+};
+
+Tensor token_logprobs_bwd(const optional<Tensor>& grad_logprobs, const optional<Tensor>& grad_entropy,
+                          const Tensor& logits, const Tensor& tokens, const Tensor& stats, double temperature,
+                          int64_t ignore_index) {
+  check_student_logits(logits);
+  check_tokens(tokens, logits);
+  check_kept(stats, "stats", at::kFloat, 4 * logits.size(0), logits);
+  const Api& a = api();
+  const c10::DeviceGuard guard(logits.device());
+  const RowGrad g(grad_logprobs, "grad_logprobs", logits), h(grad_entropy, "grad_entropy", logits);
+  Tensor dx = at::empty(logits.sizes(), logits.options());
+  check(a, a.token_logprobs_backward(g.ptr(), h.ptr(), logits.data_ptr(), logits_dtype(logits), row_stride(logits),
+                                     tokens.data_ptr(), tokens.scalar_type() == at::kLong, f32(stats), logits.size(0),
+                                     logits.size(1), ignore_index, (float)temperature, dx.data_ptr(), row_stride(dx),
+                                     stream(logits.device())));
+  return dx;
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> linear_token_logprobs_fwd(
+    const Tensor& hidden_, const Tensor& weight_, const optional<Tensor>& bias, const Tensor& tokens, double temperature,
+    int64_t top_k, int64_t ignore_index) {
+  check_head(hidden_, weight_, bias);
+  check_tokens(tokens, hidden_);
+  const Api& a = api();
+  const c10::DeviceGuard guard(hidden_.device());
+  const Tensor hidden = aligned(hidden_), weight = aligned(weight_);
+  const int64_t N = hidden.size(0), d = hidden.size(1), V = weight.size(0);
+  const LogprobsOut o(hidden, top_k, V);
+  size_t bytes = 0;
+  check(a, a.linear_token_logprobs_workspace_bytes(N, d, V, top_k, &bytes));
+  const Tensor ws = at::empty({(int64_t)bytes}, hidden.options().dtype(at::kByte));
+  check(a, a.linear_token_logprobs_forward(hidden.data_ptr(), weight.data_ptr(), bias_ptr(bias), tokens.data_ptr(),
+                                           tokens.scalar_type() == at::kLong, N, d, V, ignore_index, (float)temperature,
+                                           top_k, f32(o.logprobs), f32(o.entropy), f32(o.stats), f32(o.top_logprobs),
+                                           o.indices(), ws.data_ptr(), bytes, stream(hidden.device())));
+  return o.all();
+}
+
+std::tuple<Tensor, Tensor, Tensor> linear_token_logprobs_bwd(
+    const optional<Tensor>& grad_logprobs, const optional<Tensor>& grad_entropy, const Tensor& hidden_,
+    const Tensor& weight_, const optional<Tensor>& bias, const Tensor& tokens, const Tensor& stats, double temperature,
+    int64_t ignore_index, int64_t chunk_size, bool need_dh, bool need_dw, bool need_db, bool dh_f32, bool dw_f32) {
+  check_head(hidden_, weight_, bias);
+  check_tokens(tokens, hidden_);
+  TORCH_CHECK(!need_db || bias.has_value(), "need_db requires a bias");
+  const Api& a = api();
+  const c10::DeviceGuard guard(hidden_.device());
+  const Tensor hidden = aligned(hidden_), weight = aligned(weight_);
+  const int64_t N = hidden.size(0), d = hidden.size(1), V = weight.size(0);
+  check_kept(stats, "stats", at::kFloat, 4 * N, hidden);
+  const RowGrad g(grad_logprobs, "grad_logprobs", hidden), h(grad_entropy, "grad_entropy", hidden);
+  const auto opt = hidden.options().dtype(at::kFloat);
+  auto empty = [&](bool need, at::IntArrayRef size, bool f) {
+    return at::empty(need ? size : at::IntArrayRef{0}, f ? opt : hidden.options());
+  };
+  Tensor dh = empty(need_dh, {N, d}, dh_f32), dw = empty(need_dw, {V, d}, dw_f32), db = empty(need_db, {V}, true);
+  if (need_dh || need_dw || need_db) {
+    const int hdt = dh_f32 ? CCE_DTYPE_F32 : CCE_DTYPE_BF16, wdt = dw_f32 ? CCE_DTYPE_F32 : CCE_DTYPE_BF16;
+    size_t bytes = 0;
+    check(a, a.linear_token_logprobs_backward_workspace_bytes(N, d, V, chunk_size, need_dh, hdt, need_dw, wdt, &bytes));
+    const Tensor ws = at::empty({(int64_t)bytes}, hidden.options().dtype(at::kByte));
+    check(a, a.linear_token_logprobs_backward(
+                 g.ptr(), h.ptr(), hidden.data_ptr(), weight.data_ptr(), bias_ptr(bias), tokens.data_ptr(),
+                 tokens.scalar_type() == at::kLong, f32(stats), N, d, V, ignore_index, (float)temperature, chunk_size,
+                 need_dh ? dh.data_ptr() : nullptr, hdt, need_dw ? dw.data_ptr() : nullptr, wdt,
+                 need_db ? f32(db) : nullptr, ws.data_ptr(), bytes, stream(hidden.device())));
+  }
+  return {dh, dw, db};
+}
+
+// Operands of an RMS norm: the weight's type, and the residual's as the C functions take it.
+struct RmsArgs {
+  int param, dtype;
+  const void* residual = nullptr;
+  int residual_dtype;
+  int64_t ldr;
+  RmsArgs(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& r) {
+    check_norm_rows(x, "rms_norm");
+    dtype = residual_dtype = logits_dtype(x);
+    ldr = x.size(1);
+    param = check_norm(x, weight, std::nullopt);
+    if (!r.has_value()) return;
+    check_norm_rows(*r, "rms_norm residual");
+    TORCH_CHECK(r->sizes() == x.sizes() && r->device() == x.device() &&
+                    (r->scalar_type() == x.scalar_type() || r->scalar_type() == at::kFloat),
+                "residual must have the input's shape and device, and its dtype or fp32, got ", r->scalar_type(), " ",
+                r->sizes());
+    residual = r->data_ptr();
+    residual_dtype = logits_dtype(*r);
+    ldr = row_stride(*r);
+  }
+};
+
+Tensor sum_like(const Tensor& x, const optional<Tensor>& residual) {
+  return residual.has_value() ? at::empty(x.sizes(), residual->options()) : at::empty({0}, x.options());
+}
+
+std::tuple<Tensor, Tensor, Tensor> rms_norm_fwd(const Tensor& x, const optional<Tensor>& weight,
+                                                const optional<Tensor>& residual, double eps) {
+  const RmsArgs r(x, weight, residual);
+  const Api& a = api();
+  const c10::DeviceGuard guard(x.device());
+  const int64_t N = x.size(0), D = x.size(1);
+  Tensor y = at::empty({N, D}, x.options()), sum = sum_like(x, residual);
+  Tensor rstd = at::empty({N}, x.options().dtype(at::kFloat));
+  check(a, a.rms_norm_forward(x.data_ptr(), r.dtype, row_stride(x), r.residual, r.residual_dtype, r.ldr,
+                              label_ptr(weight), r.param, N, D, (float)eps, y.data_ptr(),
+                              r.residual ? sum.data_ptr() : nullptr, f32(rstd), stream(x.device())));
+  return {y, sum, rstd};
+}
+
+std::tuple<Tensor, Tensor, Tensor> rms_norm_quantized(const Tensor& x, const optional<Tensor>& weight,
+                                                      const optional<Tensor>& residual, double eps, bool int8,
+                                                      int64_t group) {
+  const RmsArgs r(x, weight, residual);
+  TORCH_CHECK(group == 0 || group == 32 || group == 64 || group == 128 || group == 256,
+              "group must be 0 (a row), 32, 64, 128 or 256, got ", group);
+  const Api& a = api();
+  const c10::DeviceGuard guard(x.device());
+  const int64_t N = x.size(0), D = x.size(1);
+  Tensor q = at::empty({N, D}, x.options().dtype(int8 ? at::kChar : at::kFloat8_e4m3fn));
+  const auto opt = x.options().dtype(at::kFloat);
+  Tensor scales = group ? at::empty({N, (D + group - 1) / group}, opt) : at::empty({N}, opt);
+  Tensor sum = sum_like(x, residual);
+  check(a, a.rms_norm_quantized(x.data_ptr(), r.dtype, row_stride(x), r.residual, r.residual_dtype, r.ldr,
+                                label_ptr(weight), r.param, N, D, (float)eps, int8 ? CCE_DTYPE_INT8 : CCE_DTYPE_E4M3,
+                                group, q.data_ptr(), f32(scales), r.residual ? sum.data_ptr() : nullptr,
+                                stream(x.device())));
+  return {q, scales, sum};
+}
+
+std::tuple<Tensor, Tensor, Tensor> rms_norm_bwd(const Tensor& grad_y, const optional<Tensor>& grad_sum, const Tensor& sum,
+                                                const optional<Tensor>& weight, const Tensor& rstd, bool param_f32,
+                                                bool need_dx, bool need_dr, bool need_dw) {
+  const RmsArgs r(grad_y, weight, sum);
+  const int pdt = param_f32 ? CCE_DTYPE_F32 : r.dtype;
+  TORCH_CHECK(!weight.has_value() || r.param == pdt, "param_f32 does not fit the weight's dtype");
+  TORCH_CHECK(grad_y.is_contiguous(), "grad_y must be contiguous");
+  TORCH_CHECK(!grad_sum.has_value() || (grad_sum->sizes() == sum.sizes() && grad_sum->is_contiguous() &&
+                                        grad_sum->scalar_type() == sum.scalar_type() && grad_sum->device() == sum.device()),
+              "grad_sum must be a contiguous tensor of the sum's shape, dtype and device");
+  const int64_t N = grad_y.size(0), D = grad_y.size(1);
+  check_kept(rstd, "rstd", at::kFloat, N, grad_y);
+  const Api& a = api();
+  const c10::DeviceGuard guard(grad_y.device());
+  Tensor dx = at::empty(need_dx ? grad_y.sizes() : at::IntArrayRef{0}, grad_y.options());
+  Tensor dr = at::empty(need_dr ? grad_y.sizes() : at::IntArrayRef{0}, sum.options());
+  Tensor dw = at::empty({need_dw ? D : 0}, grad_y.options().dtype(param_f32 ? at::kFloat : grad_y.scalar_type()));
+  size_t bytes = 0;
+  check(a, a.rms_norm_backward_workspace_bytes(N, D, r.dtype, need_dw, &bytes));
+  const Tensor ws = at::empty({(int64_t)bytes}, grad_y.options().dtype(at::kByte));
+  check(a, a.rms_norm_backward(grad_y.data_ptr(), label_ptr(grad_sum), sum.data_ptr(), r.dtype, r.residual_dtype, r.ldr,
+                               label_ptr(weight), pdt, f32(rstd), N, D, need_dx ? dx.data_ptr() : nullptr,
+                               need_dr ? dr.data_ptr() : nullptr, need_dw ? dw.data_ptr() : nullptr, ws.data_ptr(), bytes,
+                               stream(grad_y.device())));
+  return {dx, dr, dw};
+}
+
+// ---------------------------------------------------------------------------
 // Differentiable operators: autograd functions over the ones above, which they
 // call through the dispatcher, so that a trace sees those.  The gradients are
 // kernels' results and have none of their own (gradients()).
@@ -573,11 +804,11 @@ Tensor scalar(const Tensor& t) { return at::_unsafe_view(t, at::IntArrayRef()); 
 
 // The body of a backward: the gradients are computed without a graph of their own.
 // Where one is asked for (create_graph), they lead to what the function's inputs
-// and its incoming gradient came from, through a node that raises.  Without it
+// and its incoming gradients came from, through a node that raises.  Without it
 // they would be constants where the operands saved are copies (of another type,
 // of strided rows), and a penalty on them would be left out without a word.
 template <typename F>
-variable_list gradients(const Tensor& grad, F&& compute) {
+variable_list gradients(at::ArrayRef<Tensor> grads, F&& compute) {
   const bool twice = at::GradMode::is_enabled();
   variable_list out;
   {
@@ -587,7 +818,8 @@ variable_list gradients(const Tensor& grad, F&& compute) {
   if (!twice) return out;
   torch::autograd::edge_list edges;
   if (const auto node = torch::autograd::get_current_node()) edges = node->next_edges();
-  if (grad.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(grad));
+  for (const Tensor& grad : grads)
+    if (grad.defined() && grad.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(grad));
   const auto error = std::make_shared<torch::autograd::Error>(
       "the gradients of chronicals_hip operators cannot be differentiated again", std::move(edges));
   for (Tensor& t : out) {
@@ -735,6 +967,175 @@ Tensor distill_linear(const Tensor& hidden, const Tensor& weight, const optional
   return DistillLinear::apply(hidden, weight, bias, t, index, labels, chunk_size, temperature, distill_weight, ce_weight, ignore_index, reduction);
 }
 
+// A result of N rows in the shape of the rows of x, whose last dimension is left out,
+// followed by the result's own last one, if it has one.
+Tensor shaped_rows(const Tensor& t, const Tensor& x) {
+  if (x.dim() == 2) return t;
+  auto shape = x.sym_sizes().vec();
+  shape.pop_back();
+  for (int64_t i = 1; i < t.dim(); ++i) shape.push_back(t.sym_size(i));
+  return at::_unsafe_view_symint(t, shape);
+}
+
+typedef std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> FiveTensors;
+typedef std::tuple<Tensor, Tensor, Tensor, Tensor> FourTensors;
+
+// What the two functions below return: the alternatives carry no gradient, and the
+// gradient that is not asked for stays undefined.
+variable_list logprobs_results(AutogradContext* ctx, const FiveTensors& r, const Tensor& x) {
+  const auto& [logprobs, entropy, stats, top_logprobs, top_indices] = r;
+  variable_list out = {shaped_rows(logprobs, x), shaped_rows(entropy, x), shaped_rows(top_logprobs, x),
+                       shaped_rows(top_indices, x)};
+  ctx->mark_non_differentiable({out[2], out[3]});
+  ctx->set_materialize_grads(false);
+  return out;
+}
+
+// Tokens are contiguous [N].
+struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, double temperature,
+                               int64_t top_k, int64_t ignore_index) {
+    static const auto fwd =
+        find<FiveTensors(const Tensor&, const Tensor&, double, SymInt, SymInt)>("chronicals_hip::token_logprobs_fwd");
+    const Tensor x = as_rows(logits);
+    const FiveTensors r = fwd.call(x, tokens, temperature, top_k, ignore_index);
+    ctx->save_for_backward({x, tokens, std::get<2>(r)});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->saved_data["dim"] = logits.dim();
+    if (logits.dim() != 2) ctx->saved_data["shape"] = logits.sym_sizes();
+    return logprobs_results(ctx, r, logits);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    static const auto bwd =
+        find<Tensor(const optional<Tensor>&, const optional<Tensor>&, const Tensor&, const Tensor&, const Tensor&, double,
+                    SymInt)>("chronicals_hip::token_logprobs_bwd");
+    if (!ctx->needs_input_grad(0) || (!grads[0].defined() && !grads[1].defined())) return variable_list(5);
+    return gradients({grads[0], grads[1]}, [&] {
+      variable_list out(5);
+      const auto s = ctx->get_saved_variables();
+      out[0] = bwd.call(given(grads[0]), given(grads[1]), s[0], s[1], s[2], ctx->saved_data["temperature"].toDouble(),
+                        ctx->saved_data["ignore_index"].toInt());
+      if (ctx->saved_data["dim"].toInt() != 2) out[0] = out[0].view_symint(ctx->saved_data["shape"].toSymIntVector());
+      return out;
+    });
+  }
+};
+
+FourTensors token_logprobs(const Tensor& logits, const Tensor& tokens, double temperature, int64_t top_k,
+                           int64_t ignore_index) {
+  const auto r = TokenLogprobs::apply(logits, tokens, temperature, top_k, ignore_index);
+  return {r[0], r[1], r[2], r[3]};
+}
+
+struct LinearTokenLogprobs : torch::autograd::Function<LinearTokenLogprobs> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight,
+                               const optional<Tensor>& bias, const Tensor& tokens, int64_t chunk_size, double temperature,
+                               int64_t top_k, int64_t ignore_index) {
+    static const auto fwd = find<FiveTensors(const Tensor&, const Tensor&, const optional<Tensor>&, const Tensor&, double,
+                                             SymInt, SymInt)>("chronicals_hip::linear_token_logprobs_fwd");
+    // fp16 and fp32 operands are rounded to bf16, the GEMMs' type
+    const Tensor h = as_rows(hidden).to(at::kBFloat16).contiguous(), w = weight.to(at::kBFloat16).contiguous();
+    const Tensor b = bias.has_value() ? bias->to(at::kFloat).contiguous() : Tensor();
+    const FiveTensors r = fwd.call(h, w, given(b), tokens, temperature, top_k, ignore_index);
+    ctx->save_for_backward({h, w, b, tokens, std::get<2>(r)});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->saved_data["chunk_size"] = chunk_size;
+    ctx->saved_data["shape"] = hidden.sym_sizes();
+    ctx->saved_data["hidden"] = (int64_t)hidden.scalar_type();
+    ctx->saved_data["weight"] = (int64_t)weight.scalar_type();
+    if (bias.has_value()) ctx->saved_data["bias"] = (int64_t)bias->scalar_type();
+    return logprobs_results(ctx, r, hidden);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    static const auto bwd = find<std::tuple<Tensor, Tensor, Tensor>(
+        const optional<Tensor>&, const optional<Tensor>&, const Tensor&, const Tensor&, const optional<Tensor>&,
+        const Tensor&, const Tensor&, double, SymInt, SymInt, bool, bool, bool, bool, bool)>(
+        "chronicals_hip::linear_token_logprobs_bwd");
+    const auto s = ctx->get_saved_variables();
+    const bool need_dh = ctx->needs_input_grad(0), need_dw = ctx->needs_input_grad(1),
+               need_db = s[2].defined() && ctx->needs_input_grad(2);
+    if ((!need_dh && !need_dw && !need_db) || (!grads[0].defined() && !grads[1].defined())) return variable_list(8);
+    return gradients({grads[0], grads[1]}, [&] {
+      variable_list out(8);
+      auto& kept = ctx->saved_data;
+      const auto htype = (at::ScalarType)kept["hidden"].toInt(), wtype = (at::ScalarType)kept["weight"].toInt();
+      // bf16 inputs get bf16 gradients, fp16 and fp32 inputs get them from fp32
+      const auto [dh, dw, db] =
+          bwd.call(given(grads[0]), given(grads[1]), s[0], s[1], given(s[2]), s[3], s[4], kept["temperature"].toDouble(),
+                   kept["ignore_index"].toInt(), kept["chunk_size"].toInt(), need_dh, need_dw, need_db,
+                   htype != at::kBFloat16, wtype != at::kBFloat16);
+      if (need_dh) out[0] = dh.view_symint(kept["shape"].toSymIntVector()).to(htype);
+      if (need_dw) out[1] = dw.to(wtype);
+      if (need_db) out[2] = db.to((at::ScalarType)kept["bias"].toInt());
+      return out;
+    });
+  }
+};
+
+FourTensors linear_token_logprobs(const Tensor& hidden, const Tensor& weight, const optional<Tensor>& bias,
+                                  const Tensor& tokens, int64_t chunk_size, double temperature, int64_t top_k,
+                                  int64_t ignore_index) {
+  const auto r =
+      LinearTokenLogprobs::apply(hidden, weight, bias, tokens, chunk_size, temperature, top_k, ignore_index);
+  return {r[0], r[1], r[2], r[3]};
+}
+
+struct RmsNorm : torch::autograd::Function<RmsNorm> {
+  // y and the sum, which is empty without a residual
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const optional<Tensor>& weight,
+                               const optional<Tensor>& residual, double eps) {
+    static const auto fwd = find<std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const optional<Tensor>&,
+                                                                    const optional<Tensor>&, double)>(
+        "chronicals_hip::rms_norm_fwd");
+    const Tensor rows = as_rows(x);
+    const bool has_r = residual.has_value();
+    const auto [y, sum, rstd] = fwd.call(rows, weight, has_r ? optional<Tensor>(as_rows(*residual)) : residual, eps);
+    auto shaped = [&](const Tensor& t) { return x.dim() == 2 ? t : at::_unsafe_view_symint(t, x.sym_sizes()); };
+    variable_list out = {shaped(y), has_r ? shaped(sum) : sum};
+    ctx->save_for_backward({has_r ? out[1] : rows, weight.value_or(Tensor()), rstd});
+    ctx->saved_data["residual"] = has_r;
+    ctx->saved_data["same"] = has_r && residual->scalar_type() == x.scalar_type();
+    ctx->saved_data["x"] = (int64_t)x.scalar_type();
+    if (!has_r) ctx->mark_non_differentiable({out[1]});
+    ctx->set_materialize_grads(false);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    static const auto bwd = find<std::tuple<Tensor, Tensor, Tensor>(
+        const Tensor&, const optional<Tensor>&, const Tensor&, const optional<Tensor>&, const Tensor&, bool, bool, bool,
+        bool)>("chronicals_hip::rms_norm_bwd");
+    const auto saved = ctx->get_saved_variables();
+    auto& kept = ctx->saved_data;
+    // absent inputs have no edge
+    const bool has_w = saved[1].defined(), has_r = kept["residual"].toBool(), same = kept["same"].toBool(),
+               need_x = ctx->needs_input_grad(0), need_dw = has_w && ctx->needs_input_grad(1),
+               need_r = has_r && ctx->needs_input_grad(has_w ? 2 : 1);
+    if ((!need_x && !need_dw && !need_r) || (!grads[0].defined() && !grads[1].defined())) return variable_list(4);
+    return gradients({grads[0], grads[1]}, [&]() -> variable_list {
+      const Tensor& shaped = grads[0].defined() ? grads[0] : grads[1];
+      const Tensor sum = as_rows(saved[0]);
+      auto rows = [&](const Tensor& t) { return t.reshape_symint(sum.sym_sizes()).contiguous(); };
+      const Tensor g = grads[0].defined()
+                           ? rows(grads[0])
+                           : at::zeros_symint(sum.sym_sizes(), sum.options().dtype((at::ScalarType)kept["x"].toInt()));
+      const auto [dx, dr, dw] =
+          bwd.call(g, grads[1].defined() ? optional<Tensor>(rows(grads[1])) : std::nullopt, sum, given(saved[1]), saved[2],
+                   has_w && saved[1].scalar_type() == at::kFloat, need_x || (need_r && same), need_r && !same, need_dw);
+      auto out = [&](const Tensor& t) { return t.view_symint(shaped.sym_sizes()); };
+      // of one type the two gradients are one
+      return {need_x ? out(dx) : Tensor(), need_dw ? dw : Tensor(), need_r ? out(same ? dx : dr) : Tensor(), Tensor()};
+    });
+  }
+};
+
+std::tuple<Tensor, Tensor> rms_norm(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& residual,
+                                    double eps) {
+  const auto r = RmsNorm::apply(x, contiguous(weight), residual, eps);
+  return {r[0], r[1]};
+}
+
 }  // namespace
 
 extern "C" {
@@ -768,6 +1169,17 @@ int chronicals_torch_bind(void* handle) {
   get(a.layer_norm_forward, "cce_layer_norm_forward");
   get(a.layer_norm_backward_workspace_bytes_for, "cce_layer_norm_backward_workspace_bytes_for");
   get(a.layer_norm_backward, "cce_layer_norm_backward");
+  get(a.token_logprobs_workspace_bytes, "cce_token_logprobs_workspace_bytes");
+  get(a.token_logprobs_forward, "cce_token_logprobs_forward");
+  get(a.token_logprobs_backward, "cce_token_logprobs_backward");
+  get(a.linear_token_logprobs_workspace_bytes, "cce_linear_token_logprobs_workspace_bytes");
+  get(a.linear_token_logprobs_forward, "cce_linear_token_logprobs_forward");
+  get(a.linear_token_logprobs_backward_workspace_bytes, "cce_linear_token_logprobs_backward_workspace_bytes");
+  get(a.linear_token_logprobs_backward, "cce_linear_token_logprobs_backward");
+  get(a.rms_norm_forward, "cce_rms_norm_forward");
+  get(a.rms_norm_quantized, "cce_rms_norm_quantized");
+  get(a.rms_norm_backward_workspace_bytes, "cce_rms_norm_backward_workspace_bytes");
+  get(a.rms_norm_backward, "cce_rms_norm_backward");
   if (!ok) return 1;
   if (!g_bound.load(std::memory_order_acquire)) {
     g_api = a;
@@ -800,12 +1212,22 @@ TORCH_LIBRARY_IMPL(chronicals_hip, CUDA, m) {
   m.impl("top_logits", top_logits);
   m.impl("layer_norm_fwd", layer_norm_fwd);
   m.impl("layer_norm_bwd", layer_norm_bwd);
+  m.impl("token_logprobs_fwd", token_logprobs_fwd);
+  m.impl("token_logprobs_bwd", token_logprobs_bwd);
+  m.impl("linear_token_logprobs_fwd", linear_token_logprobs_fwd);
+  m.impl("linear_token_logprobs_bwd", linear_token_logprobs_bwd);
+  m.impl("rms_norm_fwd", rms_norm_fwd);
+  m.impl("rms_norm_quantized", rms_norm_quantized);
+  m.impl("rms_norm_bwd", rms_norm_bwd);
 }
 
 TORCH_LIBRARY_IMPL(chronicals_hip, CompositeImplicitAutograd, m) {
   m.impl("layer_norm", layer_norm);
   m.impl("distill_logits", distill_logits);
   m.impl("distill_linear", distill_linear);
+  m.impl("token_logprobs", token_logprobs);
+  m.impl("linear_token_logprobs", linear_token_logprobs);
+  m.impl("rms_norm", rms_norm);
 }
 
 // The operators on HIP tensors have no derivative of their own (the autograd functions call
@@ -813,6 +1235,8 @@ TORCH_LIBRARY_IMPL(chronicals_hip, CompositeImplicitAutograd, m) {
 TORCH_LIBRARY_IMPL(chronicals_hip, Autograd, m) {
   for (const char* op : {"cce_fwd", "cce_bwd", "ce_logits_fwd", "ce_logits_bwd", "ce_logits_fwd_bwd",
                          "distill_logits_fwd", "distill_logits_bwd", "distill_fwd", "distill_bwd", "top_logits",
-                         "layer_norm_fwd", "layer_norm_bwd"})
+                         "layer_norm_fwd", "layer_norm_bwd", "token_logprobs_fwd", "token_logprobs_bwd",
+                         "linear_token_logprobs_fwd", "linear_token_logprobs_bwd", "rms_norm_fwd", "rms_norm_quantized",
+                         "rms_norm_bwd"})
     m.impl(op, torch::autograd::autogradNotImplementedFallback());
 }

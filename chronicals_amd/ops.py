@@ -43,7 +43,9 @@ from . import build as _build
 
 __all__ = ["cce_fwd", "cce_bwd", "ce_logits_fwd", "ce_logits_bwd", "ce_logits_bwd_", "ce_logits_fwd_bwd",
            "ce_logits_fwd_bwd_", "distill_logits_fwd", "distill_logits_bwd", "distill_fwd", "distill_bwd", "top_logits",
-           "layer_norm_fwd", "layer_norm_bwd", "layer_norm", "distill_logits", "distill_linear"]
+           "layer_norm_fwd", "layer_norm_bwd", "layer_norm", "distill_logits", "distill_linear", "token_logprobs_fwd",
+           "token_logprobs_bwd", "linear_token_logprobs_fwd", "linear_token_logprobs_bwd", "rms_norm_fwd",
+           "rms_norm_quantized", "rms_norm_bwd", "token_logprobs", "linear_token_logprobs", "rms_norm"]
 
 _SCHEMAS = (
     "cce_fwd(Tensor hidden, Tensor weight, Tensor labels, Tensor? bias, SymInt ignore_index, float label_smoothing, "
@@ -75,6 +77,20 @@ _SCHEMAS = (
     "layer_norm_fwd(Tensor x, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor, Tensor)",
     "layer_norm_bwd(Tensor grad_y, Tensor x, Tensor? weight, Tensor mean, Tensor rstd, bool param_f32, "
     "bool need_dx, bool need_dw, bool need_db) -> (Tensor, Tensor, Tensor)",
+    "token_logprobs_fwd(Tensor logits, Tensor tokens, float temperature, SymInt top_k, SymInt ignore_index) "
+    "-> (Tensor, Tensor, Tensor, Tensor, Tensor)",
+    "token_logprobs_bwd(Tensor? grad_logprobs, Tensor? grad_entropy, Tensor logits, Tensor tokens, Tensor stats, "
+    "float temperature, SymInt ignore_index) -> Tensor",
+    "linear_token_logprobs_fwd(Tensor hidden, Tensor weight, Tensor? bias, Tensor tokens, float temperature, "
+    "SymInt top_k, SymInt ignore_index) -> (Tensor, Tensor, Tensor, Tensor, Tensor)",
+    "linear_token_logprobs_bwd(Tensor? grad_logprobs, Tensor? grad_entropy, Tensor hidden, Tensor weight, Tensor? bias, "
+    "Tensor tokens, Tensor stats, float temperature, SymInt ignore_index, SymInt chunk_size, bool need_dh, bool need_dw, "
+    "bool need_db, bool dh_f32, bool dw_f32) -> (Tensor, Tensor, Tensor)",
+    "rms_norm_fwd(Tensor x, Tensor? weight, Tensor? residual, float eps) -> (Tensor, Tensor, Tensor)",
+    "rms_norm_quantized(Tensor x, Tensor? weight, Tensor? residual, float eps, bool int8, SymInt group) "
+    "-> (Tensor, Tensor, Tensor)",
+    "rms_norm_bwd(Tensor grad_y, Tensor? grad_sum, Tensor sum, Tensor? weight, Tensor rstd, bool param_f32, bool need_dx, "
+    "bool need_dr, bool need_dw) -> (Tensor, Tensor, Tensor)",
 )
 # differentiable, made of the operators above
 _COMPOSITE = (
@@ -84,6 +100,11 @@ _COMPOSITE = (
     "distill_linear(Tensor hidden, Tensor weight, Tensor? bias, Tensor teacher_logits, Tensor teacher_indices, "
     "Tensor? labels, int chunk_size, float temperature, float distill_weight, float ce_weight, int ignore_index, "
     "int reduction) -> Tensor",
+    "token_logprobs(Tensor logits, Tensor tokens, float temperature, int top_k, int ignore_index) "
+    "-> (Tensor, Tensor, Tensor, Tensor)",
+    "linear_token_logprobs(Tensor hidden, Tensor weight, Tensor? bias, Tensor tokens, int chunk_size, "
+    "float temperature, int top_k, int ignore_index) -> (Tensor, Tensor, Tensor, Tensor)",
+    "rms_norm(Tensor x, Tensor? weight, Tensor? residual, float eps) -> (Tensor, Tensor)",
 )
 _LIBRARY = torch.library.Library("chronicals_hip", "FRAGMENT")
 for _s in _SCHEMAS + _COMPOSITE:
@@ -352,6 +373,70 @@ def _layer_norm_bwd_fake(grad_y, x, weight, mean, rstd, param_f32, need_dx, need
             x.new_empty((x.shape[1] if need_db else 0,), dtype=params))
 
 
+# ---------------------------------------------------------------------------
+# Token log-probabilities (cce_token_logprobs_*, cce_linear_token_logprobs_*) and RMS
+# norm (cce_rms_norm_*); all in C++.
+#
+# The forwards return (logprobs, entropy, stats, top_logprobs, top_indices); stats is
+# for the backward of the same operands.  tokens [N] is contiguous.  rms_norm_fwd
+# returns (y, sum, rstd) and rms_norm_quantized (q, scales, sum), sum empty without a
+# residual; rms_norm_bwd's `sum` is x then, and its residual's gradient is empty
+# unless the residual has another type than x.  token_logprobs, linear_token_logprobs
+# and rms_norm are the differentiable ones over these, for tensors of any leading
+# shape.
+# ---------------------------------------------------------------------------
+
+def _logprobs_fake(x, top_k):
+    N = x.shape[0]
+    return (*(x.new_empty((N,), dtype=torch.float32) for _ in range(2)), x.new_empty((N, 4), dtype=torch.float32),
+            x.new_empty((N, top_k), dtype=torch.float32), x.new_empty((N, top_k), dtype=torch.int64))
+
+
+@torch.library.register_fake("chronicals_hip::token_logprobs_fwd", lib=_LIBRARY)
+def _token_logprobs_fwd_fake(logits, tokens, temperature, top_k, ignore_index):
+    return _logprobs_fake(logits, top_k)
+
+
+@torch.library.register_fake("chronicals_hip::token_logprobs_bwd", lib=_LIBRARY)
+def _token_logprobs_bwd_fake(grad_logprobs, grad_entropy, logits, *args):
+    return logits.new_empty(tuple(logits.shape))
+
+
+@torch.library.register_fake("chronicals_hip::linear_token_logprobs_fwd", lib=_LIBRARY)
+def _linear_token_logprobs_fwd_fake(hidden, weight, bias, tokens, temperature, top_k, ignore_index):
+    return _logprobs_fake(hidden, top_k)
+
+
+@torch.library.register_fake("chronicals_hip::linear_token_logprobs_bwd", lib=_LIBRARY)
+def _linear_token_logprobs_bwd_fake(grad_logprobs, grad_entropy, hidden, weight, bias, tokens, stats, temperature,
+                                    ignore_index, chunk_size, need_dh, need_dw, need_db, dh_f32, dw_f32):
+    return _cce_bwd_fake(None, hidden, weight, tokens, stats, None, bias, ignore_index, 0.0, 0.0, 0, chunk_size, need_dh,
+                         need_dw, need_db, dh_f32, dw_f32)
+
+
+def _sum_fake(x, residual):
+    return x.new_empty((0,)) if residual is None else residual.new_empty(tuple(x.shape))
+
+
+@torch.library.register_fake("chronicals_hip::rms_norm_fwd", lib=_LIBRARY)
+def _rms_norm_fwd_fake(x, weight, residual, eps):
+    return x.new_empty(tuple(x.shape)), _sum_fake(x, residual), x.new_empty((x.shape[0],), dtype=torch.float32)
+
+
+@torch.library.register_fake("chronicals_hip::rms_norm_quantized", lib=_LIBRARY)
+def _rms_norm_quantized_fake(x, weight, residual, eps, int8, group):
+    N, D = x.shape
+    return (x.new_empty((N, D), dtype=torch.int8 if int8 else torch.float8_e4m3fn),
+            x.new_empty((N, (D + group - 1) // group) if group else (N,), dtype=torch.float32), _sum_fake(x, residual))
+
+
+@torch.library.register_fake("chronicals_hip::rms_norm_bwd", lib=_LIBRARY)
+def _rms_norm_bwd_fake(grad_y, grad_sum, sum, weight, rstd, param_f32, need_dx, need_dr, need_dw):
+    shape = tuple(grad_y.shape)
+    return (grad_y.new_empty(shape if need_dx else (0,)), sum.new_empty(shape if need_dr else (0,)),
+            grad_y.new_empty((shape[1] if need_dw else 0,), dtype=torch.float32 if param_f32 else grad_y.dtype))
+
+
 cce_fwd = torch.ops.chronicals_hip.cce_fwd
 cce_bwd = torch.ops.chronicals_hip.cce_bwd
 ce_logits_fwd = torch.ops.chronicals_hip.ce_logits_fwd
@@ -367,3 +452,13 @@ layer_norm_bwd = torch.ops.chronicals_hip.layer_norm_bwd
 layer_norm = torch.ops.chronicals_hip.layer_norm
 distill_logits = torch.ops.chronicals_hip.distill_logits
 distill_linear = torch.ops.chronicals_hip.distill_linear
+token_logprobs_fwd = torch.ops.chronicals_hip.token_logprobs_fwd
+token_logprobs_bwd = torch.ops.chronicals_hip.token_logprobs_bwd
+linear_token_logprobs_fwd = torch.ops.chronicals_hip.linear_token_logprobs_fwd
+linear_token_logprobs_bwd = torch.ops.chronicals_hip.linear_token_logprobs_bwd
+rms_norm_fwd = torch.ops.chronicals_hip.rms_norm_fwd
+rms_norm_quantized = torch.ops.chronicals_hip.rms_norm_quantized
+rms_norm_bwd = torch.ops.chronicals_hip.rms_norm_bwd
+token_logprobs = torch.ops.chronicals_hip.token_logprobs
+linear_token_logprobs = torch.ops.chronicals_hip.linear_token_logprobs
+rms_norm = torch.ops.chronicals_hip.rms_norm

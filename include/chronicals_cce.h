@@ -43,7 +43,7 @@
 extern "C" {
 #endif
 
-#define CCE_ABI_VERSION 9
+#define CCE_ABI_VERSION 10
 
 #define CCE_OK 0
 #define CCE_ERR_INVALID_ARG 1
@@ -59,6 +59,9 @@ extern "C" {
 #define CCE_DTYPE_BF16 0
 #define CCE_DTYPE_F32 1
 #define CCE_DTYPE_F16 2
+/* 8-bit outputs of cce_rms_norm_quantized */
+#define CCE_DTYPE_E4M3 3 /* OCP e4m3: largest finite value 448 */
+#define CCE_DTYPE_INT8 4
 
 /* label-smoothing forms of the logits-in entry points */
 #define CCE_SMOOTH_LOGV 0    /* eps*log(V) (cut_cross_entropy.py:1237-1239)                   */
@@ -355,6 +358,89 @@ int cce_layer_norm_backward(const void* grad_y, const void* x, int dtype, int64_
                             int param_dtype, const float* mean, const float* rstd, int64_t N, int64_t D, void* grad_x,
                             void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes,
                             void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Log-probabilities of given tokens, with the entropy and the largest alternatives
+ * of each row.  No reference counterpart.  With z = x / temperature:
+ *   logprobs_out[n] = z[token] - logsumexp(z)
+ *   entropy_out[n]  = -sum_v p_v log p_v,  p = softmax(z)
+ *   the top_k largest logits (0 .. min(V, CCE_MAX_TEACHER_ENTRIES); ordered as by
+ *   cce_top_logits): their columns [N][top_k] and z - logsumexp(z) there
+ * A row whose token is ignore_index gives 0 (columns: -1) and a zero gradient, whatever
+ * it holds.  A token outside [0, V) that is not ignore_index has no log-probability: 0,
+ * without a gradient.  Where every logit is -inf the log-probabilities are -inf, the
+ * entropy 0 and the gradient 0.  The temperature is in [0.01, 1000].
+ *
+ * The backward takes the gradients of logprobs_out and entropy_out ([N] each; NULL:
+ * none) and stats_out ([N][4], 16-byte aligned) of the forward of the same form:
+ *   dx_v = (g ([v == token] - p_v) - h p_v (log p_v + entropy)) / temperature
+ */
+
+/* Over logits that exist: [N][ld], of logits_dtype.  grad_logits has the logits'
+ * dtype, any row stride, and is not the logits. */
+int cce_token_logprobs_workspace_bytes(int64_t N, int64_t V, int64_t top_k, size_t* bytes);
+int cce_token_logprobs_forward(const void* logits, int logits_dtype, int64_t ld, const void* tokens, int tokens_int64,
+                               int64_t N, int64_t V, int64_t ignore_index, float temperature, int64_t top_k,
+                               float* logprobs_out, float* entropy_out, float* stats_out, float* top_logprobs_out,
+                               int64_t* top_indices_out, void* workspace, size_t workspace_bytes, void* stream);
+int cce_token_logprobs_backward(const float* grad_logprobs, const float* grad_entropy, const void* logits,
+                                int logits_dtype, int64_t ld, const void* tokens, int tokens_int64, const float* stats,
+                                int64_t N, int64_t V, int64_t ignore_index, float temperature, void* grad_logits,
+                                int64_t ld_grad, void* stream);
+
+/* Fused with the head's product, x = hidden . weight^T + bias, operands as
+ * cce_forward's and cce_backward's (the rows of hidden that do not count are finite:
+ * the backward's products run over them with zero coefficients).  With top_k the logits
+ * of a block of rows are in the workspace, at most 512 MiB of them (or 256 rows, if
+ * that is more); without, none are stored. */
+int cce_linear_token_logprobs_workspace_bytes(int64_t N, int64_t d, int64_t V, int64_t top_k, size_t* bytes);
+int cce_linear_token_logprobs_forward(const void* hidden, const void* weight, const float* bias, const void* tokens,
+                                      int tokens_int64, int64_t N, int64_t d, int64_t V, int64_t ignore_index,
+                                      float temperature, int64_t top_k, float* logprobs_out, float* entropy_out,
+                                      float* stats_out, float* top_logprobs_out, int64_t* top_indices_out,
+                                      void* workspace, size_t workspace_bytes, void* stream);
+int cce_linear_token_logprobs_backward_workspace_bytes(int64_t N, int64_t d, int64_t V, int64_t chunk_size,
+                                                       int need_grad_hidden, int grad_hidden_dtype,
+                                                       int need_grad_weight, int grad_weight_dtype, size_t* bytes);
+int cce_linear_token_logprobs_backward(const float* grad_logprobs, const float* grad_entropy, const void* hidden,
+                                       const void* weight, const float* bias, const void* tokens, int tokens_int64,
+                                       const float* stats, int64_t N, int64_t d, int64_t V, int64_t ignore_index,
+                                       float temperature, int64_t chunk_size, void* grad_hidden, int grad_hidden_dtype,
+                                       void* grad_weight, int grad_weight_dtype, float* grad_bias, void* workspace,
+                                       size_t workspace_bytes, void* stream);
+
+/*
+ * Root-mean-square norm over rows of D elements, D <= 2^20, with the addition of a
+ * residual (NULL: none):
+ *   sum = x + residual, rounded to the residual's dtype (x's or fp32) and written to
+ *   sum_out;  y = sum * rstd * weight, rstd = 1 / sqrt(mean(sum^2) + eps)
+ * x and residual have row strides; sum_out and y_out (of x's dtype) are contiguous and
+ * overlap no input.  weight (NULL: ones) and its gradient are of param_dtype, which is
+ * x's or fp32; statistics are fp32, rstd_out [N].  Without a residual residual_dtype is
+ * x's or fp32 and nothing else is made of it.
+ *
+ * The quantized form writes y in 8 bits, with a scale per row (group 0, scales_out [N])
+ * or per `group` columns (32, 64, 128 or 256; scales_out [N][ceil(D / group)]):
+ *   scale = max(largest |y|, 1e-30) / M,  q = round(y / scale) to nearest even,
+ *   M = 448 (CCE_DTYPE_E4M3) or 127 (CCE_DTYPE_INT8)
+ * A NaN in a group makes its scale a NaN.
+ *
+ * The backward takes the gradients of y and (NULL: none) of sum, and sum itself: without
+ * a residual that is x.  grad_x and grad_residual are the same numbers in the dtypes of
+ * x and of sum; NULL leaves one out, and grad_weight.  The workspace is what the query
+ * gives (0 bytes, which may be NULL, without grad_weight).  No reference counterpart.
+ */
+int cce_rms_norm_forward(const void* x, int dtype, int64_t ldx, const void* residual, int residual_dtype, int64_t ldr,
+                         const void* weight, int param_dtype, int64_t N, int64_t D, float eps, void* y_out, void* sum_out,
+                         float* rstd_out, void* stream);
+int cce_rms_norm_quantized(const void* x, int dtype, int64_t ldx, const void* residual, int residual_dtype, int64_t ldr,
+                           const void* weight, int param_dtype, int64_t N, int64_t D, float eps, int q_dtype,
+                           int64_t group, void* q_out, float* scales_out, void* sum_out, void* stream);
+int cce_rms_norm_backward_workspace_bytes(int64_t N, int64_t D, int dtype, int need_grad_weight, size_t* bytes);
+int cce_rms_norm_backward(const void* grad_y, const void* grad_sum, const void* sum, int dtype, int sum_dtype,
+                          int64_t ld_sum, const void* weight, int param_dtype, const float* rstd, int64_t N, int64_t D,
+                          void* grad_x, void* grad_residual, void* grad_weight, void* workspace, size_t workspace_bytes,
+                          void* stream);
 
 /*
  * Per-kernel timing for measurement tools (no counterpart in the reference).
