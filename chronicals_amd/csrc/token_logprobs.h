@@ -44,19 +44,29 @@ struct LpSums {
     s += e;
     w = __builtin_fmaf(e, fmaxf(u, kLeastExponent), w);  // a NaN stays in e
   }
-  template <typename T>
-  __device__ inline void add_chunk(const u32x4& raw, float scale) {
+  // U chunks at once: one change of the maximum for all
+  template <typename T, int U>
+  __device__ inline void add_chunks(const u32x4 (&raw)[U], float scale) {
     constexpr int E = 16 / sizeof(T);
-    const T* v = reinterpret_cast<const T*>(&raw);
-    float x[E], mx = m;
+    float mx = m;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      x[e] = elem_to_f32(v[e]);
-      mx = fmaxf(mx, x[e]);
+    for (int u = 0; u < U; ++u) {
+      const T* v = reinterpret_cast<const T*>(&raw[u]);
+#pragma unroll
+      for (int e = 0; e < E; ++e) mx = fmaxf(mx, elem_to_f32(v[e]));
     }
     rescale(mx, scale);
 #pragma unroll
-    for (int e = 0; e < E; ++e) add(x[e], scale);
+    for (int u = 0; u < U; ++u) {
+      const T* v = reinterpret_cast<const T*>(&raw[u]);
+#pragma unroll
+      for (int e = 0; e < E; ++e) add(elem_to_f32(v[e]), scale);
+    }
+  }
+  template <typename T>
+  __device__ inline void add_chunk(const u32x4& raw, float scale) {
+    const u32x4 one[1] = {raw};
+    add_chunks<T, 1>(one, scale);
   }
   __device__ inline void add_one(float x, float scale) {
     rescale(fmaxf(m, x), scale);
@@ -167,8 +177,16 @@ __global__ __launch_bounds__(256) void lp_stream_kernel(const T* __restrict__ X,
   LpSums k;
   if (tid < sp.head) k.add_one(elem_to_f32(row[tid]), a.scale);
   if (tid < c1 - c0 - sp.tail_start) k.add_one(elem_to_f32(row[sp.tail_start + tid]), a.scale);
-  for_each_chunk(reinterpret_cast<const u32x4*>(row + sp.head), sp.chunks, tid,
-                 [&](int, const u32x4& raw) { k.template add_chunk<T>(raw, a.scale); });
+  const u32x4* const body = reinterpret_cast<const u32x4*>(row + sp.head);
+  constexpr int U = 4;
+  int c = tid;
+  for (; c + (U - 1) * 256 < sp.chunks; c += U * 256) {
+    u32x4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = __builtin_nontemporal_load(body + c + u * 256);
+    k.template add_chunks<T, U>(raw, a.scale);
+  }
+  for (; c < sp.chunks; c += 256) k.template add_chunk<T>(__builtin_nontemporal_load(body + c), a.scale);
   k.merge_block(a.scale, red);
   if (tid != 0) return;
   if (S == 1)

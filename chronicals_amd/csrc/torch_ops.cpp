@@ -149,8 +149,11 @@ const float* bias_ptr(const optional<Tensor>& bias) {
   return bias.has_value() ? static_cast<const float*>(bias->data_ptr()) : nullptr;
 }
 
-// A per-row or scalar gradient as contiguous fp32.
-Tensor grad_rows(const Tensor& g) { return g.detach().to(at::kFloat).reshape({-1}).contiguous(); }
+// A per-row or scalar gradient as contiguous fp32 (most are: four calls of torch's less).
+Tensor grad_rows(const Tensor& g) {
+  if (g.dim() == 1 && g.scalar_type() == at::kFloat && g.is_contiguous()) return g;
+  return g.detach().to(at::kFloat).reshape({-1}).contiguous();
+}
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> cce_fwd(const Tensor& hidden_, const Tensor& weight_, const Tensor& labels_,
                                                    const optional<Tensor>& bias, int64_t ignore_index,
@@ -802,6 +805,15 @@ optional<Tensor> contiguous(const optional<Tensor>& t) { return t.has_value() ? 
 // _unsafe_view elsewhere, counts as none, and nothing else holds its storage.
 Tensor scalar(const Tensor& t) { return at::_unsafe_view(t, at::IntArrayRef()); }
 
+// An operator's call without the dispatcher's autograd step, whose boxed "no derivative"
+// kernel costs a few microseconds: an autograd function's forward and backward run
+// with gradients off as they are.
+template <typename F>
+auto below_autograd(F&& call) {
+  const at::AutoDispatchBelowAutograd guard;
+  return call();
+}
+
 // The body of a backward: the gradients are computed without a graph of their own.
 // Where one is asked for (create_graph), they lead to what the function's inputs
 // and its incoming gradients came from, through a node that raises.  Without it
@@ -998,7 +1010,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     static const auto fwd =
         find<FiveTensors(const Tensor&, const Tensor&, double, SymInt, SymInt)>("chronicals_hip::token_logprobs_fwd");
     const Tensor x = as_rows(logits);
-    const FiveTensors r = fwd.call(x, tokens, temperature, top_k, ignore_index);
+    const FiveTensors r = below_autograd([&] { return fwd.call(x, tokens, temperature, top_k, ignore_index); });
     ctx->save_for_backward({x, tokens, std::get<2>(r)});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["ignore_index"] = ignore_index;
@@ -1014,8 +1026,10 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     return gradients({grads[0], grads[1]}, [&] {
       variable_list out(5);
       const auto s = ctx->get_saved_variables();
-      out[0] = bwd.call(given(grads[0]), given(grads[1]), s[0], s[1], s[2], ctx->saved_data["temperature"].toDouble(),
+      out[0] = below_autograd([&] {
+        return bwd.call(given(grads[0]), given(grads[1]), s[0], s[1], s[2], ctx->saved_data["temperature"].toDouble(),
                         ctx->saved_data["ignore_index"].toInt());
+      });
       if (ctx->saved_data["dim"].toInt() != 2) out[0] = out[0].view_symint(ctx->saved_data["shape"].toSymIntVector());
       return out;
     });
@@ -1037,7 +1051,8 @@ struct LinearTokenLogprobs : torch::autograd::Function<LinearTokenLogprobs> {
     // fp16 and fp32 operands are rounded to bf16, the GEMMs' type
     const Tensor h = as_rows(hidden).to(at::kBFloat16).contiguous(), w = weight.to(at::kBFloat16).contiguous();
     const Tensor b = bias.has_value() ? bias->to(at::kFloat).contiguous() : Tensor();
-    const FiveTensors r = fwd.call(h, w, given(b), tokens, temperature, top_k, ignore_index);
+    const FiveTensors r =
+        below_autograd([&] { return fwd.call(h, w, given(b), tokens, temperature, top_k, ignore_index); });
     ctx->save_for_backward({h, w, b, tokens, std::get<2>(r)});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["ignore_index"] = ignore_index;
@@ -1062,10 +1077,11 @@ struct LinearTokenLogprobs : torch::autograd::Function<LinearTokenLogprobs> {
       auto& kept = ctx->saved_data;
       const auto htype = (at::ScalarType)kept["hidden"].toInt(), wtype = (at::ScalarType)kept["weight"].toInt();
       // bf16 inputs get bf16 gradients, fp16 and fp32 inputs get them from fp32
-      const auto [dh, dw, db] =
-          bwd.call(given(grads[0]), given(grads[1]), s[0], s[1], given(s[2]), s[3], s[4], kept["temperature"].toDouble(),
-                   kept["ignore_index"].toInt(), kept["chunk_size"].toInt(), need_dh, need_dw, need_db,
-                   htype != at::kBFloat16, wtype != at::kBFloat16);
+      const auto [dh, dw, db] = below_autograd([&] {
+        return bwd.call(given(grads[0]), given(grads[1]), s[0], s[1], given(s[2]), s[3], s[4],
+                        kept["temperature"].toDouble(), kept["ignore_index"].toInt(), kept["chunk_size"].toInt(), need_dh,
+                        need_dw, need_db, htype != at::kBFloat16, wtype != at::kBFloat16);
+      });
       if (need_dh) out[0] = dh.view_symint(kept["shape"].toSymIntVector()).to(htype);
       if (need_dw) out[1] = dw.to(wtype);
       if (need_db) out[2] = db.to((at::ScalarType)kept["bias"].toInt());
@@ -1091,7 +1107,8 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
         "chronicals_hip::rms_norm_fwd");
     const Tensor rows = as_rows(x);
     const bool has_r = residual.has_value();
-    const auto [y, sum, rstd] = fwd.call(rows, weight, has_r ? optional<Tensor>(as_rows(*residual)) : residual, eps);
+    const optional<Tensor> r = has_r ? optional<Tensor>(as_rows(*residual)) : residual;
+    const auto [y, sum, rstd] = below_autograd([&] { return fwd.call(rows, weight, r, eps); });
     auto shaped = [&](const Tensor& t) { return x.dim() == 2 ? t : at::_unsafe_view_symint(t, x.sym_sizes()); };
     variable_list out = {shaped(y), has_r ? shaped(sum) : sum};
     ctx->save_for_backward({has_r ? out[1] : rows, weight.value_or(Tensor()), rstd});
@@ -1120,9 +1137,11 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
       const Tensor g = grads[0].defined()
                            ? rows(grads[0])
                            : at::zeros_symint(sum.sym_sizes(), sum.options().dtype((at::ScalarType)kept["x"].toInt()));
-      const auto [dx, dr, dw] =
-          bwd.call(g, grads[1].defined() ? optional<Tensor>(rows(grads[1])) : std::nullopt, sum, given(saved[1]), saved[2],
-                   has_w && saved[1].scalar_type() == at::kFloat, need_x || (need_r && same), need_r && !same, need_dw);
+      const optional<Tensor> gs = grads[1].defined() ? optional<Tensor>(rows(grads[1])) : std::nullopt;
+      const auto [dx, dr, dw] = below_autograd([&] {
+        return bwd.call(g, gs, sum, given(saved[1]), saved[2], has_w && saved[1].scalar_type() == at::kFloat,
+                        need_x || (need_r && same), need_r && !same, need_dw);
+      });
       auto out = [&](const Tensor& t) { return t.view_symint(shaped.sym_sizes()); };
       // of one type the two gradients are one
       return {need_x ? out(dx) : Tensor(), need_dw ? dw : Tensor(), need_r ? out(same ? dx : dr) : Tensor(), Tensor()};
