@@ -139,7 +139,7 @@ struct DistillGrad {
 __device__ inline float mantissa(float x) { return __uint_as_float((__float_as_uint(x) & 0x007fffffu) | 0x3f800000u); }
 __device__ inline float unit_of(const Teacher& a, float g) { return mantissa(g * (a.ce != 0.f ? a.ce : a.kdg)); }
 
-// The largest finite magnitude of v[0, N), by a workgroup of 1024; thread 0 gets it.
+// The largest finite magnitude of v[0, N), by a workgroup of 1024.
 __device__ inline float largest_finite(const float* __restrict__ v, int N) {
   __shared__ float red[16];
   float g = 0.f;
@@ -248,7 +248,7 @@ int distill_forward_run(const bf16_t* H, const bf16_t* W, const float* bias, lon
   if (F.idx) {
     hipLaunchKernelGGL(kd_rows_kernel, dim3((unsigned)ceil_div(N, 4)), dim3(256), 0, st, a, (int)N, (int)V, rows);
     HIP_TRY(hipGetLastError());
-    const int rc = order_rows(rows, 0, -1L, H, N, d, V, slots, F, st);
+    const int rc = order_rows(rows, 0, -1L, H, N, d, (int)ceil_div(V, kBN), slots, F, st);
     if (rc) return rc;
   }
   const GemmShape g = forward_shape(H, W, N, d, V, F);

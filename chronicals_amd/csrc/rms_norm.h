@@ -15,36 +15,48 @@
 // Rows stay in registers as in layer_norm.h, whose shapes these are; longer rows go by
 // the kernels further below, which read them two or three times.
 
-// A row of type S, in the chunks that RowRegs<T, TR, C> holds (16 bytes of T, so fp32
-// beside a 16-bit T takes two loads a chunk), as fp32; 0 past the row's end.
+// A row of type S on its way, in the chunks that RowRegs<T, TR, C> holds: 16 bytes of
+// T, so fp32 beside a 16-bit T takes two loads a chunk.
 template <typename T, typename S, int TR, int C>
-__device__ inline void load_chunks(float (&v)[C][16 / sizeof(T)], const S* row, int D, int t) {
-  constexpr int E = 16 / sizeof(T), ES = 16 / sizeof(S);
-  u32x4 raw[C][E / ES];
+struct RawChunks {
+  static constexpr int E = 16 / sizeof(T), ES = 16 / sizeof(S);
+  u32x4 v[C][E / ES];
+  __device__ inline void issue(const S* row, int D, int t) {
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int at = RowRegs<T, TR, C>::first(c, t);
+    for (int c = 0; c < C; ++c) {
+      const int at = RowRegs<T, TR, C>::first(c, t);
 #pragma unroll
-    for (int i = 0; i < E / ES; ++i) {
-      raw[c][i] = u32x4{0u, 0u, 0u, 0u};
-      if (at + E <= D) raw[c][i] = __builtin_nontemporal_load(reinterpret_cast<const loose_u32x4*>(row + at + i * ES));
+      for (int i = 0; i < E / ES; ++i) {
+        v[c][i] = u32x4{0u, 0u, 0u, 0u};
+        if (at + E <= D) v[c][i] = __builtin_nontemporal_load(reinterpret_cast<const loose_u32x4*>(row + at + i * ES));
+      }
     }
   }
+  // as fp32; 0 past the row's end
+  __device__ inline void take(float (&x)[C][E], const S* row, int D, int t) const {
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const S* e = reinterpret_cast<const S*>(raw[c]);
+    for (int c = 0; c < C; ++c) {
+      const S* e = reinterpret_cast<const S*>(v[c]);
 #pragma unroll
-    for (int i = 0; i < E; ++i) v[c][i] = elem_to_f32(e[i]);
+      for (int i = 0; i < E; ++i) x[c][i] = elem_to_f32(e[i]);
+    }
+    if (D % E == 0) return;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int at = RowRegs<T, TR, C>::first(c, t);
+      if (at >= D || at + E <= D) continue;
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (at + i < D) x[c][i] = elem_to_f32(row[at + i]);
+    }
   }
-  if (D % E == 0) return;
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int at = RowRegs<T, TR, C>::first(c, t);
-    if (at >= D || at + E <= D) continue;
-#pragma unroll
-    for (int i = 0; i < E; ++i)
-      if (at + i < D) v[c][i] = elem_to_f32(row[at + i]);
-  }
+};
+
+template <typename T, typename S, int TR, int C>
+__device__ inline void load_chunks(float (&v)[C][16 / sizeof(T)], const S* row, int D, int t) {
+  RawChunks<T, S, TR, C> raw;
+  raw.issue(row, D, t);
+  raw.take(v, row, D, t);
 }
 
 template <typename T, typename S, int TR, int C>
@@ -223,11 +235,27 @@ __global__ __launch_bounds__(TR < 256 ? 256 : TR) void rms_bwd_rows_kernel(
   Row wr;
   wr.load_params(w, param_f32, D, t, 1.f);
   float sw[C][E] = {};
-  for (long n = (long)blockIdx.x * kRows + threadIdx.x / TR; n < N; n += (long)gridDim.x * kRows) {
+  const long step = (long)gridDim.x * kRows;
+  long n = (long)blockIdx.x * kRows + threadIdx.x / TR;
+  RawChunks<T, S, TR, C> raw_x;
+  RawChunks<T, T, TR, C> raw_g;
+  float next_r = 0.f;
+  auto issue = [&](long m) {
+    raw_x.issue(sum + m * lds, D, t);
+    raw_g.issue(dY + m * D, D, t);
+    next_r = rstd[m];
+  };
+  constexpr bool kAhead = TR < 1024;  // as in layer_norm_bwd_rows_kernel
+  if (kAhead && n < N) issue(n);
+  for (; n < N; n += step) {
+    if (!kAhead) issue(n);
     float x[C][E], g[C][E];
-    load_chunks<T, S, TR, C>(x, sum + n * lds, D, t);
-    load_chunks<T, T, TR, C>(g, dY + n * D, D, t);
-    const float r = rstd[n];
+    raw_x.take(x, sum + n * lds, D, t);
+    raw_g.take(g, dY + n * D, D, t);
+    const float r = next_r;
+    RawChunks<T, S, TR, C> raw_s;
+    if (dS) raw_s.issue(dS + n * D, D, t);
+    if (kAhead && n + step < N) issue(n + step);  // the next row, while this one is worked on
     float san = 0.f;
 #pragma unroll
     for (int c = 0; c < C; ++c)
@@ -245,7 +273,7 @@ __global__ __launch_bounds__(TR < 256 ? 256 : TR) void rms_bwd_rows_kernel(
 #pragma unroll
       for (int i = 0; i < E; ++i) x[c][i] = r * __builtin_fmaf(-x[c][i], san, g[c][i]);
     if (dS) {
-      load_chunks<T, S, TR, C>(g, dS + n * D, D, t);
+      raw_s.take(g, dS + n * D, D, t);
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -415,9 +443,33 @@ int check_rms(int64_t N, int64_t D, int dtype, int64_t ldx, int rdtype, int64_t 
   return CCE_OK;
 }
 
-// Parts of dw, as layer norm's backward has them, without its db.
+// The backward's shapes are layer norm's, but for rows of a workgroup that would hold
+// 32 elements a thread (16-bit types past 4096): with the next row's loads beside they
+// take 250 registers, and the barriers of a row find one other workgroup on the CU.
+// 1024 threads of 16 elements, 4096 x 8192 bf16: 70 -> 63 us.  Waves of 32 elements
+// stay (16384 x 2048 63 us, by 256 threads of 16 70), and 256 threads of 16 (8192 x
+// 4096 fp32 92 us, by 1024 98).
+template <int E, int kMost, typename F>
+bool rms_bwd_shape(long D, F&& f) {
+  if (E == 8 && D > 256 * 2 * E && D <= 1024 * 2 * E) {
+    f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 2>{});
+    return true;
+  }
+  return norm_shape<E, kMost>(D, f);
+}
+
+// Parts of dw, one per workgroup of the backward.
+long rms_parts(int dtype, long N, long D) {
+  int threads = 256;
+  auto shape = [&](auto tr, auto) { threads = decltype(tr)::value; };
+  if (dtype == CCE_DTYPE_F32)
+    rms_bwd_shape<4, kNormRegD>(D, shape);
+  else
+    rms_bwd_shape<8, kNormRegD>(D, shape);
+  return norm_parts(N, D, threads);
+}
 size_t rms_bytes(int dtype, long N, long D, bool need_dw) {
-  return need_dw ? align_up((size_t)(norm_parts(N, D, norm_threads(dtype, D)) * D) * sizeof(float), 256) : 0;
+  return need_dw ? align_up((size_t)(rms_parts(dtype, N, D) * D) * sizeof(float), 256) : 0;
 }
 
 template <bool Q>
@@ -452,8 +504,8 @@ int rms_backward(const void* dy, const void* ds, const void* sum, int dtype, int
     typedef decltype(s) S;
     if (!dx && !dr && !dw) return CCE_OK;
     const int f32 = wdtype == CCE_DTYPE_F32;
-    const long parts = norm_parts(N, D, norm_threads(dtype, D));
-    const bool in_registers = norm_shape<16 / sizeof(T), kNormRegD>(D, [&](auto tr, auto c) {
+    const long parts = rms_parts(dtype, N, D);
+    const bool in_registers = rms_bwd_shape<16 / sizeof(T), kNormRegD>(D, [&](auto tr, auto c) {
       constexpr int TR = decltype(tr)::value;
       hipLaunchKernelGGL((rms_bwd_rows_kernel<T, S, TR, decltype(c)::value>), dim3((unsigned)parts),
                          dim3(std::max(TR, 256)), 0, st, static_cast<const T*>(dy), static_cast<const S*>(ds),

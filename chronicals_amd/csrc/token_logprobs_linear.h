@@ -70,16 +70,24 @@ struct LpLinearGrad {
 
 // The unit of G (distill_linear.h): at a row's token G is nearly -g / T, so the
 // mantissa of the largest one, which all rows have where the gradient is a mean's.
+__device__ inline float lp_unit(const LpGrad& p, int N) {
+  return mantissa((p.g ? largest_finite(p.g, N) : 0.f) * p.inv_t);
+}
 __global__ __launch_bounds__(1024) void lp_unit_kernel(LpGrad p, int N, float* __restrict__ unit) {
-  const float g = p.g ? largest_finite(p.g, N) : 0.f;
-  if (threadIdx.x == 0) *unit = mantissa(g * p.inv_t);
+  const float u = lp_unit(p, N);
+  if (threadIdx.x == 0) *unit = u;
 }
 
-// Coefficients of GEMM row i, of source row idx[i] (null: i), in units of *unit.
-__global__ __launch_bounds__(256) void lp_linear_prep_kernel(LpLinearGrad q, const int* __restrict__ idx, int N,
-                                                             float4* __restrict__ rowp, int* __restrict__ rowlab,
-                                                             const float* __restrict__ unit) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
+// Coefficients of GEMM row i, of source row idx[i] (null: i), in units of *unit, which
+// every workgroup finds by itself where FIND (few rows: a launch less, 2 to 5 us).
+constexpr long kUnitRows = 16384;  // 16 workgroups that read 64 KB each
+template <bool FIND>
+__global__ __launch_bounds__(1024) void lp_linear_prep_kernel(LpLinearGrad q, const int* __restrict__ idx, int N,
+                                                              float4* __restrict__ rowp, int* __restrict__ rowlab,
+                                                              float* __restrict__ unit) {
+  const int i = blockIdx.x * 1024 + threadIdx.x;
+  const float u = FIND ? lp_unit(q.p, N) : *unit;
+  if (FIND && i == 0) *unit = u;
   if (i >= N) return;
   const long n = idx ? idx[i] : i;
   int col;
@@ -89,7 +97,6 @@ __global__ __launch_bounds__(256) void lp_linear_prep_kernel(LpLinearGrad q, con
   if (counts && st.y != FLT_MAX) {
     float c, b, at;
     q.p.row(n, col, st.z, c, b, at);
-    const float u = *unit;
     rp = make_float4(st.x + st.y, c / u, -at / u, b / u);
   } else {
     col = -1;
@@ -101,10 +108,12 @@ __global__ __launch_bounds__(256) void lp_linear_prep_kernel(LpLinearGrad q, con
 int lp_prep(const SparseGrad& s, const int* idx, long N, float4* rowp, int* rowlab, int*, float*, float* unit,
             hipStream_t st) {
   const LpLinearGrad& q = *static_cast<const LpLinearGrad*>(s.args);
-  hipLaunchKernelGGL(lp_unit_kernel, dim3(1), dim3(1024), 0, st, q.p, (int)N, unit);
-  HIP_TRY(hipGetLastError());
-  hipLaunchKernelGGL(lp_linear_prep_kernel, dim3((unsigned)ceil_div(N, 256)), dim3(256), 0, st, q, idx, (int)N, rowp,
-                     rowlab, unit);
+  if (N > kUnitRows) {
+    hipLaunchKernelGGL(lp_unit_kernel, dim3(1), dim3(1024), 0, st, q.p, (int)N, unit);
+    HIP_TRY(hipGetLastError());
+  }
+  hipLaunchKernelGGL((N > kUnitRows ? lp_linear_prep_kernel<false> : lp_linear_prep_kernel<true>),
+                     dim3((unsigned)ceil_div(N, 1024)), dim3(1024), 0, st, q, idx, (int)N, rowp, rowlab, unit);
   HIP_TRY(hipGetLastError());
   return CCE_OK;
 }
@@ -117,9 +126,18 @@ long logits_block(long N, long V) {
   return std::min<long>(std::max<long>(kLogitsBudget / (4 * logits_ld(V)) / kBM * kBM, kBM), std::max<long>(N, 1));
 }
 
+// Columns of the forward's vocabulary tiles: half as wide where twice as many still are
+// one round of workgroups (half_tiles).  64 x 896 x 32000 25 -> 19 us; 64 x 896 x 60000,
+// two rounds of halves, 33 -> 39.
+int lp_tile_width(long N, long V) { return half_tiles(ceil_div(N, kBM) * ceil_div(V, kBN)) ? kTailBN : kBN; }
+long lp_slots(long N, long V, bool compact) {
+  const int bn = lp_tile_width(N, V);
+  return bn == kBN ? forward_slots(N, V, compact) : ceil_div(std::max<long>(N, 1), kBM) * ceil_div(V, bn);
+}
+
 struct LpLinearLayout {
   FwdLayout f;
-  float* pw;
+  float *pm, *ps, *pw;  // a slot's maxima and sums
   float* logits;
   void* rows;  // workspace of a block's row kernels
   size_t bytes;
@@ -132,7 +150,7 @@ LpLinearLayout lp_linear_layout(void* ws, long N, long d, long V, long k) {
   c.off = L.f.bytes;
   if (k > 0) {
     const long R = logits_block(N, V);
-    L.pw = nullptr;
+    L.pm = L.ps = L.pw = nullptr;
     L.logits = c.take<float>((size_t)(R * logits_ld(V)));
     // the last block has fewer rows, which may be split over more workgroups
     const long last = N > 0 ? (N - 1) % R + 1 : 0;
@@ -140,7 +158,11 @@ LpLinearLayout lp_linear_layout(void* ws, long N, long d, long V, long k) {
     L.bytes = align_up(c.off, 256);
     return L;
   }
-  L.pw = c.take<float>((size_t)forward_slots(N, V, fwd_compacts(N, d, CCE_LSE_LABELLED_ROWS)) * kBM);
+  const size_t parts = (size_t)lp_slots(N, V, fwd_compacts(N, d, CCE_LSE_LABELLED_ROWS)) * kBM;
+  const bool whole = lp_tile_width(N, V) == kBN;  // the cross-entropy's slots
+  L.pm = whole ? L.f.pm : c.take<float>(parts);
+  L.ps = whole ? L.f.ps : c.take<float>(parts);
+  L.pw = c.take<float>(parts);
   L.logits = nullptr;
   L.rows = nullptr;
   L.bytes = align_up(c.off, 256);
@@ -159,8 +181,8 @@ int launch_out(const GemmShape& g, const OutParams& e, hipStream_t st) {
 int lp_linear_forward_run(const bf16_t* H, const bf16_t* W, const float* bias, long N, long d, long V, long k,
                           const Tokens& a, LpOut out, const LpLinearLayout& L, hipStream_t st) {
   const FwdLayout& F = L.f;
-  const int slots = (int)forward_slots(N, V, F.idx != nullptr);
-  int rc = order_rows(a.ids, a.ids64, a.ignore_index, H, N, d, V, slots, F, st);
+  const int slots = (int)lp_slots(N, V, F.idx != nullptr), bn = lp_tile_width(N, V);
+  int rc = order_rows(a.ids, a.ids64, a.ignore_index, H, N, d, (int)ceil_div(V, bn), slots, F, st);
   if (rc) return rc;
   GemmShape g = forward_shape(H, W, N, d, V, F);
   if (k > 0) {
@@ -196,16 +218,20 @@ int lp_linear_forward_run(const bf16_t* H, const bf16_t* W, const float* bias, l
   }
   LseParams ep;
   ep.bias = bias;
-  ep.pm = F.pm;
-  ep.ps = F.ps;
+  ep.pm = L.pm;
+  ep.ps = L.ps;
   ep.ps1 = L.pw;
   ep.ldp = N;
-  ep.splits = forward_splits(N, V);
-  ep.tiles_n = (int)ceil_div(V, kBN);
+  ep.tiles_n = (int)ceil_div(V, bn);
+  ep.splits = bn == kBN ? forward_splits(N, V) : ep.tiles_n;
   ep.scale = a.scale;
-  rc = bias ? launch_lse<EpiLseBiasEntropy>(g, ep, slots, st) : launch_lse<EpiLseEntropy>(g, ep, slots, st);
+  if (bn == kBN)
+    rc = bias ? launch_lse<EpiLseBiasEntropy>(g, ep, slots, st) : launch_lse<EpiLseEntropy>(g, ep, slots, st);
+  else
+    rc = bias ? launch_lse<EpiLseBiasEntropy, kTailBN>(g, ep, slots, st)
+              : launch_lse<EpiLseEntropy, kTailBN>(g, ep, slots, st);
   if (rc) return rc;
-  hipLaunchKernelGGL(lp_linear_join_kernel, dim3((unsigned)ceil_div(N, 4)), dim3(256), 0, st, F.pm, F.ps, L.pw, ep.splits,
+  hipLaunchKernelGGL(lp_linear_join_kernel, dim3((unsigned)ceil_div(N, 4)), dim3(256), 0, st, L.pm, L.ps, L.pw, ep.splits,
                      (long)N, H, W, bias, (int)N, (int)d, (int)V, a, F.idx, F.live, out);
   HIP_TRY(hipGetLastError());
   return CCE_OK;
