@@ -21,6 +21,7 @@
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/Exceptions.h>
@@ -814,6 +815,28 @@ auto below_autograd(F&& call) {
   return call();
 }
 
+// Refuses a backward pass that is captured into a HIP graph where a gradient goes on to
+// a node of the default stream: that is a leaf's, made before the capture and kept by
+// another graph of the same leaves.  The engine would make the default stream wait for
+// the capturing one, which a capture does not survive: its end ends the process.
+void check_capture(at::ArrayRef<Tensor> grads) {
+  for (const Tensor& grad : grads) {
+    if (!grad.defined() || !grad.is_cuda()) continue;
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const auto node = torch::autograd::get_current_node();
+    if (!node) return;
+    const c10::StreamId other = c10::hip::getDefaultHIPStream(grad.device().index()).id();
+    for (const auto& edge : node->next_edges()) {
+      if (!edge.is_valid()) continue;
+      const auto at = edge.function->stream();
+      TORCH_CHECK(!at.has_value() || at->id() != other,
+                  "a backward pass cannot be captured into a graph while another graph of the same leaves lives: drop "
+                  "the results of earlier steps, or make them on the stream that is captured");
+    }
+    return;
+  }
+}
+
 // The body of a backward: the gradients are computed without a graph of their own.
 // Where one is asked for (create_graph), they lead to what the function's inputs
 // and its incoming gradients came from, through a node that raises.  Without it
@@ -821,6 +844,7 @@ auto below_autograd(F&& call) {
 // of strided rows), and a penalty on them would be left out without a word.
 template <typename F>
 variable_list gradients(at::ArrayRef<Tensor> grads, F&& compute) {
+  check_capture(grads);
   const bool twice = at::GradMode::is_enabled();
   variable_list out;
   {
@@ -1005,12 +1029,15 @@ variable_list logprobs_results(AutogradContext* ctx, const FiveTensors& r, const
 
 // Tokens are contiguous [N].
 struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, double temperature,
-                               int64_t top_k, int64_t ignore_index) {
+  static const auto& op() {
     static const auto fwd =
         find<FiveTensors(const Tensor&, const Tensor&, double, SymInt, SymInt)>("chronicals_hip::token_logprobs_fwd");
+    return fwd;
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, double temperature,
+                               int64_t top_k, int64_t ignore_index) {
     const Tensor x = as_rows(logits);
-    const FiveTensors r = below_autograd([&] { return fwd.call(x, tokens, temperature, top_k, ignore_index); });
+    const FiveTensors r = below_autograd([&] { return op().call(x, tokens, temperature, top_k, ignore_index); });
     ctx->save_for_backward({x, tokens, std::get<2>(r)});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["ignore_index"] = ignore_index;
@@ -1036,28 +1063,56 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
   }
 };
 
+// t of another type; a call of torch's less where it has that one.
+Tensor as_type(const Tensor& t, at::ScalarType type) { return t.scalar_type() == type ? t : t.to(type); }
+
+// Whether a call is recorded for a backward.  One that is not goes to its operator as
+// it is, without an autograd function's node (1 us of 7); the dispatcher's autograd
+// step then refuses what the function would (forward-mode tensors).
+bool recorded(const Tensor& a, const optional<Tensor>& b = std::nullopt, const optional<Tensor>& c = std::nullopt) {
+  auto one = [](const optional<Tensor>& t) { return t.has_value() && t->requires_grad(); };
+  return at::GradMode::is_enabled() && (a.requires_grad() || one(b) || one(c));
+}
+
+// The results of a forward that is not recorded.
+FourTensors plain_results(const FiveTensors& r, const Tensor& x) {
+  return {shaped_rows(std::get<0>(r), x), shaped_rows(std::get<1>(r), x), shaped_rows(std::get<3>(r), x),
+          shaped_rows(std::get<4>(r), x)};
+}
+
 FourTensors token_logprobs(const Tensor& logits, const Tensor& tokens, double temperature, int64_t top_k,
                            int64_t ignore_index) {
+  if (!recorded(logits))
+    return plain_results(TokenLogprobs::op().call(as_rows(logits), tokens, temperature, top_k, ignore_index), logits);
   const auto r = TokenLogprobs::apply(logits, tokens, temperature, top_k, ignore_index);
   return {r[0], r[1], r[2], r[3]};
 }
 
+// fp16 and fp32 operands of the head are rounded to bf16, the GEMMs' type.
+Tensor head_rows(const Tensor& hidden) { return as_type(as_rows(hidden), at::kBFloat16).contiguous(); }
+Tensor head_weight(const Tensor& weight) { return as_type(weight, at::kBFloat16).contiguous(); }
+Tensor head_bias(const optional<Tensor>& bias) {
+  return bias.has_value() ? as_type(*bias, at::kFloat).contiguous() : Tensor();
+}
+
 struct LinearTokenLogprobs : torch::autograd::Function<LinearTokenLogprobs> {
+  static const auto& op() {
+    static const auto fwd = find<FiveTensors(const Tensor&, const Tensor&, const optional<Tensor>&, const Tensor&, double,
+                                             SymInt, SymInt)>("chronicals_hip::linear_token_logprobs_fwd");
+    return fwd;
+  }
   static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight,
                                const optional<Tensor>& bias, const Tensor& tokens, int64_t chunk_size, double temperature,
                                int64_t top_k, int64_t ignore_index) {
-    static const auto fwd = find<FiveTensors(const Tensor&, const Tensor&, const optional<Tensor>&, const Tensor&, double,
-                                             SymInt, SymInt)>("chronicals_hip::linear_token_logprobs_fwd");
-    // fp16 and fp32 operands are rounded to bf16, the GEMMs' type
-    const Tensor h = as_rows(hidden).to(at::kBFloat16).contiguous(), w = weight.to(at::kBFloat16).contiguous();
-    const Tensor b = bias.has_value() ? bias->to(at::kFloat).contiguous() : Tensor();
+    const Tensor h = head_rows(hidden), w = head_weight(weight), b = head_bias(bias);
     const FiveTensors r =
-        below_autograd([&] { return fwd.call(h, w, given(b), tokens, temperature, top_k, ignore_index); });
+        below_autograd([&] { return op().call(h, w, given(b), tokens, temperature, top_k, ignore_index); });
     ctx->save_for_backward({h, w, b, tokens, std::get<2>(r)});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["ignore_index"] = ignore_index;
     ctx->saved_data["chunk_size"] = chunk_size;
-    ctx->saved_data["shape"] = hidden.sym_sizes();
+    if (hidden.dim() != 2) ctx->saved_data["shape"] = hidden.sym_sizes();
+    ctx->saved_data["dim"] = hidden.dim();
     ctx->saved_data["hidden"] = (int64_t)hidden.scalar_type();
     ctx->saved_data["weight"] = (int64_t)weight.scalar_type();
     if (bias.has_value()) ctx->saved_data["bias"] = (int64_t)bias->scalar_type();
@@ -1082,9 +1137,10 @@ struct LinearTokenLogprobs : torch::autograd::Function<LinearTokenLogprobs> {
                         kept["temperature"].toDouble(), kept["ignore_index"].toInt(), kept["chunk_size"].toInt(), need_dh,
                         need_dw, need_db, htype != at::kBFloat16, wtype != at::kBFloat16);
       });
-      if (need_dh) out[0] = dh.view_symint(kept["shape"].toSymIntVector()).to(htype);
-      if (need_dw) out[1] = dw.to(wtype);
-      if (need_db) out[2] = db.to((at::ScalarType)kept["bias"].toInt());
+      if (need_dh)
+        out[0] = as_type(kept["dim"].toInt() == 2 ? dh : dh.view_symint(kept["shape"].toSymIntVector()), htype);
+      if (need_dw) out[1] = as_type(dw, wtype);
+      if (need_db) out[2] = as_type(db, (at::ScalarType)kept["bias"].toInt());
       return out;
     });
   }
@@ -1093,24 +1149,33 @@ struct LinearTokenLogprobs : torch::autograd::Function<LinearTokenLogprobs> {
 FourTensors linear_token_logprobs(const Tensor& hidden, const Tensor& weight, const optional<Tensor>& bias,
                                   const Tensor& tokens, int64_t chunk_size, double temperature, int64_t top_k,
                                   int64_t ignore_index) {
+  if (!recorded(hidden, weight, bias))
+    return plain_results(LinearTokenLogprobs::op().call(head_rows(hidden), head_weight(weight), given(head_bias(bias)),
+                                                        tokens, temperature, top_k, ignore_index),
+                         hidden);
   const auto r =
       LinearTokenLogprobs::apply(hidden, weight, bias, tokens, chunk_size, temperature, top_k, ignore_index);
   return {r[0], r[1], r[2], r[3]};
 }
 
 struct RmsNorm : torch::autograd::Function<RmsNorm> {
-  // y and the sum, which is empty without a residual
-  static variable_list forward(AutogradContext* ctx, const Tensor& x, const optional<Tensor>& weight,
-                               const optional<Tensor>& residual, double eps) {
+  static const auto& op() {
     static const auto fwd = find<std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const optional<Tensor>&,
                                                                     const optional<Tensor>&, double)>(
         "chronicals_hip::rms_norm_fwd");
+    return fwd;
+  }
+  static Tensor shaped(const Tensor& t, const Tensor& x) {
+    return x.dim() == 2 ? t : at::_unsafe_view_symint(t, x.sym_sizes());
+  }
+  // y and the sum, which is empty without a residual
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const optional<Tensor>& weight,
+                               const optional<Tensor>& residual, double eps) {
     const Tensor rows = as_rows(x);
     const bool has_r = residual.has_value();
     const optional<Tensor> r = has_r ? optional<Tensor>(as_rows(*residual)) : residual;
-    const auto [y, sum, rstd] = below_autograd([&] { return fwd.call(rows, weight, r, eps); });
-    auto shaped = [&](const Tensor& t) { return x.dim() == 2 ? t : at::_unsafe_view_symint(t, x.sym_sizes()); };
-    variable_list out = {shaped(y), has_r ? shaped(sum) : sum};
+    const auto [y, sum, rstd] = below_autograd([&] { return op().call(rows, weight, r, eps); });
+    variable_list out = {shaped(y, x), has_r ? shaped(sum, x) : sum};
     ctx->save_for_backward({has_r ? out[1] : rows, weight.value_or(Tensor()), rstd});
     ctx->saved_data["residual"] = has_r;
     ctx->saved_data["same"] = has_r && residual->scalar_type() == x.scalar_type();
@@ -1131,9 +1196,11 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
                need_r = has_r && ctx->needs_input_grad(has_w ? 2 : 1);
     if ((!need_x && !need_dw && !need_r) || (!grads[0].defined() && !grads[1].defined())) return variable_list(4);
     return gradients({grads[0], grads[1]}, [&]() -> variable_list {
-      const Tensor& shaped = grads[0].defined() ? grads[0] : grads[1];
+      const Tensor& like = grads[0].defined() ? grads[0] : grads[1];
       const Tensor sum = as_rows(saved[0]);
-      auto rows = [&](const Tensor& t) { return t.reshape_symint(sum.sym_sizes()).contiguous(); };
+      auto rows = [&](const Tensor& t) {
+        return (t.dim() == 2 ? t : t.reshape_symint(sum.sym_sizes())).contiguous();
+      };
       const Tensor g = grads[0].defined()
                            ? rows(grads[0])
                            : at::zeros_symint(sum.sym_sizes(), sum.options().dtype((at::ScalarType)kept["x"].toInt()));
@@ -1142,7 +1209,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
         return bwd.call(g, gs, sum, given(saved[1]), saved[2], has_w && saved[1].scalar_type() == at::kFloat,
                         need_x || (need_r && same), need_r && !same, need_dw);
       });
-      auto out = [&](const Tensor& t) { return t.view_symint(shaped.sym_sizes()); };
+      auto out = [&](const Tensor& t) { return like.dim() == 2 ? t : t.view_symint(like.sym_sizes()); };
       // of one type the two gradients are one
       return {need_x ? out(dx) : Tensor(), need_dw ? dw : Tensor(), need_r ? out(same ? dx : dr) : Tensor(), Tensor()};
     });
@@ -1151,6 +1218,11 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
 
 std::tuple<Tensor, Tensor> rms_norm(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& residual,
                                     double eps) {
+  if (!recorded(x, weight, residual)) {
+    const auto [y, sum, rstd] = RmsNorm::op().call(
+        as_rows(x), contiguous(weight), residual.has_value() ? optional<Tensor>(as_rows(*residual)) : residual, eps);
+    return {RmsNorm::shaped(y, x), residual.has_value() ? RmsNorm::shaped(sum, x) : sum};
+  }
   const auto r = RmsNorm::apply(x, contiguous(weight), residual, eps);
   return {r[0], r[1]};
 }

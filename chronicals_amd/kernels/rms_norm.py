@@ -84,7 +84,9 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: O
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """[..., D] as [N, D] with a contiguous last dimension and rows that do not overlap."""
-    r = t.detach().reshape(-1, t.shape[-1])
+    r = t.detach() if t.requires_grad else t
+    if r.dim() != 2:
+        r = r.reshape(-1, t.shape[-1])
     if (r.shape[1] > 1 and r.stride(1) != 1) or (r.shape[0] > 1 and r.stride(0) < r.shape[1]):
         r = r.contiguous()
     return r
@@ -104,11 +106,14 @@ def rms_norm_quantized(x: torch.Tensor, weight: Optional[torch.Tensor] = None, r
         raise ValueError(f"dtype must be torch.float8_e4m3fn or torch.int8, got {dtype}")
     if group_size is not None and group_size not in _GROUPS:
         raise ValueError(f"group_size must be None or one of {_GROUPS}, got {group_size}")
-    q, scales, s = _rms_norm_quantized(_rows(x), None if weight is None else weight.detach().contiguous(),
-                                       None if residual is None else _rows(residual), eps, dtype == torch.int8,
-                                       group_size or 0)
-    q, scales = q.view(x.shape), scales.view((*x.shape[:-1], *scales.shape[1:]))
-    return (q, scales) if residual is None else (q, scales, s.view(x.shape))
+    if weight is not None:
+        weight = (weight.detach() if weight.requires_grad else weight).contiguous()
+    q, scales, s = _rms_norm_quantized(_rows(x), weight, None if residual is None else _rows(residual), eps,
+                                       dtype == torch.int8, group_size or 0)
+    if x.dim() != 2:
+        q, scales = q.view(x.shape), scales.view((*x.shape[:-1], *scales.shape[1:]))
+        s = s if residual is None else s.view(x.shape)
+    return (q, scales) if residual is None else (q, scales, s)
 
 
 class RMSNorm(nn.Module):

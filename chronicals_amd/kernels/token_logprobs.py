@@ -75,7 +75,7 @@ def _check(x: torch.Tensor, tokens: torch.Tensor, V: int, temperature: float, to
         raise ValueError(f"temperature must be in [0.01, 1000], got {temperature}")
     if not 0 <= top_k <= min(V, MAX_ENTRIES):
         raise ValueError(f"top_k must be in [0, min({MAX_ENTRIES}, V = {V})], got {top_k}")
-    return tokens.reshape(-1).contiguous()
+    return (tokens if tokens.dim() == 1 else tokens.reshape(-1)).contiguous()
 
 
 def _results(out, top_k: int) -> TokenLogprobs:
