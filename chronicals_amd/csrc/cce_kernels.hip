@@ -2432,12 +2432,16 @@ bool dh_fold(int ks) { return ks >= 4; }
 // K is split so that tiles x splits reaches about 128 workgroups, with at
 // least 8 slabs of 64 per split (more splits cost more in the fp32 partials'
 // reduction than their shorter K loops return).
-int dh_splits(long N, long d, long Vb) {
+// `alone`: no dW shares the launch, which then waits for dH: 256 workgroups where dH
+// has up to 16 tiles.  Frozen weight, backward, 128 / 256 in us: 64 x 896 x 32000 51 /
+// 47, 64 x 4096 x 32000 142 / 121, 500 x 2048 x 30000 164 / 145; but with 32 tiles,
+// 2048 x 896 x 151936, 1431 / 1634, and beside a dW 64 x 896 x 32000 65 / 71.
+int dh_splits(long N, long d, long Vb, bool alone = false) {
   if (N <= 0 || d <= 0) return 1;
   const long dmain = band_dmain(d);
   const long tiles = ceil_div(N, kBM) * (ceil_div(dmain, kBN) + (dmain < d ? 1 : 0));
   if (tiles <= 0 || tiles >= 128) return 1;
-  const long ks = std::min<long>(ceil_div(128, tiles), Vb / 512);
+  const long ks = std::min<long>(ceil_div(alone && tiles <= 16 ? 256 : 128, tiles), Vb / 512);
   return ks < 2 ? 1 : (int)ks;
 }
 
@@ -2447,7 +2451,7 @@ int dh_splits(long N, long d, long Vb) {
 long ht_cols(long N) { return (long)align_up((size_t)N, kBK); }
 
 BwdLayout bwd_layout(void* ws, long N, long d, long V, long Vb, bool need_dh, bool need_dw, bool dh_f32,
-                     bool dw_f32, int entries = -1) {  // a SparseGrad's; -1: none
+                     bool dw_f32, int entries = -1) {  // a SparseGrad's (0: token log-probabilities); -1: none
   Carver c(ws);
   BwdLayout L;
   L.N = N;
@@ -2473,7 +2477,7 @@ BwdLayout bwd_layout(void* ws, long N, long d, long V, long Vb, bool need_dh, bo
   L.idx = N > kBM ? c.take<int>((size_t)N) : nullptr;
   L.live = N > kBM ? c.take<int>(1) : nullptr;
   L.Hc = copied && !L.hc_out ? c.take<bf16_t>((size_t)N * d) : nullptr;
-  L.dh_ks = need_dh ? dh_splits(L.Nb, d, Vb) : 1;
+  L.dh_ks = need_dh ? dh_splits(L.Nb, d, Vb, entries == 0 && !need_dw) : 1;
   // a second partial buffer only when the reduction rides in the next
   // launch (dh_fold); otherwise each unit's reduction runs before the next
   // band launch writes the one buffer again

@@ -207,8 +207,8 @@ constexpr int kTopCandidates = 2048, kTopGroups = 1024;
 // workgroups per CU instead of seven.  With all but 20 columns of a row at a mask's
 // value 390 us, and by top_exact after the overflow 2510.
 //
-// Pass 1 hands every chunk to each(chunk); without a pass 1 (fewer chunks than k)
-// nothing is handed out.
+// Pass 1 hands every chunk to each(chunks), arrays of four or one; without a pass 1
+// (fewer chunks than k) nothing is handed out.
 template <typename T, typename Each>
 __device__ void top_of_row(const T* row, int V, int k, uint32_t* hist, uint16_t* groups, const TopList& list,
                            Each&& each) {
@@ -229,16 +229,14 @@ __device__ void top_of_row(const T* row, int V, int k, uint32_t* hist, uint16_t*
 #pragma unroll
           for (int u = 0; u < U; ++u) raw[u] = __builtin_nontemporal_load(body + c + u * 256);
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
-            part[r][u].add(raw[u]);
-            each(raw[u]);
-          }
+          for (int u = 0; u < U; ++u) part[r][u].add(raw[u]);
+          each(raw);
         } else {
 #pragma unroll
           for (int u = 0; u < U; ++u)
             if (c + u * 256 < sp.chunks) {
-              const u32x4 raw = body[c + u * 256];
-              part[r][u].add(raw);
+              const u32x4 raw[1] = {body[c + u * 256]};
+              part[r][u].add(raw[0]);
               each(raw);
             }
         }
@@ -372,7 +370,7 @@ __global__ __launch_bounds__(256) void top_logits_kernel(const T* __restrict__ X
   split_span(V, S, blockIdx.x % S, c0, c1);
   const T* const row = X + n * ld + c0;
   const int m = min(k, c1 - c0);
-  if (m > 0) top_of_row(row, c1 - c0, m, hist, groups, list, [](const u32x4&) {});
+  if (m > 0) top_of_row(row, c1 - c0, m, hist, groups, list, [](const auto&) {});
   if (S == 1) {
     top_ranked(list, k, [&](int rank, uint64_t c) {
       values[n * k + rank] = row[column(c)];

@@ -816,8 +816,8 @@ auto below_autograd(F&& call) {
 }
 
 // Refuses a backward pass that is captured into a HIP graph where a gradient goes on to
-// a node of the default stream: that is a leaf's, made before the capture and kept by
-// another graph of the same leaves.  The engine would make the default stream wait for
+// a node of the default stream: a leaf's, made before the capture and kept by another
+// graph of the same leaves.  The engine would make the default stream wait for
 // the capturing one, which a capture does not survive: its end ends the process.
 void check_capture(at::ArrayRef<Tensor> grads) {
   for (const Tensor& grad : grads) {
@@ -826,9 +826,9 @@ void check_capture(at::ArrayRef<Tensor> grads) {
     const auto node = torch::autograd::get_current_node();
     if (!node) return;
     const c10::StreamId other = c10::hip::getDefaultHIPStream(grad.device().index()).id();
-    for (const auto& edge : node->next_edges()) {
-      if (!edge.is_valid()) continue;
-      const auto at = edge.function->stream();
+    for (size_t i = 0; i < node->num_outputs(); ++i) {
+      if (!node->task_should_compute_output(i)) continue;  // not asked for: nothing goes there
+      const auto at = node->next_edge(i).function->stream();
       TORCH_CHECK(!at.has_value() || at->id() != other,
                   "a backward pass cannot be captured into a graph while another graph of the same leaves lives: drop "
                   "the results of earlier steps, or make them on the stream that is captured");

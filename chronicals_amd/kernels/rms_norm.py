@@ -25,8 +25,8 @@ group's) scale a NaN.
   * The results may be changed in place, s only where no backward needs it.  Gradients
     are kernels' results: differentiating them again raises an error.
 
-The reference's norm without a residual is triton_kernels.py:2224 (``rmsnorm``), its
-activations in 8 bits have a scale per 128 columns (fp8_deepseek.py:512-706).
+The reference's norm, without a residual, is triton_kernels.py:2224 (``rmsnorm``); it
+quantizes activations in blocks in kernels of their own (fp8_deepseek.py:512-706).
 """
 from __future__ import annotations
 

@@ -37,7 +37,8 @@ Per row, with z = x / temperature and p = softmax(z):
     to bf16 once, in units that hold the largest token's share of it exactly; gradients
     come back in the input dtypes.
 
-``-logprobs`` at temperature 1 is ``cut_cross_entropy``'s loss with reduction 'none'.
+For a token in [0, V) ``-logprobs`` at temperature 1 is the loss of ``cut_cross_entropy``
+with reduction 'none'.  Logits that are NaN or +inf make their row's results NaN.
 The reference has no counterpart; the argument order follows its losses.
 """
 from __future__ import annotations

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from tests.distill_common import DTYPES, EXP_ERR, IGNORE, close, half_step
+from tests.distill_common import DTYPES, EXP_ERR, EXP_LEAST, IGNORE, close, half_step
 from tests.logprobs_common import Reference, tokens
 
 pytestmark = pytest.mark.gpu
@@ -293,6 +293,11 @@ def check_linear(gpu, h, w, tok, bias=None, T=1.0, k=0, frozen=False, chunk_size
     # exponentials and by the logits' own error; products add fp32 rounding
     G, M = ref.grad, ref.mag
     e = 2.0 ** -8 * G.abs() * (1 + 2.0 ** -7) + (2 * EXP_ERR + 2 * off * (1 + ref.entropy[:, None])) * M
+    # What is below 2^-126 may be lost: of a power of two, before its coefficient
+    # (|g| + |h| (1000 + H)) / T at most (the exponent counts from -1000 up), and of G in
+    # its unit, which is below 2.  At a low temperature columns have such gradients
+    # alone: 0 came out for -1.1e-39.
+    e = e + EXP_LEAST * (((g.abs() + gh.abs() * (1000 + ref.entropy)) / T)[:, None] + 2)
     acc = (max(h.shape[0], w.shape[0]) + 64) * 2.0 ** -24
     wants = [(hg, G @ wd, (e + acc * M) @ wd.abs())]
     if not frozen:
@@ -317,6 +322,11 @@ LINEAR = [
     (300, 1000, 600, 1.0, False, False, 8192),
     (700, 64, 1500, 1.5, False, True, 512),
     (700, 64, 1500, 0.5, True, False, 8192),
+    (64, 128, 5003, 0.05, True, False, 8192),
+    (9, 64, 32768, 1.0, False, False, 8192),   # one round of half-width tiles, exactly
+    (9, 64, 32769, 1.0, True, False, 8192),    # whole tiles
+    (20, 72, 33000, 1.0, False, True, 8192),   # dH alone, over many splits
+    (300, 128, 12000, 0.8, False, True, 8192),
 ]
 
 
