@@ -35,7 +35,9 @@ Per row, with z = x / temperature and p = softmax(z):
   * ``linear_token_logprobs`` computes in bf16 with fp32 accumulation (fp16 and fp32
     operands are rounded to bf16 at the boundary) and rounds the gradient of the logits
     to bf16 once, in units that hold the largest token's share of it exactly; gradients
-    come back in the input dtypes.
+    come back in the input dtypes.  The token's logit is a dot product beside the one of
+    the sums: the order of the additions, some 2^-24 of a logit's terms, is left even in
+    rows that are sure of their token (3e-6 of -0.3 under logits of 15).
 
 For a token in [0, V) ``-logprobs`` at temperature 1 is the loss of ``cut_cross_entropy``
 with reduction 'none'.  Logits that are NaN or +inf make their row's results NaN.
