@@ -550,6 +550,57 @@ def test_offsets_past_32_bits(gpu):
     assert not dx[:-2].any()
 
 
+def test_shared_and_broadcast_leaves(gpu):
+    """A head that two calls share, one row for many tokens, a transposed head: each gradient is the sum of the parts'."""
+    t = entry_points()
+    g = torch.Generator().manual_seed(28)
+    h, w = (v.to(gpu) for v in head(g, 12, 64, 2000))
+    tok = tokens(g, 12, 2000).to(gpu)
+    parts = []
+    for rows in (slice(0, 5), slice(5, 12)):
+        wl = w.clone().requires_grad_(True)
+        t.linear_token_logprobs(h[rows], wl, tok[rows]).logprobs.sum().backward()
+        parts.append(wl.grad)
+    wl = w.clone().requires_grad_(True)
+    sum(t.linear_token_logprobs(h[r], wl, tok[r]).logprobs.sum() for r in (slice(0, 5), slice(5, 12))).backward()
+    assert torch.equal(wl.grad, parts[0] + parts[1])
+
+    wt = w.t().contiguous().requires_grad_(True)
+    t.linear_token_logprobs(h[:5], wt.t(), tok[:5]).logprobs.sum().backward()
+    assert torch.equal(wt.grad.t(), parts[0])
+
+    for f, row in ((lambda x: t.linear_token_logprobs(x, w, tok, top_k=2), h[:1]),
+                   (lambda x: t.token_logprobs(x, tok, top_k=2), torch.randn(1, 2000, generator=g).to(gpu))):
+        one, many = row.clone().requires_grad_(True), row.repeat(12, 1).requires_grad_(True)
+        a, b = f(one.expand(12, -1)), f(many)
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+        (a.logprobs.sum() + a.entropy.sum()).backward()
+        (b.logprobs.sum() + b.entropy.sum()).backward()
+        assert torch.equal(one.grad, many.grad.sum(0, keepdim=True))
+
+
+def test_one_hidden_vector(gpu):
+    """Results without a dimension for the rows, and the gradient of a vector."""
+    t = entry_points()
+    g = torch.Generator().manual_seed(29)
+    h, w, _ = exact_head(g, 1, 64, 500)
+    x, tok = h.double() @ w.double().t(), torch.tensor([499])
+    ref = Reference(x, tok, 1.0, torch.ones(1))
+    for k in (0, 3):
+        hg = h[0].to(gpu).requires_grad_(True)
+        out = t.linear_token_logprobs(hg, w.to(gpu), tok[0].to(gpu), top_k=k)
+        assert out.logprobs.shape == out.entropy.shape == ()
+        close(out.logprobs, ref.logprobs[0], ref.tol[0])  # the logits are exact
+        close(out.entropy, ref.entropy[0], ref.tol[0])
+        if k:
+            assert out.top_logprobs.shape == (k,) and torch.equal(out.top_indices.cpu(), ref.top(x, k)[1][0])
+        out.logprobs.backward()
+        # half a step of bf16 of G's elements and of the result; 500 products in fp32
+        want, parts = (ref.grad @ w.double())[0], (ref.mag @ w.double().abs())[0]
+        err = 2.0 ** -8 * (1 + 2.0 ** -7) * (ref.grad.abs() @ w.double().abs())[0] + (2 * EXP_ERR + 564 * 2.0 ** -24) * parts
+        close(hg.grad, want, 2.0 ** -8 * want.abs() * (1 + 2.0 ** -7) + err * (1 + 2.0 ** -8) + half_step(torch.bfloat16)[1])
+
+
 def test_grad_modes(gpu):
     t = entry_points()
     g = torch.Generator().manual_seed(22)
