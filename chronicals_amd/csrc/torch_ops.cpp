@@ -1210,8 +1210,11 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
                         need_x || (need_r && same), need_r && !same, need_dw);
       });
       auto out = [&](const Tensor& t) { return like.dim() == 2 ? t : t.view_symint(like.sym_sizes()); };
-      // of one type the two gradients are one
-      return {need_x ? out(dx) : Tensor(), need_dw ? dw : Tensor(), need_r ? out(same ? dx : dr) : Tensor(), Tensor()};
+      // Of one type the two gradients are one tensor, as an addition's are.  It has to be one
+      // object: its two owners are how the engine knows that a leaf's .grad needs a copy (two
+      // views of one storage would each pass for a tensor that nobody else has).
+      const Tensor gx = need_x || (need_r && same) ? out(dx) : Tensor();
+      return {need_x ? gx : Tensor(), need_dw ? dw : Tensor(), need_r ? (same ? gx : out(dr)) : Tensor(), Tensor()};
     });
   }
 };

@@ -24,6 +24,9 @@ group's) scale a NaN.
     copied).  weight is [D], of x's dtype or fp32.
   * The results may be changed in place, s only where no backward needs it.  Gradients
     are kernels' results: differentiating them again raises an error.
+  * x and a residual of its dtype have one gradient: ``torch.autograd.grad`` returns the
+    same tensor for both, as for ``x + residual``; leaves' ``.grad`` are tensors of their
+    own.
 
 The reference's norm, without a residual, is triton_kernels.py:2224 (``rmsnorm``); it
 quantizes activations in blocks in kernels of their own (fp8_deepseek.py:512-706).
