@@ -858,10 +858,17 @@ variable_list gradients(at::ArrayRef<Tensor> grads, F&& compute) {
     if (grad.defined() && grad.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(grad));
   const auto error = std::make_shared<torch::autograd::Error>(
       "the gradients of chronicals_hip operators cannot be differentiated again", std::move(edges));
-  for (Tensor& t : out) {
-    if (!t.defined()) continue;
-    t = t.tensor_data();  // no view: it gets a graph
-    torch::autograd::set_history(t, error);
+  const variable_list plain = out;
+  for (size_t i = 0; i < out.size(); ++i) {
+    if (!out[i].defined()) continue;
+    size_t first = 0;
+    while (!plain[first].is_same(plain[i])) ++first;
+    if (first < i) {  // what was one tensor stays one
+      out[i] = out[first];
+      continue;
+    }
+    out[i] = plain[i].tensor_data();  // no view: it gets a graph
+    torch::autograd::set_history(out[i], error);
   }
   return out;
 }

@@ -60,3 +60,19 @@ def test_the_others(shape):
     h.grad = w.grad = b.grad = None
     ops.distill_linear(h, w, b, meta(n, 5), meta(n, 5, dtype=torch.int64), None, 8192, 1.0, 1.0, 0.0, -100, 1).backward()
     assert apart([h, w, b])
+
+
+@pytest.mark.filterwarnings("ignore:Using backward")
+@pytest.mark.parametrize("shape", SHAPES)
+def test_rms_norm_of_one_type_as_an_addition(shape):
+    """Asked for by torch.autograd.grad, the gradients of x and of a residual of its type are one tensor, as those of
+    x + residual are: nothing that looks like two."""
+    for twice in (False, True):
+        x, r = leaf(*shape), leaf(*shape)
+        y, s = ops.rms_norm(x, None, r, 1e-6)
+        gx, gr = torch.autograd.grad(y.sum() + s.sum(), [x, r], create_graph=twice)
+        assert gx is gr and gx.requires_grad == twice
+        y, s = ops.rms_norm(x, None, r, 1e-6)
+        (y.sum() + s.sum()).backward(create_graph=twice)
+        assert apart([x, r])
+        x.grad = r.grad = None
