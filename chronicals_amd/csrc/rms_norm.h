@@ -5,7 +5,7 @@
 //   a = dy * w;  ds' = rstd * (a - n * sum(a * n) / D) + ds;  dx = dr = ds'
 //   dw = sum over rows of dy * n
 //   8 bits: scale = max(amax(|y|), 1e-30) / M over a row or a group of its columns,
-//   q = round(y / scale), M = 448 (e4m3) or 127 (int8)
+//   q = round(y / scale), M = 448 (e4m3) or 127 (int8), y and the quotient in fp32
 //
 // s is rounded to the residual's type first, and what is normalised is the rounded
 // one: it is what the caller keeps as the stream, what the backward reads, and what a
@@ -18,8 +18,8 @@
 // Bound by HBM.  bf16 with a bf16 residual, forward / backward with both gradients and
 // the join of its parts (TB/s of what has to move; a large copy reaches 4.8): 16384 x
 // 896 24 / 29 us (4.9 / 4.1), 65536 x 896 81 / 88 (5.8 / 5.3), 8192 x 4096 48 / 53 (5.6 /
-// 5.1), fp32 91 / 92 (5.9 / 5.8).  In 8 bits 8192 x 3584 39 us (5.2), by rows and by
-// groups of 128 alike.  The backward without the next row's loads ahead: 16384 x 896 35.
+// 5.1), fp32 91 / 92 (5.9 / 5.8).  In 8 bits 8192 x 3584 40 to 42 us (5.0), by rows
+// and by groups of 128 alike.  The backward without the next row's loads ahead: 16384 x 896 35.
 
 // A row of type S on its way, in the chunks that RowRegs<T, TR, C> holds: 16 bytes of
 // T, so fp32 beside a 16-bit T takes two loads a chunk.
@@ -107,11 +107,31 @@ __device__ inline float quant_scale(const RmsQuant& o, uint32_t amax) {
   const float a = __uint_as_float(amax);
   return (a < 1e-30f ? 1e-30f : a) / (o.int8 ? 127.f : 448.f);
 }
+
+// Quotients by a scale, from its reciprocal r and what that lacks, e = 1 - r scale (exact):
+// v / scale = v r / (1 - e) is rounded once, from a value that is off by at most 2^-22 of
+// a step of fp32 (e^2, and u's rounding).  v r alone is off by up to 1.5 steps, which takes
+// values beside a midpoint of the 8-bit type to the wrong code.  8192 x 3584 bf16 into e4m3
+// with a scale per row: v r alone 41 us, this 42, the compiler's division 47.
+struct Quotient {
+  float r, e;
+  __device__ inline explicit Quotient(float scale) {
+    r = 1.f / scale;
+    // an infinite scale takes finite values to 0
+    e = scale < INFINITY ? __builtin_fmaf(-r, scale, 1.f) : 0.f;
+  }
+  __device__ inline float of(float v) const {
+    const float u = v * r * e;
+    return __builtin_fmaf(v, r, u);
+  }
+};
+
 __device__ inline uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// Four values over their scale, rounded to nearest even: |v| is at most M and a few
-// 2^-24 of it, which round to M in either type (e4m3's midpoint above 448 is 464).
-__device__ inline uint32_t quant4(const RmsQuant& o, float a, float b, float c, float d) {
+// Four values over their scale, rounded to nearest even: the quotients are at most M and
+// a few 2^-24 of it, which round to M in either type (e4m3's midpoint above 448 is 464).
+__device__ inline uint32_t quant4(const RmsQuant& o, const Quotient& by, const float* v) {
+  const float a = by.of(v[0]), b = by.of(v[1]), c = by.of(v[2]), d = by.of(v[3]);
   if (o.int8) {
     // within the type also where a NaN has no integer (its group's scale is a NaN)
     auto whole = [](float v) { return (uint32_t)(int)rintf(__builtin_amdgcn_fmed3f(v, -127.f, 127.f)) & 255u; };
@@ -204,12 +224,12 @@ __global__ __launch_bounds__(TR < 256 ? 256 : TR) void rms_fwd_rows_kernel(
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         const int at = Row::first(c, t);
-        const float scale = quant_scale(o, o.group ? mx[c] : all), by = 1.f / scale;
+        const float scale = quant_scale(o, o.group ? mx[c] : all);
+        const Quotient by(scale);
         if (o.starts(at) && at < D) o.scales[o.place(n, at)] = scale;
         uint32_t b[E / 4];
 #pragma unroll
-        for (int i = 0; i < E; i += 4)
-          b[i / 4] = quant4(o, v[c][i] * by, v[c][i + 1] * by, v[c][i + 2] * by, v[c][i + 3] * by);
+        for (int i = 0; i < E; i += 4) b[i / 4] = quant4(o, by, &v[c][i]);
         if (at + E <= D) {
           if constexpr (E == 8)
             *reinterpret_cast<u32x2_any*>(row + at) = u32x2_any{b[0], b[1]};
@@ -376,11 +396,12 @@ __global__ __launch_bounds__(256) void rms_fwd_kernel(const T* __restrict__ X, l
         mx = max(mx, magnitude(v[i]));
       }
       if (o.group) mx = lanes_max(mx, o.group / 8);
-      const float scale = quant_scale(o, o.group ? mx : all), by = 1.f / scale;
+      const float scale = quant_scale(o, o.group ? mx : all);
+      const Quotient by(scale);
       if (o.starts(c) && c < D) o.scales[o.place(n, c)] = scale;
 #pragma unroll
       for (int i = 0; i < 8; i += 4) {
-        const uint32_t b = quant4(o, v[i] * by, v[i + 1] * by, v[i + 2] * by, v[i + 3] * by);
+        const uint32_t b = quant4(o, by, &v[i]);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           if (c + i + k < D) o.q[n * D + c + i + k] = (uint8_t)(b >> (k * 8));

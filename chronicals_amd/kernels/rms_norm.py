@@ -15,7 +15,7 @@ fixed order: the same bits on every run) to the weight's type.
 ``rms_norm_quantized`` writes y in 8 bits, e4m3 (``torch.float8_e4m3fn``) or int8, with
 fp32 scales per row or per ``group_size`` columns:
   scale = max(largest |y|, 1e-30) / M, M = 448 or 127;  q = round(y / scale) to nearest even
-so that ``q * scale`` stands for y.  It has no gradient.  A NaN makes its row's (its
+(y, the scale and the quotient in fp32) so that ``q * scale`` stands for y.  It has no gradient.  A NaN makes its row's (its
 group's) scale a NaN.
 
   * Tensors must live on a HIP device; there is no CPU path.

@@ -422,7 +422,7 @@ int cce_linear_token_logprobs_backward(const float* grad_logprobs, const float* 
  * The quantized form writes y in 8 bits, with a scale per row (group 0, scales_out [N])
  * or per `group` columns (32, 64, 128 or 256; scales_out [N][ceil(D / group)]):
  *   scale = max(largest |y|, 1e-30) / M,  q = round(y / scale) to nearest even,
- *   M = 448 (CCE_DTYPE_E4M3) or 127 (CCE_DTYPE_INT8)
+ *   M = 448 (CCE_DTYPE_E4M3) or 127 (CCE_DTYPE_INT8), y and the quotient in fp32
  * A NaN in a group makes its scale a NaN.
  *
  * The backward takes the gradients of y and (NULL: none) of sum, and sum itself: without
