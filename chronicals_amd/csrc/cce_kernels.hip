@@ -1158,13 +1158,6 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(1, 1))
 // at d = 4096 (8192 rows), and the copies and their memory are gone.  With dH split over K on very
 // few rows, the previous band's partials are reduced by the last population.
 
-// dH of one band split over the band's K (few row tiles): the ks fp32
-// partials P[k] = P + k * stride ([rows][d], GEMM row order) of each live row
-// are summed in fixed order and applied with the band's accumulator mode, as
-// the GEMM epilogue applies an unsplit tile: 0 out = s, 1 acc = s,
-// 2 acc += s, 3 out = acc + s, 4 out += s (fp32 out); out rows go through the
-// row map.  The rows are a block starting at row live_base of the compacted
-// order (P, acc and rowmap point at the block).
 // A block of logits in fp32: out = C, with HB plus the columns' bias.  The output's
 // rows hold whole fours of columns (ldo a multiple of 4, N or more); those past N get
 // numbers of no meaning.  Stored in whole rows of a wave's columns, as EpiAccT's.
@@ -1223,6 +1216,13 @@ using EpiOut = EpiOutT<BN, false>;
 template <int BN>
 using EpiOutBias = EpiOutT<BN, true>;
 
+// dH of one band split over the band's K (few row tiles): the ks fp32
+// partials P[k] = P + k * stride ([rows][d], GEMM row order) of each live row
+// are summed in fixed order and applied with the band's accumulator mode, as
+// the GEMM epilogue applies an unsplit tile: 0 out = s, 1 acc = s,
+// 2 acc += s, 3 out = acc + s, 4 out += s (fp32 out); out rows go through the
+// row map.  The rows are a block starting at row live_base of the compacted
+// order (P, acc and rowmap point at the block).
 struct DhReduce {
   const float* P;
   long stride;

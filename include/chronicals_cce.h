@@ -428,7 +428,9 @@ int cce_linear_token_logprobs_backward(const float* grad_logprobs, const float* 
  * The backward takes the gradients of y and (NULL: none) of sum, and sum itself: without
  * a residual that is x.  grad_x and grad_residual are the same numbers in the dtypes of
  * x and of sum; NULL leaves one out, and grad_weight.  The workspace is what the query
- * gives (0 bytes, which may be NULL, without grad_weight).  No reference counterpart.
+ * gives (0 bytes, which may be NULL, without grad_weight).  The reference's norm, without a
+ * residual, is triton_kernels.py:2224; it quantizes in kernels of their own
+ * (fp8_deepseek.py:512-706).
  */
 int cce_rms_norm_forward(const void* x, int dtype, int64_t ldx, const void* residual, int residual_dtype, int64_t ldr,
                          const void* weight, int param_dtype, int64_t N, int64_t D, float eps, void* y_out, void* sum_out,
