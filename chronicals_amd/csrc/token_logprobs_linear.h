@@ -60,7 +60,10 @@ __global__ __launch_bounds__(256) void lp_linear_join_kernel(const float* __rest
   const bool none = s == 0.f;
   // the maximum's logit and the token's are sums in different orders: where they are
   // one, their difference may come out above 0
-  float lp = none ? -INFINITY : kLn2 * (__builtin_fmaf(x, a.scale, -m) - log2f(s));
+  const float u = __builtin_fmaf(x, a.scale, -m);
+  float lp = none ? -INFINITY : kLn2 * (u - log2f(s));
+  // a mask's lowest value: past fp32 in base 2 only
+  if (!none && u == -INFINITY) lp = x * a.inv_t;
   if (lp > 0.f) lp = 0.f;
   const float h = none ? 0.f : kLn2 * (log2f(s) - w / s);
   out.logprobs[n] = col >= 0 ? lp : 0.f;
