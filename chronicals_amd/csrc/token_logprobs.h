@@ -114,6 +114,10 @@ struct LpSums {
     }
     *this = all;
   }
+  // a row whose maximum is below the floor counts as one of -inf alone (a NaN stays)
+  __device__ inline void drop_below(float floor) {
+    if (m < floor && s == s) s = 0.f;
+  }
   __device__ inline float4 packed() const { return make_float4(m, s, w, 0.f); }
   static __device__ inline LpSums of(float4 p) {
     LpSums k;
@@ -132,6 +136,7 @@ struct LpOut {
   float stat_scale;
   float* top_logprobs;  // [N][k]
   int64_t* top_indices;
+  float floor = -INFINITY;  // with alternatives: LpSums::drop_below
 };
 
 // The row's results, by one thread.  x: the token's logit, where it has one (col >= 0).
@@ -268,6 +273,7 @@ __global__ __launch_bounds__(256) void lp_top_kernel(const T* __restrict__ X, lo
   }
   sums.merge_block(a.scale, red);
   if (S == 1) {
+    sums.drop_below(out.floor);
     const float log_s = logf(sums.s);
     top_ranked(list, k, [&](int rank, uint64_t c) {
       out.top_logprobs[n * k + rank] = lp_alternative(a, sums, log_s, elem_to_f32(row[column(c)]));
@@ -300,6 +306,7 @@ __global__ __launch_bounds__(256) void lp_top_join_kernel(const T* __restrict__ 
   LpSums sums;  // by every wave
   for (int s = tid & 63; s < S; s += 64) sums.merge(LpSums::of(part[i * S + s]), a.scale);
   sums.merge_wave(a.scale);
+  sums.drop_below(out.floor);
   const float log_s = logf(sums.s);
   top_join(top_part + i * S * k, S, k, [&](int rank, uint64_t c) {
     out.top_logprobs[n * k + rank] = lp_alternative(a, sums, log_s, elem_to_f32(row[column(c)]));

@@ -200,6 +200,7 @@ int lp_linear_forward_run(const bf16_t* H, const bf16_t* W, const float* bias, l
   if (k > 0) {
     const long R = logits_block(N, V), ld = logits_ld(V);
     out.stat_scale = a.scale;
+    out.floor = kLogitFloor / a.scale;  // as without alternatives
     const OutParams e = {L.logits, ld, bias};
     for (long m0 = 0; m0 < N; m0 += R) {
       const long rows = std::min(R, N - m0);

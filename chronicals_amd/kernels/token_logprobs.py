@@ -26,7 +26,10 @@ Per row, with z = x / temperature and p = softmax(z):
   * A token outside [0, V) that is not ``ignore_index`` has no log-probability: 0,
     without a gradient.  The row's entropy and alternatives are as any other's.
   * Logits of -inf have no probability and take no part; where all of a row's are,
-    its log-probabilities are -inf, its entropy 0 and its gradient 0.
+    its log-probabilities are -inf, its entropy 0 and its gradient 0.  In the linear form
+    a row whose logits over the temperature are all below -1e30 log(2) counts as such a
+    one (a bias of fp32's lowest value in every column); beside others such a column is
+    one of probability 0, whose log-probability is what fp32 holds of it.
   * top_k is at most min(V, 256), the temperature in [0.01, 1000].
   * Sums are added in a fixed order: the same bits on every run.
   * Tensors must live on a HIP device; there is no CPU path.  Results may be changed in

@@ -392,7 +392,8 @@ int cce_token_logprobs_backward(const float* grad_logprobs, const float* grad_en
  * cce_forward's and cce_backward's (the rows of hidden that do not count are finite:
  * the backward's products run over them with zero coefficients).  With top_k the logits
  * of a block of rows are in the workspace, at most 512 MiB of them (or 256 rows, if
- * that is more); without, none are stored. */
+ * that is more); without, none are stored.  A row whose logits over the temperature are
+ * all below -1e30 log(2) counts as one where every logit is -inf. */
 int cce_linear_token_logprobs_workspace_bytes(int64_t N, int64_t d, int64_t V, int64_t top_k, size_t* bytes);
 int cce_linear_token_logprobs_forward(const void* hidden, const void* weight, const float* bias, const void* tokens,
                                       int tokens_int64, int64_t N, int64_t d, int64_t V, int64_t ignore_index,

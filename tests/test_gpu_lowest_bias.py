@@ -52,3 +52,23 @@ def test_some_columns(gpu, N, V, T, k):
     else:
         # 1 / T and the product are rounded, and the logits' other terms are below 2^-90 of it
         assert ((got[0][at].double() - low).abs() <= 3 * 2.0 ** -24 * abs(low)).all()
+
+
+@pytest.mark.parametrize("k", [0, 3])
+@pytest.mark.parametrize("T", [0.05, 1.0, 2.0, 1000.0])
+@pytest.mark.parametrize("N,V", [(6, 300), (300, 1000), (3, 40000)])
+@pytest.mark.parametrize("kind", ["lowest", "low", "one"])
+def test_every_column(gpu, N, V, T, k, kind):
+    """Rows of which nothing is left: as under a bias of -inf alone, with alternatives and without."""
+    h, w, b, tok, ups = operands(N, V)
+    b[:] = {"lowest": LOW, "low": -1e34, "one": -math.inf}[kind]
+    if kind == "one":
+        b[7] = LOW
+    got, grads = run(gpu, h, w, b, tok, T, k, ups)
+    counts = tok != IGNORE
+    assert torch.equal(got[0], torch.where(counts, -math.inf, 0.0)) and not got[1].any()
+    assert not any(v.any() for v in grads)
+    if k:
+        order = [0, 1, 2] if kind != "one" else [7, 0, 1]
+        assert torch.equal(got[2], torch.where(counts, -math.inf, 0.0)[:, None].expand(N, k))
+        assert torch.equal(got[3], torch.where(counts[:, None], torch.tensor(order), -1))
