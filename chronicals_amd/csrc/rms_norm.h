@@ -349,7 +349,10 @@ __device__ inline float param_at(const void* w, int f32, int c) {
 }
 
 // Longer rows, one workgroup per row: s and its sum of squares, then (Q: the scales,
-// with the row's largest magnitude, then) the output.
+// with the row's largest magnitude, then) the output.  Element by element, each pass adding
+// x and r again: 2048 x 20000 bf16 with a bf16 residual 132 us (2.5 TB/s of what has to
+// move), in 8 bits 170 us with group scales and 238 with a row's; backward 187 us and 242
+// with dw.  Rows of 16384, in registers: 54, 53, 54; 49 and 61.
 template <typename T, typename S, bool Q>
 __global__ __launch_bounds__(256) void rms_fwd_kernel(const T* __restrict__ X, long ldx, const S* __restrict__ R, long ldr,
                                                       const void* __restrict__ w, int param_f32, int D, float eps,

@@ -131,7 +131,8 @@ int lp_prep(const SparseGrad& s, const int* idx, long N, float4* rowp, int* rowl
 // Rows of a block whose logits go through memory, with k alternatives: fp32 logits of
 // 512 MiB, whole row tiles.  k = 20 of 511 x 1000 x 50257: 77 us for the product (1.5
 // rounds of tiles, whose 103 MB of logits leave behind each tile's multiplications),
-// 34 us for the rows.
+// 34 us for the rows.  A decoding step is bound by the weight: 8 x 896 x 151936 65 us for
+// the product, 11 and 8 for the rows and their join; 8 x 4096 x 128256 209 us in all.
 constexpr long kLogitsBudget = 512L << 20;
 long logits_ld(long V) { return (long)align_up((size_t)V, 64); }
 long logits_block(long N, long V) {

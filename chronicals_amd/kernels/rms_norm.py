@@ -15,8 +15,9 @@ fixed order: the same bits on every run) to the weight's type.
 ``rms_norm_quantized`` writes y in 8 bits, e4m3 (``torch.float8_e4m3fn``) or int8, with
 fp32 scales per row or per ``group_size`` columns:
   scale = max(largest |y|, 1e-30) / M, M = 448 or 127;  q = round(y / scale) to nearest even
-(y, the scale and the quotient in fp32) so that ``q * scale`` stands for y.  It has no gradient.  A NaN makes its row's (its
-group's) scale a NaN.
+(y, the scale and the quotient in fp32), so that ``q * scale`` stands for y.  It has no
+gradient.  A NaN makes its row's (its group's) scale a NaN and an infinity makes it
+infinite; their codes stand for nothing.
 
   * Tensors must live on a HIP device; there is no CPU path.
   * x is bf16, fp16 or fp32 of any shape; the residual has its shape, and its dtype or
@@ -24,6 +25,8 @@ group's) scale a NaN.
     copied).  weight is [D], of x's dtype or fp32.
   * The results may be changed in place, s only where no backward needs it.  Gradients
     are kernels' results: differentiating them again raises an error.
+  * Squares are summed in fp32, as torch's norm does: a row whose sum passes its range
+    comes out as 0, and with eps 0 one whose squares vanish has no finite norm.
   * x and a residual of its dtype have one gradient: ``torch.autograd.grad`` returns the
     same tensor for both, as for ``x + residual``; leaves' ``.grad`` are tensors of their
     own.
