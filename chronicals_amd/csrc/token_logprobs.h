@@ -306,6 +306,10 @@ __global__ __launch_bounds__(256) void lp_top_join_kernel(const T* __restrict__ 
   LpSums sums;  // by every wave
   for (int s = tid & 63; s < S; s += 64) sums.merge(LpSums::of(part[i * S + s]), a.scale);
   sums.merge_wave(a.scale);
+  // Lane 0's for all: the lanes of a pair add their two products the other way round, of
+  // which one is rounded, and which lane writes which candidate is not the same every run
+  sums.m = __shfl(sums.m, 0);
+  sums.s = __shfl(sums.s, 0);
   sums.drop_below(out.floor);
   const float log_s = logf(sums.s);
   top_join(top_part + i * S * k, S, k, [&](int rank, uint64_t c) {
